@@ -21,6 +21,7 @@ MAX_LAYERS = 8
 TRACE_SELF_ATTN, TRACE_H_SELF, TRACE_CROSS_ATTN, TRACE_H_CROSS, TRACE_FFN, TRACE_H_FFN = 0, 1280, 2560, 3840, 5120, 10240
 TRACE_LAYER = 11520
 MAX_ENC_LAYERS = 32
+FW_F16, FW_BF16, FW_F32 = range(3)
 
 vp = c_void_p
 i64p = POINTER(c_int64)
@@ -115,6 +116,9 @@ _SIGNATURES = {
     'fw_layernorm_rows': (c_int, [vp, vp, vp, vp, c_int, c_int, c_float, vp]),
     'fw_encoder_attention': (c_int, [vp, c_int64, c_int, c_int, vp, c_int, c_int, vp, vp]),
     'fw_encoder_forward': (c_int, [POINTER(Encoder), vp]),
+    'fw_embed_scaled': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_float, c_int, vp]),
+    'fw_embed_grad': (c_int, [vp, vp, vp, c_int, c_int, c_int, c_float, c_int64, c_int, c_int, vp, c_int64, vp]),
+    'fw_embed_grad_workspace': (c_int, [c_int, c_int, i64p]),
 }
 
 _lib = None

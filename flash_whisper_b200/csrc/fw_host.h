@@ -51,6 +51,7 @@ EncodeTiledFn tensor_map_encode_fn();
 unsigned int read_decode_errors(bool clear);
 unsigned int read_logmel_errors(bool clear);
 unsigned int read_encoder_errors(bool clear);
+unsigned int read_embed_errors(bool clear);
 
 }  // namespace fw
 

@@ -45,6 +45,47 @@ def _check_cuda(t, dtype, name, what):
     _check(t.is_cuda and t.is_contiguous() and t.dtype == dtype, f'{name} must be contiguous CUDA {what}')
 
 
+_DTYPES = {torch.float16: _lib.FW_F16, torch.bfloat16: _lib.FW_BF16, torch.float32: _lib.FW_F32}
+
+
+def _check_typed(t, like, name):
+    """A contiguous CUDA tensor of like's type on like's device."""
+    if not (t.is_cuda and t.is_contiguous() and t.dtype == like.dtype and t.device == like.device):
+        raise RuntimeError(f'{name} must be contiguous CUDA {str(like.dtype)[6:]} on {like.device}')
+
+
+def _check_ints(t, n, like, name):
+    if not (t.is_cuda and t.is_contiguous() and t.dtype == torch.long and t.numel() == n and t.device == like.device):
+        raise RuntimeError(f'{name} must be contiguous CUDA int64 [{n}] on {like.device}')
+
+
+class _On:
+    """Makes `device` current for the calls within (nothing to do where it is already)."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _workspace(ws, name, sizes, device):
+    """The caller's scratch after a check of its size, or (None) scratch of the current stream."""
+    need = ctypes.c_int64(0)
+    _lib.call(name, *sizes, ctypes.byref(need))
+    if ws is None:
+        return torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+    if not (ws.is_cuda and ws.is_contiguous() and ws.dtype == torch.uint8 and ws.device == device
+            and ws.numel() >= need.value):
+        raise RuntimeError(f'ws must be contiguous CUDA uint8 on {device} of at least {need.value} bytes')
+    return ws
+
+
 class Ext:
     """Reference-compatible kernel module backed by libflashwhisper.so."""
 
@@ -260,6 +301,52 @@ class Ext:
         _check_half(vt, 'vt')
         _lib.call('fw_encoder_attention', _ptr(qkv), qkv.stride(0), int(kcol), int(vcol), _ptr(out), qkv.size(0),
                   int(heads), _ptr(vt), _stream())
+
+    # ---- whole transcripts ---------------------------------------------------------------------
+    # These take the tensors' own device, whichever is current, and its current stream. `ws` is uint8
+    # scratch of at least the matching *_workspace bytes; without it scratch is allocated on that stream.
+    def embed_scaled(self, embed, ids, out, scale=1.0, pos_embed=None, positions=None):
+        """out[i] = embed[ids[i]] * scale (+ pos_embed[positions[i]]) in fp16, bf16 or fp32."""
+        _check(embed.dtype in _DTYPES, 'embed must be fp16, bf16 or fp32')
+        _check_typed(embed, embed, 'embed')
+        _check_typed(out, embed, 'out')
+        n = ids.numel()
+        _check_ints(ids, n, embed, 'ids')
+        _check(embed.dim() == 2 and embed.numel() > 0, 'embed must be [vocab, hidden]')
+        vocab, hidden = embed.shape
+        _check((pos_embed is None) == (positions is None), 'pos_embed and positions must be given together')
+        max_pos = 0
+        if pos_embed is not None:
+            _check_typed(pos_embed, embed, 'pos_embed')
+            _check_ints(positions, n, embed, 'positions')
+            _check(pos_embed.dim() == 2 and pos_embed.size(1) == hidden and pos_embed.numel() > 0,
+                   'pos_embed must be [max_pos, hidden]')
+            max_pos = pos_embed.size(0)
+        _check(out.numel() == n * hidden, 'embed_scaled: out must be [n, hidden]')
+        with _On(embed.device):
+            _lib.call('fw_embed_scaled', _ptr(embed), _ptr(pos_embed), _ptr(ids), _ptr(positions), _ptr(out), n, vocab,
+                      max_pos, hidden, float(scale), _DTYPES[embed.dtype], _stream())
+
+    def embed_grad_workspace(self, n, hidden):
+        need = ctypes.c_int64(0)
+        _lib.call('fw_embed_grad_workspace', int(n), int(hidden), ctypes.byref(need))
+        return need.value
+
+    def embed_grad(self, dout, ids, dembed, scale=1.0, padding_idx=-1, accumulate=False, ws=None):
+        """dembed[v] = (dembed[v] if accumulate) + scale * sum of dout[i] over ids[i] == v != padding_idx, summed in
+        fp32 in the order of i. With ids = positions and scale 1 it is the position table's gradient."""
+        _check(dembed.dtype in _DTYPES, 'dembed must be fp16, bf16 or fp32')
+        _check_typed(dembed, dembed, 'dembed')
+        _check_typed(dout, dembed, 'dout')
+        n = ids.numel()
+        _check_ints(ids, n, dembed, 'ids')
+        _check(dembed.dim() == 2 and dembed.numel() > 0, 'dembed must be [vocab, hidden]')
+        vocab, hidden = dembed.shape
+        _check(dout.numel() == n * hidden, 'embed_grad: dout must be [n, hidden]')
+        with _On(dembed.device):
+            ws = _workspace(ws, 'fw_embed_grad_workspace', (n, hidden), dembed.device)
+            _lib.call('fw_embed_grad', _ptr(dout), _ptr(ids), _ptr(dembed), n, vocab, hidden, float(scale),
+                      int(padding_idx), int(bool(accumulate)), _DTYPES[dembed.dtype], _ptr(ws), ws.numel(), _stream())
 
     def decoder_step(self, desc, steps=1):
         _lib.call('fw_decoder_step', ctypes.byref(desc), int(steps), _stream())

@@ -40,6 +40,11 @@ enum {
 #define FW_DEVERR_TIMEOUT 1u    /* a bounded wait inside a kernel gave up */
 #define FW_DEVERR_BAD_INDEX 2u  /* a token id / position read from device memory was out of range */
 
+/* Element types of the whole-transcript operators (embed_*, prompt_attention*, lm_head_loss*). */
+#define FW_F16 0
+#define FW_BF16 1
+#define FW_F32 2
+
 /* Message for the last failing call on this thread ("" if none). */
 const char* fw_last_error_string(void);
 /* ABI version of this library. */
@@ -370,6 +375,34 @@ typedef struct {
 
 /* mel -> encoder states -> cross K/V for every decoder layer (custom/model.py:143-147). */
 int fw_encoder_forward(const fw_encoder_t* e, fw_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Whole transcripts at once: the token path of the decoder for packed transcripts (scoring with
+ * teacher forcing, long prompts, training). The reference decodes token by token only
+ * (custom/model.py:107-123), so these have no counterpart there. Element types are FW_F16, FW_BF16
+ * (and FW_F32 for the embedding); sums are held in fp32 and rounded once.
+ * A *_workspace call writes the bytes of 16-byte aligned device scratch that the operator needs for
+ * these sizes (it depends on nothing else). The scratch needs no initial value, keeps nothing between
+ * calls, and must not be shared by calls that overlap on the GPU.
+ * ---------------------------------------------------------------------------------------- */
+
+/* out[i] = T(scale * embed[ids[i]] + pos_embed[positions[i]]), i < n; rows of `hidden` elements of type
+ * dtype. pos_embed and positions are given together or both NULL. fw_embed_pos with a scale, with the
+ * positions optional and in every type; ids and positions out of range are clamped and set
+ * FW_DEVERR_BAD_INDEX as there. */
+int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids, const int64_t* positions, void* out,
+                    int n, int vocab, int max_pos, int hidden, float scale, int dtype, fw_stream_t stream);
+
+/* Gradient of fw_embed_scaled with respect to embed (or, with ids = positions and scale 1, to pos_embed):
+ * dembed[v] = [dembed[v] +] scale * sum over i with ids[i] == v of dout[i], for every v < vocab. The sum
+ * runs in fp32 in the order of i (tokens are sorted, no atomics: the result is the same in every run).
+ * accumulate 0 writes every row (zero where no token names it); 1 adds to dembed and touches only the
+ * rows that tokens name. Tokens equal to padding_idx (-1: none) are left out; ids out of range are left
+ * out and set FW_DEVERR_BAD_INDEX. */
+int fw_embed_grad(const void* dout, const int64_t* ids, void* dembed, int n, int vocab, int hidden, float scale,
+                  int64_t padding_idx, int accumulate, int dtype, void* workspace, int64_t workspace_bytes,
+                  fw_stream_t stream);
+int fw_embed_grad_workspace(int n, int hidden, int64_t* bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,67 @@
+"""CPU tests of the whole-transcript operators' refusals: the C entry points reject bad sizes, types, alignment and
+workspaces before anything touches a GPU, and the wrappers reject tensors that are not on one."""
+
+import ctypes
+
+import pytest
+import torch
+
+from flash_whisper_b200 import _lib
+from flash_whisper_b200.ext import Ext
+
+P = ctypes.c_void_p(256)
+ODD = ctypes.c_void_p(257)
+
+
+def _refused(name, args, status, text):
+    lib = _lib.lib()
+    assert getattr(lib, name)(*args) == status, lib.fw_last_error_string()
+    assert text in lib.fw_last_error_string().decode(), lib.fw_last_error_string()
+
+
+@pytest.mark.parametrize('args,status,text', [
+    ((None, None, P, None, P, 4, 10, 0, 64, 1.0, 0, None), 1, 'required'),
+    ((P, None, None, None, P, 4, 10, 0, 64, 1.0, 0, None), 1, 'required'),
+    ((P, P, P, None, P, 4, 10, 5, 64, 1.0, 0, None), 4, 'given together'),
+    ((P, None, P, None, P, -1, 10, 0, 64, 1.0, 0, None), 2, 'bad sizes'),
+    ((P, None, P, None, P, 4, 0, 0, 64, 1.0, 0, None), 2, 'bad sizes'),
+    ((P, P, P, P, P, 4, 10, 0, 64, 1.0, 0, None), 2, 'bad sizes'),
+    ((P, None, P, None, P, 4, 10, 0, 64, 1.0, 3, None), 4, 'dtype'),
+    ((ODD, None, P, None, P, 4, 10, 0, 64, 1.0, 1, None), 3, 'aligned'),
+])
+def test_embed_scaled_refuses(args, status, text):
+    _refused('fw_embed_scaled', args, status, text)
+
+
+@pytest.mark.parametrize('args,status,text', [
+    ((P, P, None, 4, 10, 64, 1.0, -1, 0, 0, P, 1 << 20, None), 1, 'required'),
+    ((P, P, P, 4, 10, 64, 1.0, -1, 0, 0, None, 1 << 20, None), 1, 'required'),
+    ((P, P, P, 4, 10, 0, 1.0, -1, 0, 0, P, 1 << 20, None), 2, 'bad sizes'),
+    ((P, P, P, 4, (1 << 30) + 1, 64, 1.0, -1, 0, 0, P, 1 << 20, None), 2, 'bad sizes'),
+    ((P, P, P, 4, 10, 64, 1.0, -1, 0, 7, P, 1 << 20, None), 4, 'dtype'),
+    ((P, P, ODD, 4, 10, 64, 1.0, -1, 0, 2, P, 1 << 20, None), 3, 'aligned'),
+    ((P, P, P, 4, 10, 64, 1.0, -1, 0, 0, ODD, 1 << 20, None), 3, 'workspace'),
+    ((P, P, P, 4, 10, 64, 1.0, -1, 0, 0, P, 100, None), 2, 'workspace too small'),
+])
+def test_embed_grad_refuses(args, status, text):
+    _refused('fw_embed_grad', args, status, text)
+
+
+def test_nothing_to_do_needs_no_gpu():
+    lib = _lib.lib()
+    assert lib.fw_embed_scaled(P, None, None, None, None, 0, 10, 0, 64, 1.0, 0, None) == 0
+    assert lib.fw_embed_grad(None, None, P, 0, 10, 64, 1.0, -1, 1, 0, None, 0, None) == 0
+
+
+def test_embed_wrappers_refuse_cpu_tensors():
+    ext = Ext()
+    h, ids = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(4, dtype=torch.long)
+    with pytest.raises(RuntimeError, match='embed must be contiguous CUDA float16'):
+        ext.embed_scaled(h, ids, h)
+    with pytest.raises(RuntimeError, match='dembed must be contiguous CUDA float16'):
+        ext.embed_grad(h, ids, h)
+    with pytest.raises(RuntimeError, match='fp16, bf16 or fp32'):
+        ext.embed_scaled(h.double(), ids, h)
+    assert ext.embed_grad_workspace(100, 64) > 0
+    with pytest.raises(RuntimeError, match='bad sizes'):
+        ext.embed_grad_workspace(-1, 64)
