@@ -119,6 +119,11 @@ _SIGNATURES = {
     'fw_embed_scaled': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_float, c_int, vp]),
     'fw_embed_grad': (c_int, [vp, vp, vp, c_int, c_int, c_int, c_float, c_int64, c_int, c_int, vp, c_int64, vp]),
     'fw_embed_grad_workspace': (c_int, [c_int, c_int, i64p]),
+    'fw_lm_head_loss': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, vp, c_int64, vp]),
+    'fw_lm_head_loss_workspace': (c_int, [c_int, c_int, i64p]),
+    'fw_lm_head_loss_grad': (c_int, [vp, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, c_int, vp,
+                                     c_int64, vp]),
+    'fw_lm_head_loss_grad_workspace': (c_int, [c_int, c_int, c_int, i64p]),
 }
 
 _lib = None

@@ -1,0 +1,723 @@
+// Softmax cross entropy over the tied vocabulary matrix, and its gradient, without ever keeping the logits.
+//
+//   z = h W^T   (n x vocab, fp32 accumulators in tensor memory)
+//   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_i,t(i)        (0 where the target is ignored)
+//   dz_iv = g_i (exp(z_iv - lse_i) - [v = t(i)])        dh = dz W        dW = dz^T h
+//
+// All products run in one persistent tcgen05 kernel on CTA pairs (cta_group::2, 256 x 256 tiles: each CTA stages
+// 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a third less L2 traffic than two 128 x 256
+// tiles), fed by TMA through a 6-stage ring, with the accumulators of two tiles in tensor memory so that the
+// epilogue of one runs under the MMAs of the next.
+//   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
+//     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
+//     row and half tile.
+//   * gradient: the vocabulary is taken in pieces whose dz (16 bits) fits the scratch and mostly L2. Per piece one
+//     launch recomputes z and writes dz, a second one has both products of it: dh (contraction over the piece; fp32
+//     partial sums per k split, carried from piece to piece) and dW (contraction over the rows, final).
+// 16-bit dz: exp(z - lse) - [v = t] lies in [-1, 1] whatever g is, so it is stored without g (times 2^12 in fp16,
+// which keeps probabilities down to 2^-36 above the smallest subnormal); g multiplies dh's rows in fp32 at the end, and
+// is folded into the 16-bit copy of h that dW's product reads, relative to the largest |g|, so that with equal
+// weights nothing is rounded a second time.
+#include "fw_host.h"
+#include "fw_tc.cuh"
+
+namespace fw {
+
+FW_DEFINE_ERROR_WORD();
+
+__device__ __forceinline__ void loss_flag(unsigned bits) { atomicOr(&g_fw_dev_error, bits); }
+
+constexpr int kBM = 256, kBN = 256, kBK = 64;  // tile of a CTA pair
+constexpr int kStages = 6;
+constexpr uint32_t kHalfBytes = 128 * kBK * 2;  // a CTA's share of A (or B) per stage: 16 KB
+constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+constexpr int kLossSmem = kStages * kStageBytes + 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kLossThreads = 32 * (2 + kEpiWarps);
+constexpr int kMGroup = 32;  // row tiles that run against a vocabulary tile before the next one: h stays in L2
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+enum Kind { kStats, kDz, kGrads };  // what a launch computes
+
+struct LossArgs {
+  int n, hidden, width;      // rows, hidden size, columns of this launch's vocabulary piece
+  int v0, vocab;             // first vocabulary row of the piece; all rows
+  int m_tiles, n_tiles;      // kStats, kDz: over (rows, piece); kGrads: dW over (piece, hidden)
+  int dh_m_tiles, splits;    // kGrads: dh over (rows, hidden), each tile's contraction in `splits` parts
+  int64_t ignore;
+  const int64_t* targets;
+  const float* lse;
+  float2* stats;             // [2 * all n tiles][n]
+  float* target_logit;       // [n]
+  void* dz;                  // [n][ld_dz]
+  int64_t ld_dz;
+  float dz_scale;            // the factor stored with dz
+  float* part;               // [splits][n][hidden]
+  void* dw;                  // [vocab][hidden]
+  const float* gmax;
+  int first_piece, accumulate;
+};
+
+struct Tile {
+  int m0, n0, kb0, kbs;
+  int split;
+  bool dh;  // kGrads
+};
+
+template <int kKind>
+__device__ __forceinline__ int tile_count(const LossArgs& a) {
+  return kKind == kGrads ? a.dh_m_tiles * a.splits * a.n_tiles + a.m_tiles * a.n_tiles : a.m_tiles * a.n_tiles;
+}
+
+template <int kKind>
+__device__ __forceinline__ Tile tile_at(const LossArgs& a, int t) {
+  Tile x;
+  if (kKind != kGrads) {
+    // groups of kMGroup row tiles; within a group the row tiles run against one vocabulary tile after the other
+    const int per = kMGroup * a.n_tiles, grp = t / per, in = t - grp * per;
+    const int rows = min(kMGroup, a.m_tiles - grp * kMGroup);
+    x.m0 = (grp * kMGroup + in % rows) * kBM;
+    x.n0 = in / rows * kBN;
+    x.kb0 = 0;
+    x.kbs = (a.hidden + kBK - 1) / kBK;
+    x.split = 0;
+    x.dh = false;
+    return x;
+  }
+  const int dh_tiles = a.dh_m_tiles * a.splits * a.n_tiles;
+  x.dh = t < dh_tiles;
+  if (x.dh) {
+    const int kb = (a.width + kBK - 1) / kBK;
+    x.n0 = t % a.n_tiles * kBN;
+    const int u = t / a.n_tiles;
+    x.split = u % a.splits;
+    x.m0 = u / a.splits * kBM;
+    x.kb0 = static_cast<int>(static_cast<int64_t>(kb) * x.split / a.splits);
+    x.kbs = static_cast<int>(static_cast<int64_t>(kb) * (x.split + 1) / a.splits) - x.kb0;
+  } else {
+    t -= dh_tiles;
+    x.n0 = t % a.n_tiles * kBN;
+    x.m0 = t / a.n_tiles * kBM;
+    x.kb0 = 0;
+    x.kbs = (a.n + kBK - 1) / kBK;
+    x.split = 0;
+  }
+  return x;
+}
+
+// A CTA's 128 rows of an operand for one k block. K-major: one box of 64 k x 128 rows. MN-major: two boxes of 64
+// rows (contiguous) x 64 k.
+template <bool kMn>
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint32_t rbar, int row, int k) {
+  if (kMn) {
+    tma_load_2d_pair(dst, map, rbar, row, k);
+    tma_load_2d_pair(dst + kHalfBytes / 2, map, rbar, row + 64, k);
+  } else {
+    tma_load_2d_pair(dst, map, rbar, k, row);
+  }
+}
+
+template <bool kMn>
+__device__ __forceinline__ uint64_t half_desc(uint32_t addr) {
+  return kMn ? sw128_mn_desc(addr, kHalfBytes / 2) : sw128_desc(addr);
+}
+
+template <typename T, bool kAMn, bool kBMn>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a_addr, bool fresh) {
+  constexpr uint32_t idesc = make_idesc(kBM, kBN, Type16<T>::kBf16, kAMn, kBMn);
+  const uint64_t ad = half_desc<kAMn>(a_addr), bd = half_desc<kBMn>(a_addr + kHalfBytes);
+#pragma unroll
+  for (int kk = 0; kk < kBK / 16; ++kk)
+    tc_mma_pair(d, ad + kk * (kAMn ? 128 : 2), bd + kk * (kBMn ? 128 : 2), idesc, fresh && kk == 0 ? 0u : 1u);
+}
+
+// tmA, tmB: the operands of kStats, kDz and of kGrads' dh; tmA2, tmB2: of kGrads' dW.
+template <int kKind, typename T>
+__global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
+    loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2, LossArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base_sh;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
+  const int tiles = tile_count<kKind>(a);
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);   // leader's: both CTAs' bytes, one arrival
+      mbar_init(&empty_bar[s], 1);  // each CTA's: the pair's MMAs have read the stage
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);  // leader's: both CTAs' epilogue warps have drained the buffer
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    if (kKind == kGrads) {
+      tma_prefetch_desc(&tmA2);
+      tma_prefetch_desc(&tmB2);
+    }
+  }
+  if (warp == 1) tmem_alloc_pair(&tmem_base_sh, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += pairs) {
+        const Tile x = tile_at<kKind>(a, t);
+        for (int kb = 0; kb < x.kbs; ++kb, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && !mbar_wait(&empty_bar[s], ((it / kStages) & 1u) ^ 1u)) {
+            loss_flag(FW_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kStageBytes);
+          const uint32_t rbar = cluster_map(&full_bar[s], 0);
+          uint8_t* dst = smem + s * kStageBytes;
+          const int row_a = x.m0 + 128 * static_cast<int>(rank), row_b = x.n0 + 128 * static_cast<int>(rank);
+          const int k = (x.kb0 + kb) * kBK;
+          if (kKind != kGrads) {
+            load_half<false>(dst, &tmA, rbar, row_a, k);
+            load_half<false>(dst + kHalfBytes, &tmB, rbar, row_b, k);
+          } else if (x.dh) {
+            load_half<false>(dst, &tmA, rbar, row_a, k);
+            load_half<true>(dst + kHalfBytes, &tmB, rbar, row_b, k);
+          } else {
+            load_half<true>(dst, &tmA2, rbar, row_a, k);
+            load_half<true>(dst + kHalfBytes, &tmB2, rbar, row_b, k);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += pairs, ++local) {
+        const Tile x = tile_at<kKind>(a, t);
+        const int buf = local & 1;
+        if (local >= 2 && !mbar_wait(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u)) {
+          loss_flag(FW_DEVERR_TIMEOUT);
+          ok = false;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * kBN;
+        for (int kb = 0; kb < x.kbs && ok; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&full_bar[s], (it / kStages) & 1u)) {
+            loss_flag(FW_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t at = base + s * kStageBytes;
+          if (kKind != kGrads)
+            mma_block<T, false, false>(d, at, kb == 0);
+          else if (x.dh)
+            mma_block<T, false, true>(d, at, kb == 0);
+          else
+            mma_block<T, true, true>(d, at, kb == 0);
+          tc_commit_pair(&empty_bar[s]);
+        }
+        tc_commit_pair(&acc_full[buf]);
+      }
+    }
+  } else {
+    // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns
+    // 128 ((w - 2) / 4) .. + 127.
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    const uint32_t drained = cluster_map(&acc_empty[0], 0);
+    bool failed = false;
+    int local = 0;
+    for (int t = first; t < tiles; t += pairs, ++local) {
+      const Tile x = tile_at<kKind>(a, t);
+      const int buf = local & 1;
+      const int row = x.m0 + 128 * static_cast<int>(rank) + q * 32 + lane;
+      const int c0 = x.n0 + 128 * part;
+      int64_t target = -1;  // relative to this launch's vocabulary piece
+      float neg_lse = 0.f;
+      bool kept = false;
+      if (kKind != kGrads && row < a.n) {
+        const int64_t tg = a.targets[row];
+        kept = tg != a.ignore && tg >= 0 && tg < a.vocab;
+        target = tg - a.v0;
+        if (kKind == kDz) neg_lse = -a.lse[row] * kLog2e;
+      }
+      if (failed || !mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
+        if (!failed) loss_flag(FW_DEVERR_TIMEOUT);
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + 128 * part;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t r[32];
+        tc_load32(d + c, r);
+        tc_wait_ld();
+        const int col = c0 + c;
+        if (kKind == kStats) {
+          if (col + 32 > a.width) {  // columns behind the vocabulary count as -inf
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= a.width) r[j] = 0xff800000u;
+          }
+          float m = top;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(r[j]));
+          const float off = m == -INFINITY ? 0.f : -m * kLog2e;
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j & 3] += ex2(fmaf(__uint_as_float(r[j]), kLog2e, off));
+          sum = fmaf(sum, ex2(fmaf(top, kLog2e, off)), (acc[0] + acc[1]) + (acc[2] + acc[3]));
+          top = m;
+          if (target >= col && target < col + 32) {
+            const int at = static_cast<int>(target) - col;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == at) a.target_logit[row] = __uint_as_float(r[j]);
+          }
+        } else if (kKind == kDz && row < a.n) {
+          const int at = target >= col && target < col + 32 ? static_cast<int>(target) - col : -1;
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.dz) + static_cast<int64_t>(row) * a.ld_dz + col);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float p = ex2(fmaf(__uint_as_float(r[j]), kLog2e, neg_lse)) - (j == at ? 1.f : 0.f);
+            r[j] = __float_as_uint(kept ? p * a.dz_scale : 0.f);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_uint4(Type16<T>::pack(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1])),
+                                Type16<T>::pack(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3])),
+                                Type16<T>::pack(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5])),
+                                Type16<T>::pack(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7])));
+        } else if (kKind == kGrads && x.dh && row < a.n) {
+          float* dst = a.part + (static_cast<int64_t>(x.split) * a.n + row) * a.hidden + col;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            if (col + j >= a.hidden) break;
+            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                                   __uint_as_float(r[j + 3]));
+            float4* at = reinterpret_cast<float4*>(dst + j);
+            if (!a.first_piece) {
+              const float4 o = *at;
+              v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+            }
+            *at = v;
+          }
+        } else if (kKind == kGrads && !x.dh && row < a.width) {
+          const float f = *a.gmax / a.dz_scale;
+          uint4* dst =
+              reinterpret_cast<uint4*>(static_cast<T*>(a.dw) + (static_cast<int64_t>(a.v0) + row) * a.hidden + col);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (col + 8 * j >= a.hidden) break;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[8 * j + i]) * f;
+            if (a.accumulate) {
+              const uint4 o = dst[j];
+              const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 u = Type16<T>::unpack(ow[i]);
+                v[2 * i] += u.x;
+                v[2 * i + 1] += u.y;
+              }
+            }
+            dst[j] = make_uint4(Type16<T>::pack(v[0], v[1]), Type16<T>::pack(v[2], v[3]), Type16<T>::pack(v[4], v[5]),
+                                Type16<T>::pack(v[6], v[7]));
+          }
+        }
+        __syncwarp();  // the next load is a warp-wide instruction
+      }
+      if (kKind == kStats && row < a.n)
+        a.stats[static_cast<int64_t>(2 * (x.n0 / kBN) + part) * a.n + row] = make_float2(top, sum);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(drained + 8 * buf);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer's barriers or tensor memory are in use
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+// Joins the (max, sum) of all half tiles of a row: 32 rows per CTA (lanes), the half tiles over its warps.
+constexpr int kCombineThreads = 512;
+__global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const float2* __restrict__ stats, int halves,
+                                                                       int n, const int64_t* __restrict__ targets,
+                                                                       int64_t ignore, int vocab, float* loss,
+                                                                       float* __restrict__ lse) {
+  constexpr int kWarps = kCombineThreads / 32;
+  __shared__ float2 s_part[kWarps][32];
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 32 + lane;
+  float top = -INFINITY, sum = 0.f;
+  if (row < n) {
+#pragma unroll 4
+    for (int i = warp; i < halves; i += kWarps) {
+      const float2 v = stats[static_cast<int64_t>(i) * n + row];
+      const float m = fmaxf(top, v.x), off = m == -INFINITY ? 0.f : -m * kLog2e;
+      sum = sum * ex2(fmaf(top, kLog2e, off)) + v.y * ex2(fmaf(v.x, kLog2e, off));
+      top = m;
+    }
+  }
+  s_part[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (warp != 0 || row >= n) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_part[w][lane].x);
+  const float off = m == -INFINITY ? 0.f : -m * kLog2e;
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) s += s_part[w][lane].y * ex2(fmaf(s_part[w][lane].x, kLog2e, off));
+  const float l = m + logf(s);
+  const int64_t t = targets[row];
+  const bool bad = t != ignore && (t < 0 || t >= vocab);
+  if (bad) loss_flag(FW_DEVERR_BAD_INDEX);
+  lse[row] = l;
+  loss[row] = t == ignore || bad ? 0.f : l - loss[row];  // held the target's logit
+}
+
+// Gradient, before the products: the largest finite |g| of the rows that count (each CTA finds it by itself from L2)
+// and h scaled by g relative to it, zero in rows that do not count.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_scale_kernel(const T* __restrict__ h, const float* __restrict__ g,
+                                                         const int64_t* __restrict__ targets, int64_t ignore,
+                                                         int vocab, int n, int hidden, T* __restrict__ scaled,
+                                                         float* __restrict__ gmax) {
+  __shared__ float s_max[8];
+  pdl_trigger();
+  float m = 0.f;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t t = targets[i];
+    const float v = fabsf(g[i]);
+    const bool bad = t != ignore && (t < 0 || t >= vocab);
+    if (bad && blockIdx.x == 0) loss_flag(FW_DEVERR_BAD_INDEX);
+    if (t != ignore && !bad && v < INFINITY) m = fmaxf(m, v);  // NaN fails the comparison
+  }
+  m = warp_max(m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, s_max[w]);
+  if (m == 0.f) m = 1.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *gmax = m;
+  const int packs = hidden / 8;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < static_cast<int64_t>(n) * packs;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int row = static_cast<int>(i / packs);
+    const int64_t t = targets[row];
+    const bool counts = t >= 0 && t < vocab && t != ignore;
+    const float f = counts ? g[row] / m : 0.f;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (counts) {
+      v = reinterpret_cast<const uint4*>(h)[i];
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 u = Type16<T>::unpack(w[j]);
+        w[j] = Type16<T>::pack(u.x * f, u.y * f);
+      }
+    }
+    reinterpret_cast<uint4*>(scaled)[i] = v;
+  }
+}
+
+// Gradient, after the products: dh = T(g / dz_scale * sum over the k splits), zero in rows that do not count.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_dh_kernel(const float* __restrict__ part, int splits,
+                                                      const float* __restrict__ g, const int64_t* __restrict__ targets,
+                                                      int64_t ignore, int vocab, int n, int hidden, float dz_scale,
+                                                      T* __restrict__ dh) {
+  pdl_wait();
+  const int packs = hidden / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= static_cast<int64_t>(n) * packs) return;
+  const int row = static_cast<int>(i / packs);
+  const int64_t t = targets[row];
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (t >= 0 && t < vocab && t != ignore) {
+    float acc[8] = {};
+    const float4* src = reinterpret_cast<const float4*>(part) + 2 * i;
+    const int64_t step = static_cast<int64_t>(n) * packs * 2;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float4 x = src[s * step], y = src[s * step + 1];
+      acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
+      acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
+    }
+    const float f = g[row] / dz_scale;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = Type16<T>::pack(acc[2 * j] * f, acc[2 * j + 1] * f);
+  }
+  reinterpret_cast<uint4*>(dh)[i] = v;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+static int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+constexpr int kPairs = 74;                        // CTA pairs of a B200
+constexpr int64_t kDzBytes = int64_t(96) << 20;  // a piece's dz at most: it and what it meets stay mostly in L2
+
+struct LossLayout {
+  int n_tiles;
+  int64_t total;
+};
+static LossLayout loss_layout(int n, int vocab) {
+  LossLayout l;
+  l.n_tiles = (vocab + kBN - 1) / kBN;
+  l.total = 2 * static_cast<int64_t>(l.n_tiles) * n * static_cast<int64_t>(sizeof(float2));
+  return l;
+}
+
+struct GradLayout {
+  int pieces, width, splits;  // width: columns of a piece, a multiple of the tile
+  int64_t gmax, dz, part, total;
+};
+static GradLayout grad_layout(int n, int vocab, int hidden) {
+  GradLayout l;
+  const int64_t tiles = (vocab + kBN - 1) / kBN;
+  int64_t most = kDzBytes / (2 * static_cast<int64_t>(n > 0 ? n : 1)) / kBN;
+  if (most < 1) most = 1;
+  l.pieces = static_cast<int>((tiles + most - 1) / most);
+  const int64_t per = (tiles + l.pieces - 1) / l.pieces;
+  l.width = static_cast<int>(per * kBN);
+  // Few rows: dh has few tiles with a contraction as long as the piece; split it until every pair has one.
+  const int64_t dh_tiles = up(n, kBM) / kBM * (up(hidden, kBN) / kBN);
+  int64_t s = dh_tiles > 0 ? kPairs / dh_tiles : 1;
+  const int64_t kb = up(vocab < l.width ? vocab : l.width, kBK) / kBK / 4;  // at least 4 k blocks a part
+  if (s > kb) s = kb;
+  l.splits = static_cast<int>(s < 1 ? 1 : s);
+  // every piece, the last one too, has at least one k block for each split
+  const int64_t last = (vocab - static_cast<int64_t>(l.pieces - 1) * l.width + kBK - 1) / kBK;
+  if (l.splits > last) l.splits = static_cast<int>(last < 1 ? 1 : last);
+  l.gmax = up(static_cast<int64_t>(n) * hidden * 2, 256);
+  l.dz = l.gmax + 256;
+  l.part = l.dz + up(static_cast<int64_t>(n) * l.width * 2, 256);
+  l.total = l.part + static_cast<int64_t>(l.splits) * n * hidden * 4;
+  return l;
+}
+
+// 2-D map with 128-byte swizzle over rows of `inner` contiguous 16-bit elements; boxes of 64 x box_outer.
+static int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* ptr, int64_t inner, int64_t outer, int64_t ld,
+                    int box_outer) {
+  EncodeTiledFn enc = tensor_map_encode_fn();
+  if (!enc) return set_error(FW_ERR_LAUNCH, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_outer)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(m, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FW_ERR_ARG, "lm_head_loss: tensor map encode failed (%d)", static_cast<int>(r));
+  return FW_OK;
+}
+
+template <int kKind, typename T>
+static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta2, const CUtensorMap& tb2,
+                       const LossArgs& a, int tiles, cudaStream_t s, bool pdl) {
+  auto kern = loss_gemm_kernel<kKind, T>;
+  cudaError_t e = ensure_smem(kern, kLossSmem);
+  if (e == cudaSuccess) {
+    const int pairs = num_sms() / 2;
+    e = launch(kern, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kLossThreads), kLossSmem, s, pdl, ta, tb, ta2,
+               tb2, a);
+  }
+  return launch_status(e, "lm_head_loss");
+}
+
+template <typename T>
+static int run_loss(const void* h, const void* w, const int64_t* targets, float* loss, float* lse, int n, int vocab,
+                    int hidden, int64_t ignore, void* ws, cudaStream_t s) {
+  const LossLayout l = loss_layout(n, vocab);
+  CUtensorMap ta, tb;
+  int rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
+  if (!rc) rc = make_map(&tb, Type16<T>::kMap, w, hidden, vocab, hidden, 128);
+  if (rc) return rc;
+  LossArgs a{};
+  a.n = n;
+  a.hidden = hidden;
+  a.width = a.vocab = vocab;
+  a.m_tiles = (n + kBM - 1) / kBM;
+  a.n_tiles = l.n_tiles;
+  a.ignore = ignore;
+  a.targets = targets;
+  a.stats = static_cast<float2*>(ws);
+  a.target_logit = loss;  // replaced by the loss when the halves are joined
+  rc = launch_gemm<kStats, T>(ta, tb, ta, tb, a, a.m_tiles * a.n_tiles, s, false);
+  if (rc) return rc;
+  cudaError_t e = launch(loss_combine_kernel, dim3((n + 31) / 32), dim3(kCombineThreads), 0, s, true,
+                         static_cast<const float2*>(a.stats), 2 * l.n_tiles, n, targets, ignore, vocab, loss, lse);
+  return launch_status(e, "lm_head_loss combine");
+}
+
+template <typename T>
+static int run_loss_grad(const void* h, const void* w, const int64_t* targets, const float* lse, const float* g,
+                         void* dh, void* dw, int n, int vocab, int hidden, int64_t ignore, int accumulate, void* ws,
+                         cudaStream_t s) {
+  const GradLayout l = grad_layout(n, vocab, hidden);
+  uint8_t* b = static_cast<uint8_t*>(ws);
+  T* scaled = reinterpret_cast<T*>(b);
+  float* gmax = reinterpret_cast<float*>(b + l.gmax);
+  void* dz = b + l.dz;
+  float* part = reinterpret_cast<float*>(b + l.part);
+  const float dz_scale = Type16<T>::kBf16 ? 1.f : 4096.f;
+  const int64_t packs = static_cast<int64_t>(n) * (hidden / 8);
+  const int64_t blocks = (packs + 255) / 256;
+  cudaError_t e = launch(loss_scale_kernel<T>, dim3(static_cast<unsigned>(blocks < 4 * num_sms() ? blocks : 4 * num_sms())),
+                         dim3(256), 0, s, false, static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden, scaled,
+                         gmax);
+  int rc = launch_status(e, "lm_head_loss_grad scale");
+  CUtensorMap ta, tb, ga, gb, ga2, gb2;
+  if (!rc) rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
+  if (!rc) rc = make_map(&gb2, Type16<T>::kMap, scaled, hidden, n, hidden, 64);
+  for (int p = 0; p < l.pieces && !rc; ++p) {
+    const int v0 = p * l.width, width = vocab - v0 < l.width ? vocab - v0 : l.width;
+    const T* wp = static_cast<const T*>(w) + static_cast<int64_t>(v0) * hidden;
+    rc = make_map(&tb, Type16<T>::kMap, wp, hidden, width, hidden, 128);
+    if (!rc) rc = make_map(&ga, Type16<T>::kMap, dz, width, n, l.width, 128);
+    if (!rc) rc = make_map(&gb, Type16<T>::kMap, wp, hidden, width, hidden, 64);
+    if (!rc) rc = make_map(&ga2, Type16<T>::kMap, dz, width, n, l.width, 64);
+    if (rc) return rc;
+    LossArgs a{};
+    a.n = n;
+    a.hidden = hidden;
+    a.width = width;
+    a.v0 = v0;
+    a.vocab = vocab;
+    a.m_tiles = (n + kBM - 1) / kBM;
+    a.n_tiles = (width + kBN - 1) / kBN;
+    a.ignore = ignore;
+    a.targets = targets;
+    a.lse = lse;
+    a.dz = dz;
+    a.ld_dz = l.width;
+    a.dz_scale = dz_scale;
+    rc = launch_gemm<kDz, T>(ta, tb, ta, tb, a, a.m_tiles * a.n_tiles, s, true);
+    if (rc) return rc;
+    a.m_tiles = dw != nullptr ? (width + kBM - 1) / kBM : 0;
+    a.n_tiles = (hidden + kBN - 1) / kBN;
+    a.dh_m_tiles = dh != nullptr ? (n + kBM - 1) / kBM : 0;
+    a.splits = l.splits;
+    a.part = part;
+    a.dw = dw;
+    a.gmax = gmax;
+    a.first_piece = p == 0;
+    a.accumulate = accumulate;
+    rc = launch_gemm<kGrads, T>(ga, gb, ga2, gb2, a, (a.dh_m_tiles * a.splits + a.m_tiles) * a.n_tiles, s, true);
+  }
+  if (rc || dh == nullptr) return rc;
+  e = launch(loss_dh_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, true,
+             static_cast<const float*>(part), l.splits, g, targets, ignore, vocab, n, hidden, dz_scale,
+             static_cast<T*>(dh));
+  return launch_status(e, "lm_head_loss_grad dh");
+}
+
+// Checks that both entry points share.
+static int check_loss(const char* what, const void* h, const void* w, const int64_t* targets, int n, int vocab,
+                      int hidden, int dtype, const void* ws, int64_t ws_bytes, int64_t need) {
+  FW_REQUIRE(n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= (1 << 22), FW_ERR_SHAPE,
+             "%s: n and vocab must be at most %d", what, 1 << 22);
+  FW_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= 65536, FW_ERR_SHAPE,
+             "%s: hidden must be a multiple of 8, at most 65536", what);
+  FW_REQUIRE(dtype == FW_F16 || dtype == FW_BF16, FW_ERR_ARG, "%s: dtype must be fp16 or bf16", what);
+  FW_REQUIRE(n == 0 || (h && w && targets && ws), FW_ERR_NULL, "%s: h, w, targets and workspace are required", what);
+  FW_REQUIRE(aligned16(h) && aligned16(w) && aligned16(ws), FW_ERR_ALIGN,
+             "%s: h, w and workspace must be 16-byte aligned", what);
+  FW_REQUIRE(n == 0 || ws_bytes >= need, FW_ERR_SHAPE, "%s: workspace too small (%lld of %lld bytes)", what,
+             static_cast<long long>(ws_bytes), static_cast<long long>(need));
+  return FW_OK;
+}
+
+unsigned int read_loss_errors(bool clear) {
+  unsigned int v = 0, zero = 0;
+  cudaMemcpyFromSymbol(&v, g_fw_dev_error, sizeof(v));
+  if (clear && v) cudaMemcpyToSymbol(g_fw_dev_error, &zero, sizeof(zero));
+  return v;
+}
+
+}  // namespace fw
+
+using namespace fw;
+
+extern "C" {
+
+int fw_lm_head_loss_workspace(int n, int vocab, int64_t* bytes) {
+  FW_REQUIRE(bytes != nullptr, FW_ERR_NULL, "lm_head_loss_workspace: bytes is NULL");
+  FW_REQUIRE(n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= (1 << 22), FW_ERR_SHAPE,
+             "lm_head_loss: n and vocab must be at most %d", 1 << 22);
+  *bytes = loss_layout(n, vocab).total;
+  return FW_OK;
+}
+
+int fw_lm_head_loss(const void* h, const void* w, const int64_t* targets, float* loss, float* lse, int n, int vocab,
+                    int hidden, int64_t ignore_index, int dtype, void* workspace, int64_t workspace_bytes,
+                    fw_stream_t stream) {
+  int64_t need = 0;
+  int rc = fw_lm_head_loss_workspace(n, vocab, &need);
+  if (!rc) rc = check_loss("lm_head_loss", h, w, targets, n, vocab, hidden, dtype, workspace, workspace_bytes, need);
+  if (rc || n == 0) return rc;
+  FW_REQUIRE(loss && lse, FW_ERR_NULL, "lm_head_loss: loss and lse are required");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == FW_F16
+             ? run_loss<half>(h, w, targets, loss, lse, n, vocab, hidden, ignore_index, workspace, s)
+             : run_loss<__nv_bfloat16>(h, w, targets, loss, lse, n, vocab, hidden, ignore_index, workspace, s);
+}
+
+int fw_lm_head_loss_grad_workspace(int n, int vocab, int hidden, int64_t* bytes) {
+  FW_REQUIRE(bytes != nullptr, FW_ERR_NULL, "lm_head_loss_grad_workspace: bytes is NULL");
+  FW_REQUIRE(n >= 0 && n <= (1 << 22) && vocab > 0 && vocab <= (1 << 22) && hidden > 0 && hidden <= 65536,
+             FW_ERR_SHAPE, "lm_head_loss_grad: n and vocab must be at most %d, hidden at most 65536", 1 << 22);
+  *bytes = grad_layout(n, vocab, hidden).total;
+  return FW_OK;
+}
+
+int fw_lm_head_loss_grad(const void* h, const void* w, const int64_t* targets, const float* lse, const float* g,
+                         void* dh, void* dw, int n, int vocab, int hidden, int64_t ignore_index, int accumulate,
+                         int dtype, void* workspace, int64_t workspace_bytes, fw_stream_t stream) {
+  int64_t need = 0;
+  int rc = fw_lm_head_loss_grad_workspace(n, vocab, hidden, &need);
+  if (!rc)
+    rc = check_loss("lm_head_loss_grad", h, w, targets, n, vocab, hidden, dtype, workspace, workspace_bytes, need);
+  if (rc) return rc;
+  FW_REQUIRE(aligned16(dh) && aligned16(dw), FW_ERR_ALIGN, "lm_head_loss_grad: dh and dw must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    if (dw == nullptr || accumulate) return FW_OK;
+    return launch_status(cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * hidden * 2, s), "lm_head_loss_grad");
+  }
+  FW_REQUIRE(lse && g, FW_ERR_NULL, "lm_head_loss_grad: lse and g are required");
+  FW_REQUIRE(dh != nullptr || dw != nullptr, FW_ERR_NULL, "lm_head_loss_grad: at least one of dh and dw is required");
+  return dtype == FW_F16 ? run_loss_grad<half>(h, w, targets, lse, g, dh, dw, n, vocab, hidden, ignore_index,
+                                               accumulate, workspace, s)
+                         : run_loss_grad<__nv_bfloat16>(h, w, targets, lse, g, dh, dw, n, vocab, hidden, ignore_index,
+                                                        accumulate, workspace, s);
+}
+
+}  // extern "C"

@@ -74,15 +74,19 @@ class _On:
             self.guard.__exit__(*exc)
 
 
-def _workspace(ws, name, sizes, device):
-    """The caller's scratch after a check of its size, or (None) scratch of the current stream."""
+def _workspace_bytes(name, *sizes):
     need = ctypes.c_int64(0)
-    _lib.call(name, *sizes, ctypes.byref(need))
+    _lib.call(name, *map(int, sizes), ctypes.byref(need))
+    return need.value
+
+
+def _workspace(ws, need, device):
+    """The caller's scratch after a check of its size, or (None) scratch of the current stream."""
     if ws is None:
-        return torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
     if not (ws.is_cuda and ws.is_contiguous() and ws.dtype == torch.uint8 and ws.device == device
-            and ws.numel() >= need.value):
-        raise RuntimeError(f'ws must be contiguous CUDA uint8 on {device} of at least {need.value} bytes')
+            and ws.numel() >= need):
+        raise RuntimeError(f'ws must be contiguous CUDA uint8 on {device} of at least {need} bytes')
     return ws
 
 
@@ -328,9 +332,7 @@ class Ext:
                       max_pos, hidden, float(scale), _DTYPES[embed.dtype], _stream())
 
     def embed_grad_workspace(self, n, hidden):
-        need = ctypes.c_int64(0)
-        _lib.call('fw_embed_grad_workspace', int(n), int(hidden), ctypes.byref(need))
-        return need.value
+        return _workspace_bytes('fw_embed_grad_workspace', n, hidden)
 
     def embed_grad(self, dout, ids, dembed, scale=1.0, padding_idx=-1, accumulate=False, ws=None):
         """dembed[v] = (dembed[v] if accumulate) + scale * sum of dout[i] over ids[i] == v != padding_idx, summed in
@@ -344,9 +346,58 @@ class Ext:
         vocab, hidden = dembed.shape
         _check(dout.numel() == n * hidden, 'embed_grad: dout must be [n, hidden]')
         with _On(dembed.device):
-            ws = _workspace(ws, 'fw_embed_grad_workspace', (n, hidden), dembed.device)
+            ws = _workspace(ws, self.embed_grad_workspace(n, hidden), dembed.device)
             _lib.call('fw_embed_grad', _ptr(dout), _ptr(ids), _ptr(dembed), n, vocab, hidden, float(scale),
                       int(padding_idx), int(bool(accumulate)), _DTYPES[dembed.dtype], _ptr(ws), ws.numel(), _stream())
+
+    def _check_loss(self, h, w, targets):
+        _check(h.dtype in (torch.float16, torch.bfloat16), 'h must be fp16 or bf16')
+        _check_typed(h, h, 'h')
+        _check_typed(w, h, 'w')
+        _check(h.dim() == 2 and w.dim() == 2 and w.size(1) == h.size(1) and w.size(0) > 0 and w.size(1) > 0,
+               'h must be [n, hidden], w [vocab, hidden]')
+        _check_ints(targets, h.size(0), h, 'targets')
+        return h.size(0), w.size(0), h.size(1)
+
+    def lm_head_loss_workspace(self, n, vocab):
+        return _workspace_bytes('fw_lm_head_loss_workspace', n, vocab)
+
+    def lm_head_loss(self, h, w, targets, loss, lse, ignore_index=-100, ws=None):
+        """loss[i] = lse[i] - h[i] . w[targets[i]] (0 where targets[i] == ignore_index), lse[i] = log sum_v
+        exp(h[i] . w[v]), both fp32 [n]; h, w fp16 or bf16. The logits are never stored."""
+        n, vocab, hidden = self._check_loss(h, w, targets)
+        for t, name in ((loss, 'loss'), (lse, 'lse')):
+            self._check_rows(t, n, h, name)
+        with _On(h.device):
+            ws = _workspace(ws, self.lm_head_loss_workspace(n, vocab), h.device)
+            _lib.call('fw_lm_head_loss', _ptr(h), _ptr(w), _ptr(targets), _ptr(loss), _ptr(lse), n, vocab, hidden,
+                      int(ignore_index), _DTYPES[h.dtype], _ptr(ws), ws.numel(), _stream())
+
+    @staticmethod
+    def _check_rows(t, n, like, name):
+        if not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == n
+                and t.device == like.device):
+            raise RuntimeError(f'{name} must be contiguous CUDA fp32 [{n}] on {like.device}')
+
+    def lm_head_loss_grad_workspace(self, n, vocab, hidden):
+        return _workspace_bytes('fw_lm_head_loss_grad_workspace', n, vocab, hidden)
+
+    def lm_head_loss_grad(self, h, w, targets, lse, g, dh, dw, ignore_index=-100, accumulate=False, ws=None):
+        """Gradient of sum_i g[i] loss[i] of lm_head_loss: dh like h, dw like w (either may be None); accumulate adds
+        to dw. lse is lm_head_loss's, g fp32 [n]."""
+        n, vocab, hidden = self._check_loss(h, w, targets)
+        for t, name in ((lse, 'lse'), (g, 'g')):
+            self._check_rows(t, n, h, name)
+        for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
+            if t is not None:
+                _check_typed(t, like, name)
+                _check(t.shape == like.shape, 'dh must be shaped like h, dw like w')
+        _check(dh is not None or dw is not None, 'at least one of dh and dw is required')
+        with _On(h.device):
+            ws = _workspace(ws, self.lm_head_loss_grad_workspace(n, vocab, hidden), h.device)
+            _lib.call('fw_lm_head_loss_grad', _ptr(h), _ptr(w), _ptr(targets), _ptr(lse), _ptr(g), _ptr(dh), _ptr(dw),
+                      n, vocab, hidden, int(ignore_index), int(bool(accumulate)), _DTYPES[h.dtype], _ptr(ws),
+                      ws.numel(), _stream())
 
     def decoder_step(self, desc, steps=1):
         _lib.call('fw_decoder_step', ctypes.byref(desc), int(steps), _stream())

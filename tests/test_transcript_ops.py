@@ -65,3 +65,48 @@ def test_embed_wrappers_refuse_cpu_tensors():
     assert ext.embed_grad_workspace(100, 64) > 0
     with pytest.raises(RuntimeError, match='bad sizes'):
         ext.embed_grad_workspace(-1, 64)
+
+
+@pytest.mark.parametrize('args,status,text', [
+    ((None, P, P, P, P, 4, 10, 64, -100, 0, P, 1 << 20, None), 1, 'required'),
+    ((P, P, P, None, P, 4, 10, 64, -100, 0, P, 1 << 20, None), 1, 'loss and lse'),
+    ((P, P, P, P, P, 4, 10, 60, -100, 0, P, 1 << 20, None), 2, 'multiple of 8'),
+    ((P, P, P, P, P, 4, 0, 64, -100, 0, P, 1 << 20, None), 2, 'n and vocab'),
+    ((P, P, P, P, P, (1 << 22) + 1, 10, 64, -100, 0, P, 1 << 20, None), 2, 'n and vocab'),
+    ((P, P, P, P, P, 4, 10, 64, -100, 2, P, 1 << 20, None), 4, 'dtype'),
+    ((P, ODD, P, P, P, 4, 10, 64, -100, 0, P, 1 << 20, None), 3, '16-byte aligned'),
+    ((P, P, P, P, P, 400, 1000, 64, -100, 0, P, 100, None), 2, 'workspace too small'),
+])
+def test_lm_head_loss_refuses(args, status, text):
+    _refused('fw_lm_head_loss', args, status, text)
+
+
+@pytest.mark.parametrize('args,status,text', [
+    ((P, P, P, None, P, P, P, 4, 10, 64, -100, 0, 0, P, 1 << 30, None), 1, 'lse and g'),
+    ((P, P, P, P, P, None, None, 4, 10, 64, -100, 0, 0, P, 1 << 30, None), 1, 'at least one of dh and dw'),
+    ((P, P, P, P, P, P, ODD, 4, 10, 64, -100, 0, 0, P, 1 << 30, None), 3, '16-byte aligned'),
+    ((P, P, P, P, P, P, P, 4, 10, 65544, -100, 0, 0, P, 1 << 30, None), 2, 'hidden'),
+    ((P, P, P, P, P, P, P, 4, 10, 64, -100, 0, 0, P, 100, None), 2, 'workspace too small'),
+])
+def test_lm_head_loss_grad_refuses(args, status, text):
+    _refused('fw_lm_head_loss_grad', args, status, text)
+
+
+def test_loss_wrappers_refuse():
+    ext = Ext()
+    h, t, f = torch.zeros(4, 64, dtype=torch.float16), torch.zeros(4, dtype=torch.long), torch.zeros(4)
+    with pytest.raises(RuntimeError, match='h must be contiguous CUDA float16'):
+        ext.lm_head_loss(h, h, t, f, f)
+    with pytest.raises(RuntimeError, match='h must be fp16 or bf16'):
+        ext.lm_head_loss_grad(h.float(), h, t, f, f, h, h)
+    assert ext.lm_head_loss_workspace(0, 10) == 0
+    assert ext.lm_head_loss_grad_workspace(100, 1000, 64) > 100 * 64 * 2
+    with pytest.raises(RuntimeError, match='n and vocab'):
+        ext.lm_head_loss_workspace(1, 0)
+
+
+def test_lm_head_loss_grad_scratch_is_bounded():
+    """A piece of the vocabulary at a time: the scratch does not grow with n * vocab."""
+    ext = Ext()
+    assert ext.lm_head_loss_grad_workspace(8192, 51866, 1280) < 200 << 20
+    assert ext.lm_head_loss_grad_workspace(65536, 51866, 1280) < 65536 * 51866  # half a byte a logit
