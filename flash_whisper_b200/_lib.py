@@ -65,6 +65,10 @@ class BatchDecoder(ctypes.Structure):
     ]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [('ptr', vp), ('token', c_int64), ('head', c_int64)]
+
+
 class EncoderLayer(ctypes.Structure):
     _fields_ = [(name, vp) for name in (
         'ln1_g', 'ln1_b', 'ln2_g', 'ln2_b', 'qkv_w', 'qkv_b', 'out_w', 'out_b', 'fc1_w', 'fc1_b', 'fc2_w', 'fc2_b')]
@@ -119,6 +123,9 @@ _SIGNATURES = {
     'fw_embed_scaled': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_float, c_int, vp]),
     'fw_embed_grad': (c_int, [vp, vp, vp, c_int, c_int, c_int, c_float, c_int64, c_int, c_int, vp, c_int64, vp]),
     'fw_embed_grad_workspace': (c_int, [c_int, c_int, i64p]),
+    'fw_prompt_attention': (c_int, [POINTER(Rows), POINTER(Rows), POINTER(Rows), POINTER(Rows), vp, vp, vp, c_int,
+                                    c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, vp, c_int64, vp]),
+    'fw_prompt_attention_workspace': (c_int, [c_int64, c_int64, c_int, c_int, c_int, i64p]),
     'fw_lm_head_loss': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, vp, c_int64, vp]),
     'fw_lm_head_loss_workspace': (c_int, [c_int, c_int, i64p]),
     'fw_lm_head_loss_grad': (c_int, [vp, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, c_int, vp,

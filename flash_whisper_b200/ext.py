@@ -350,6 +350,45 @@ class Ext:
             _lib.call('fw_embed_grad', _ptr(dout), _ptr(ids), _ptr(dembed), n, vocab, hidden, float(scale),
                       int(padding_idx), int(bool(accumulate)), _DTYPES[dembed.dtype], _ptr(ws), ws.numel(), _stream())
 
+    @staticmethod
+    def _rows(t, like, rows, heads, name):
+        """[rows, heads, 64] of like's type, strided over rows and heads, as a C descriptor."""
+        if not (t.is_cuda and t.dtype == like.dtype and t.device == like.device and t.dim() == 3
+                and t.shape == (rows, heads, HEAD_DIM) and (t.stride(2) == 1 or t.numel() == 0)):
+            raise RuntimeError(f'{name} must be CUDA {str(like.dtype)[6:]} [{rows}, {heads}, {HEAD_DIM}] on '
+                               f'{like.device}, its last dimension contiguous')
+        # a dimension of one element has no stride of its own
+        head = t.stride(1) if heads > 1 else HEAD_DIM
+        return _lib.Rows(t.data_ptr(), t.stride(0) if rows > 1 else heads * head, head)
+
+    def _check_prompt(self, q, k, v, cu_q, cu_k):
+        _check(q.dtype in (torch.float16, torch.bfloat16), 'q must be fp16 or bf16')
+        _check(q.dim() == 3 and k.dim() == 3, 'q and k must be [rows, heads, 64]')
+        (rows_q, heads), (rows_k, kv_heads) = q.shape[:2], k.shape[:2]
+        _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, 'heads must be a multiple of kv_heads')
+        seqs = max(cu_q.numel() - 1, 0)
+        _check_ints(cu_q, seqs + 1, q, 'cu_q')
+        _check_ints(cu_k, seqs + 1, q, 'cu_k')
+        return rows_q, rows_k, heads, kv_heads, seqs
+
+    def prompt_attention_workspace(self, rows_q, rows_k, seqs, heads, kv_heads):
+        return _workspace_bytes('fw_prompt_attention_workspace', rows_q, rows_k, seqs, heads, kv_heads)
+
+    def prompt_attention(self, q, k, v, out, cu_q, cu_k, scale, causal=True, lse=None, ws=None):
+        """Attention over packed sequences: q, out [rows_q, heads, 64], k, v [rows_k, kv_heads, 64] (fp16 or bf16, rows
+        and heads strided); sequence b has the rows cu_q[b]:cu_q[b + 1] and cu_k[b]:cu_k[b + 1] (int64). causal: the
+        last query sees the last key. lse: fp32 [heads, rows_q] or None."""
+        rows_q, rows_k, heads, kv_heads, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
+        rq, ro = self._rows(q, q, rows_q, heads, 'q'), self._rows(out, q, rows_q, heads, 'out')
+        rk, rv = self._rows(k, q, rows_k, kv_heads, 'k'), self._rows(v, q, rows_k, kv_heads, 'v')
+        if lse is not None:
+            self._check_rows(lse, heads * rows_q, q, 'lse')
+        with _On(q.device):
+            ws = _workspace(ws, self.prompt_attention_workspace(rows_q, rows_k, seqs, heads, kv_heads), q.device)
+            _lib.call('fw_prompt_attention', ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), ctypes.byref(ro),
+                      _ptr(lse), _ptr(cu_q), _ptr(cu_k), seqs, rows_q, rows_k, heads, kv_heads, float(scale),
+                      int(bool(causal)), _DTYPES[q.dtype], _ptr(ws), ws.numel(), _stream())
+
     def _check_loss(self, h, w, targets):
         _check(h.dtype in (torch.float16, torch.bfloat16), 'h must be fp16 or bf16')
         _check_typed(h, h, 'h')

@@ -404,6 +404,33 @@ int fw_embed_grad(const void* dout, const int64_t* ids, void* dembed, int n, int
                   fw_stream_t stream);
 int fw_embed_grad_workspace(int n, int hidden, int64_t* bytes);
 
+/* Packed rows of heads: [rows, heads, 64] of 16-bit elements, element (row, h, d) at
+ * ptr[row * token + h * head + d], so that q, k and v may be views of one projection's output.
+ * ptr on 16 bytes, strides multiples of 8. */
+typedef struct {
+  void* ptr;
+  int64_t token, head; /* strides in elements: from row to row, from head to head */
+} fw_rows_t;
+
+/* Attention over packed sequences: sequence b has the query rows cu_q[b] .. cu_q[b + 1] - 1 and the key
+ * rows cu_k[b] .. cu_k[b + 1] - 1 (int64 offsets on the device, seqs + 1 of each; the lengths may differ,
+ * and may be 0). Query head h reads key head h / (heads / kv_heads). With `causal` query i of a sequence
+ * sees the keys j <= i + lk - lq (the last query sees the last key: whole prompts, chunks behind a kept
+ * prefix, single tokens); without it all of its sequence's keys (cross attention).
+ *   out = softmax(scale * q . k) . v        lse (may be NULL) fp32 [heads, rows_q] = log of the softmax's sum
+ * Queries that see no key have out = 0 and lse = -inf. Rows that belong to no sequence are left as they
+ * are, and what they hold reaches no result; nor does one sequence's content reach another's. (Within a
+ * sequence a NaN or infinity in v reaches the 127 queries before it as well: the products run on tiles.)
+ * Offsets out of order or out of range set FW_DEVERR_BAD_INDEX and leave that sequence out. Scores, sums and
+ * outputs are fp32 until the one rounding of out; the probabilities are rounded to 16 bits (at most 2^8,
+ * relative to a running maximum) for their product with v. Replaces no reference kernel: the reference
+ * feeds its prompt token by token (custom/model.py:196-207). */
+int fw_prompt_attention(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t* v, const fw_rows_t* out, float* lse,
+                        const int64_t* cu_q, const int64_t* cu_k, int seqs, int64_t rows_q, int64_t rows_k, int heads,
+                        int kv_heads, float scale, int causal, int dtype, void* workspace, int64_t workspace_bytes,
+                        fw_stream_t stream);
+int fw_prompt_attention_workspace(int64_t rows_q, int64_t rows_k, int seqs, int heads, int kv_heads, int64_t* bytes);
+
 /* Softmax cross entropy of rows h [n, hidden] over the vocabulary matrix w [vocab, hidden] (the tied LM
  * head), in pieces of the vocabulary on tcgen05; the logits are never stored. With z = h . w^T (fp32):
  * lse[i] = log sum_v exp(z[i, v]), loss[i] = lse[i] - z[i, targets[i]] (minus the log probability of the
