@@ -126,6 +126,10 @@ _SIGNATURES = {
     'fw_prompt_attention': (c_int, [POINTER(Rows), POINTER(Rows), POINTER(Rows), POINTER(Rows), vp, vp, vp, c_int,
                                     c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, vp, c_int64, vp]),
     'fw_prompt_attention_workspace': (c_int, [c_int64, c_int64, c_int, c_int, c_int, i64p]),
+    'fw_prompt_attention_grad': (c_int, [POINTER(Rows)] * 5 + [vp, vp, vp, c_int, c_int64, c_int64, c_int, c_int,
+                                                               c_float, c_int, c_int] + [POINTER(Rows)] * 3 + [
+                                                                   vp, c_int64, vp]),
+    'fw_prompt_attention_grad_workspace': (c_int, [c_int64, c_int64, c_int, c_int, c_int, i64p]),
     'fw_lm_head_loss': (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, vp, c_int64, vp]),
     'fw_lm_head_loss_workspace': (c_int, [c_int, c_int, i64p]),
     'fw_lm_head_loss_grad': (c_int, [vp, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int64, c_int, c_int, vp,

@@ -48,6 +48,7 @@ struct Item {
   int64_t q0, k0;  // first rows of the sequence
   int lq, lk;
   int tile;        // index of the item within its sequence; -1: no such item
+  int seq;
 };
 
 // Finds item `index` (counting ceil(lq / per) items per sequence), by one warp. Sequences whose offsets are out of
@@ -78,6 +79,7 @@ __device__ __forceinline__ Item find_item(const int64_t* cu_a, const int64_t* cu
     const unsigned hit = __ballot_sync(0xffffffffu, index >= start && index < start + n);
     if (hit != 0) {
       const int src = __ffs(hit) - 1;
+      it.seq = b0 + src;
       it.tile = static_cast<int>(index - __shfl_sync(0xffffffffu, start, src));
       it.q0 = __shfl_sync(0xffffffffu, a0, src);
       it.lq = static_cast<int>(__shfl_sync(0xffffffffu, a1, src) - it.q0);
@@ -432,6 +434,406 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// Gradient
+//
+//   delta_i = do_i . o_i      p_ij = exp(s_ij - lse_i)      ds_ij = p_ij (do_i . v_j - delta_i)
+//   dv_j = sum_i p_ij do_i    dk_j = scale sum_i ds_ij q_i  dq_i = scale sum_j ds_ij k_j
+// (dv and dk summed over the heads of the group). prompt_delta_kernel writes {lse log2 e, delta} per row;
+// prompt_grad_kernel has CTAs of two roles, which share one pipeline, so that nothing is summed by atomics and
+// results do not vary: a key role owns 128 keys of a key head and walks the queries (64 tokens of one head a step), a
+// query role owns 128 (token, head) rows and walks the keys (64 a step). The probabilities are computed in both.
+//   first products:   X = A1 B1^T, Y = A2 B2^T       key role: A = K, V   B = Q, dO;    query role: A = Q, dO  B = K, V
+//   second products:  key role: dV += P^T dO, dK += dS^T Q;      query role: dQ += dS K
+// The A operands stay in tensor memory for the CTA's whole life, and P and dS are written over X and Y as the A
+// operands of the second products; from shared memory comes only a step's B tile pair, which serves both products
+// (K-major in the first, MN-major in the second). Two sets of X and Y: one softmax warpgroup works on each, the even
+// and the odd steps, while the tensor core works on the other.
+// fp16 range: P is kept times 2^8, and dS times 2^4 over the power of two of the largest |do| (of the row in the query
+// role, of the call in the key role), so that gradients of any size keep their bits; bf16 needs neither.
+constexpr int kStep = 64;                        // B rows of a step
+constexpr uint32_t kStepBytes = kStep * 64 * 2;  // 8 KB
+constexpr int kGradStages = 6;
+constexpr uint32_t kGradStage = 2 * kStepBytes;
+constexpr int kGradSmem = kGradStages * kGradStage + 1024;
+constexpr int kDeltaBlocks = 592;
+
+struct GradArgs {
+  PromptArgs p;
+  const void *q, *k, *v, *o, *dout;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, d_token, d_head;
+  void *dq, *dk, *dv;
+  int64_t dq_token, dq_head, dk_token, dk_head, dv_token, dv_head;
+  float2* stat;       // [heads][stat_rows]: {lse log2 e, delta}; a sequence's rows start at stat_start()
+  int64_t stat_rows;
+  float* largest;     // [kDeltaBlocks]: largest finite |do| each block met
+  int64_t key_items;  // CTAs of the key role
+  float scale;
+};
+
+// First row of sequence `seq` in stat: a multiple of 4 (16 bytes at least), behind the previous sequence's rows.
+__device__ __forceinline__ int64_t stat_start(int64_t q0, int seq) { return ((q0 + 3) / 4 + seq) * 4; }
+
+template <typename T>
+__global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
+  __shared__ float s_max[8];
+  pdl_trigger();
+  const PromptArgs& a = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t units = a.rows_q * a.heads;
+  float big = 0.f;
+  for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; u0 < units; u0 += static_cast<int64_t>(gridDim.x) * 32) {
+    const int64_t u = u0 + (lane >> 3);
+    float dot = 0.f;
+    bool mine = u < units;
+    int64_t row = 0, q0 = 0;
+    int head = 0, seq = 0;
+    if (mine) {
+      row = u / a.heads;
+      head = static_cast<int>(u % a.heads);
+      int lo = 0, hi = a.seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu_q[mid] <= row)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      seq = lo;
+      q0 = a.cu_q[lo];
+      mine = q0 >= 0 && q0 <= row && row < a.cu_q[lo + 1];  // rows of no sequence may hold anything
+    }
+    if (mine) {
+      const uint4 d = reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + row * g.d_token + head * g.d_head)[lane & 7];
+      const uint4 o = reinterpret_cast<const uint4*>(static_cast<const T*>(g.o) + row * g.o_token + head * g.o_head)[lane & 7];
+      const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = Type16<T>::unpack(dw[i]), y = Type16<T>::unpack(ow[i]);
+        dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
+        if (fabsf(x.x) < INFINITY) big = fmaxf(big, fabsf(x.x));
+        if (fabsf(x.y) < INFINITY) big = fmaxf(big, fabsf(x.y));
+      }
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (mine && (lane & 7) == 0)
+      g.stat[head * g.stat_rows + stat_start(q0, seq) + row - q0] = make_float2(a.lse[head * a.rows_q + row] * kLog2, dot);
+  }
+  big = warp_max(big);
+  if (lane == 0) s_max[warp] = big;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) big = fmaxf(big, s_max[w]);
+    g.largest[blockIdx.x] = big;
+  }
+}
+
+// The power of two that takes x into [1, 2); 1 for 0, and within what fp32 holds.
+__device__ __forceinline__ float normalizer(float x) {
+  const int e = static_cast<int>(__float_as_uint(x) >> 23);  // x >= 0 and finite
+  return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    prompt_grad_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmD,
+                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GradArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(16) float2 s_stat[kGradStages][kStep];
+  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], p_full[2], a_ready, done;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ Item s_item;
+  __shared__ float s_norm, s_row_norm[kRows];
+  const PromptArgs& a = g.p;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool keys = blockIdx.x < g.key_items;  // the role
+  const int64_t index = keys ? blockIdx.x : blockIdx.x - g.key_items;
+  const int kvh = static_cast<int>(index % a.kv_heads);
+
+  if (warp == 8) tmem_alloc(&tmem_base_sh, 512);
+  if (warp == 9) {
+    const Item it = keys ? find_item(a.cu_k, a.cu_q, a.rows_k, a.rows_q, a.seqs, kRows, index / a.kv_heads, lane)
+                         : find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, index / a.kv_heads, lane);
+    if (lane == 0) {
+      s_item = it;
+      for (int i = 0; i < kGradStages; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 1);
+      }
+      mbar_init(&landed, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&x_full[i], 1);  // X and Y of the set's next step are in tensor memory
+        mbar_init(&p_full[i], 4);  // P and dS are
+      }
+      mbar_init(&a_ready, 8);
+      mbar_init(&done, 1);
+      mbar_fence_init();
+      tma_prefetch_desc(keys ? &tmQ : &tmK);
+      tma_prefetch_desc(keys ? &tmD : &tmV);
+    }
+  }
+  pdl_wait();
+  if (warp == 8 && !Type16<T>::kBf16) {
+    float m = 0.f;
+    for (int i = lane; i < kDeltaBlocks; i += 32) m = fmaxf(m, g.largest[i]);
+    m = warp_max(m);
+    if (lane == 0) s_norm = normalizer(m);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  Item it = s_item;
+  if (it.tile >= 0) {
+    if (keys) {  // find_item was asked with the roles of q and k swapped
+      const int64_t r = it.q0;
+      const int n = it.lq;
+      it.q0 = it.k0, it.lq = it.lk;
+      it.k0 = r, it.lk = n;
+    }
+    const int shift = it.lk - it.lq;
+    // Key role: keys first .. first + 127, token blocks from `begin` on for each head of the group. Query role: tokens
+    // from `first` on, all key blocks that the last of them sees.
+    int first, begin, per_head, steps;
+    if (keys) {
+      first = it.tile * kRows;
+      begin = a.causal ? max(0, first - shift) / kStep : 0;
+      per_head = max(0, (it.lq + kStep - 1) / kStep - begin);
+      steps = per_head * a.group;
+    } else {
+      const int items = (it.lq + a.tokens - 1) / a.tokens;
+      first = (a.causal ? items - 1 - it.tile : it.tile) * a.tokens;  // causal: the longest first
+      const int last = min(it.lq, first + a.tokens) - 1;
+      begin = 0;
+      per_head = steps = ((a.causal ? max(0, min(it.lk, last + shift + 1)) : it.lk) + kStep - 1) / kStep;
+    }
+
+    if (warp == 9) {
+      // ---- loads
+      bool ok = true;
+      uint32_t cut = 0;  // tiles that end inside a step so far
+      for (int j = 0; j < steps && ok; ++j) {
+        const int s = j % kGradStages;
+        const int head = keys ? kvh * a.group + j / per_head : kvh;
+        const int at = (begin + (keys ? j % per_head : j)) * kStep;
+        const int valid = (keys ? it.lq : it.lk) - at;
+        const int row = static_cast<int>(keys ? it.q0 : it.k0) + at;
+        uint8_t* dst = smem + s * kGradStage;
+        if (lane == 0) {
+          if (j >= kGradStages) ok = mbar_wait(&empty[s], ((j / kGradStages) & 1u) ^ 1u);
+          if (ok) {
+            uint64_t* bar = valid >= kStep ? &full[s] : &landed;
+            mbar_arrive_expect_tx(bar, kGradStage + (keys ? kStep * 8 : 0));
+            tma_load_3d(dst, keys ? &tmQ : &tmK, bar, 0, head, row);
+            tma_load_3d(dst + kStepBytes, keys ? &tmD : &tmV, bar, 0, head, row);
+            if (keys)
+              bulk_g2s(s_stat[s], g.stat + head * g.stat_rows + stat_start(it.q0, it.seq) + at, kStep * 8, bar);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (ok && valid < kStep) {
+          // Rows behind the sequence's end may hold anything, and 0 x NaN must not reach a sum over them.
+          ok = mbar_wait_warp(&landed, cut & 1u);
+          ++cut;
+          for (int i = valid * 8 + lane; i < kStep * 8; i += 32) {
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
+            reinterpret_cast<uint4*>(dst + kStepBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+        if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
+      }
+    } else if (warp == 8) {
+      // ---- products
+      if (lane == 0 && steps > 0) {
+        constexpr uint32_t idesc1 = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+        constexpr uint32_t idesc2 = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
+        bool ok = mbar_wait(&a_ready, 0);
+        tc_fence_after();
+        for (int j = -1; j < steps && ok; ++j) {
+          if (j + 1 < steps) {
+            // X and Y of step j + 1, into the set that step j - 1 used: its second products were issued before
+            const int s = (j + 1) % kGradStages, set = (j + 1) & 1;
+            ok = mbar_wait(&full[s], ((j + 1) / kGradStages) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t b1 = sw128_desc(base + s * kGradStage), b2 = sw128_desc(base + s * kGradStage + kStepBytes);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_ta(tmem + set * 128, tmem + 384 + 8 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_ta(tmem + set * 128 + 64, tmem + 416 + 8 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+            tc_commit(&x_full[set]);
+          }
+          if (j < 0) continue;
+          const int s = j % kGradStages, set = j & 1;
+          ok = mbar_wait(&p_full[set], (j >> 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b1 = sw128_mn_desc(base + s * kGradStage, kStepBytes);
+          const uint64_t b2 = sw128_mn_desc(base + s * kGradStage + kStepBytes, kStepBytes);
+          if (keys) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_ta(tmem + 256, tmem + set * 128 + 8 * kk, b2 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_ta(tmem + 320, tmem + set * 128 + 64 + 8 * kk, b1 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
+          tc_commit(&empty[s]);
+        }
+        tc_commit(&done);
+        if (!ok) prompt_flag(FW_DEVERR_TIMEOUT);
+      }
+    } else {
+      // ---- softmax: thread = row of the A operands (both warpgroups), steps of its warpgroup's parity
+      const int wg = warp >> 2;
+      const int r = (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const int token = keys ? 0 : first + r / a.group;
+      const int head = keys ? kvh : kvh * a.group + r % a.group;
+      const bool live = keys ? first + r < it.lk : r < a.tokens * a.group && token < it.lq;
+      const int64_t row = keys ? it.k0 + first + r : it.q0 + token;
+      float lse2 = 0.f, delta = 0.f;
+      // A1 (warpgroup 0) and A2 (warpgroup 1) into tensor memory
+      {
+        const T* src = static_cast<const T*>(keys ? (wg == 0 ? g.k : g.v) : (wg == 0 ? g.q : g.dout));
+        const int64_t ts = keys ? (wg == 0 ? g.k_token : g.v_token) : (wg == 0 ? g.q_token : g.d_token);
+        const int64_t hs = keys ? (wg == 0 ? g.k_head : g.v_head) : (wg == 0 ? g.q_head : g.d_head);
+        uint32_t x[32];
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (live) v = reinterpret_cast<const uint4*>(src + row * ts + head * hs)[i];
+          x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+        }
+        if (!Type16<T>::kBf16 && !keys && wg == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float2 v = Type16<T>::unpack(x[i]);
+            if (fabsf(v.x) < INFINITY) big = fmaxf(big, fabsf(v.x));
+            if (fabsf(v.y) < INFINITY) big = fmaxf(big, fabsf(v.y));
+          }
+          s_row_norm[r] = normalizer(big);
+        }
+        tc_store32(tmem + lanes + 384 + 32 * wg, x);
+        tc_wait_store();
+        if (!keys && live) {
+          const float2 st = g.stat[head * g.stat_rows + stat_start(it.q0, it.seq) + token];
+          lse2 = st.x;
+          delta = st.y;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_ready);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // s_row_norm
+      constexpr float kP = Type16<T>::kBf16 ? 0.f : 8.f;  // log2 of the factor that P carries
+      const float norm = Type16<T>::kBf16 ? 1.f : 0.0625f * (keys ? s_norm : s_row_norm[r]);  // of dS besides P's
+      const int limit = keys ? 0 : a.causal ? min(it.lk - 1, token + shift) : it.lk - 1;
+      const float c = a.scale_log2;
+      const uint32_t tx = tmem + lanes + wg * 128;
+      bool ok = true;
+      int used = 0;
+      for (int j = wg; j < steps; j += 2, ++used) {
+        ok = mbar_wait_warp(&x_full[wg], used & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        const int at = (begin + (keys ? j % per_head : j)) * kStep;
+        const float2* st = s_stat[j % kGradStages];
+        // columns [lo, hi) of the step count for this row
+        int lo = 0, hi = kStep;
+        if (keys) {
+          hi = it.lq - at;
+          if (a.causal) lo = first + r - shift - at;
+        } else {
+          hi = limit + 1 - at;
+        }
+        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < kStep);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[32], y[32], p[16], d[16];
+          tc_load32(tx + 32 * h, x);
+          tc_load32(tx + 64 + 32 * h, y);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float4 two = make_float4(lse2, delta, lse2, delta);
+            if (keys) two = *reinterpret_cast<const float4*>(&st[32 * h + i]);
+            float p0 = ex2(fmaf(__uint_as_float(x[i]), c, kP - two.x));
+            float p1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, kP - two.z));
+            float d0 = p0 * ((__uint_as_float(y[i]) - two.y) * norm);
+            float d1 = p1 * ((__uint_as_float(y[i + 1]) - two.w) * norm);
+            if (cut) {
+              const int k = 32 * h + i;
+              const bool in0 = k >= lo && k < hi, in1 = k + 1 >= lo && k + 1 < hi;
+              p0 = in0 ? p0 : 0.f, d0 = in0 ? d0 : 0.f;
+              p1 = in1 ? p1 : 0.f, d1 = in1 ? d1 : 0.f;
+            }
+            p[i >> 1] = Type16<T>::pack(p0, p1);
+            d[i >> 1] = Type16<T>::pack(d0, d1);
+          }
+          // over X and Y: columns 16 h .. + 15 hold what has been read (h = 0) or is in registers by now
+          if (keys) tc_store16(tx + 16 * h, p);
+          tc_store16(tx + 64 + 16 * h, d);
+        }
+        tc_wait_store();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[wg]);
+      }
+      if (ok && steps > 0) ok = mbar_wait_warp(&done, 0);
+      if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
+      // ---- results: key role: warpgroup 0 dK, 1 dV; query role: warpgroup 0 dQ
+      if (ok && (keys || wg == 0)) {
+        tc_fence_after();
+        const bool dv = keys && wg == 1;
+        uint32_t x[2][32];
+        if (steps > 0) {
+          tc_load32(tmem + lanes + (dv ? 256 : 320), x[0]);
+          tc_load32(tmem + lanes + (dv ? 288 : 352), x[1]);
+          tc_wait_ld();
+        }
+        if (live) {
+          constexpr float kUnP = Type16<T>::kBf16 ? 1.f : 1.f / 256.f;
+          const float f = dv ? kUnP : g.scale * kUnP / norm;
+          T* dst = static_cast<T*>(keys ? (dv ? g.dv : g.dk) : g.dq) +
+                   row * (keys ? (dv ? g.dv_token : g.dk_token) : g.dq_token) +
+                   head * (keys ? (dv ? g.dv_head : g.dk_head) : g.dq_head);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int e = 8 * i + 2 * k;
+              w[k] = steps > 0 ? Type16<T>::pack(__uint_as_float(x[e >> 5][e & 31]) * f,
+                                                 __uint_as_float(x[e >> 5][(e & 31) + 1]) * f)
+                               : 0u;
+            }
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
 // Host side
 // Splits of the keys: none when the query tiles fill the SMs; else as many as make two CTAs an SM, up to one per key
 // block of an average sequence. From sizes only (the offsets are on the device).
@@ -479,6 +881,44 @@ static int run_prompt(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v
   if (rc || a.splits == 1) return rc;
   e = launch(prompt_join_kernel<T>, dim3(static_cast<unsigned>((a.rows_q * a.heads + 3) / 4)), dim3(128), 0, s, true, a);
   return launch_status(e, "prompt_attention join");
+}
+
+template <typename T>
+static int run_prompt_grad(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v, const fw_rows_t& d, GradArgs g,
+                           cudaStream_t s) {
+  const PromptArgs& a = g.p;
+  const int64_t query_items = a.rows_q > 0 ? (a.rows_q / a.tokens + a.seqs) * a.kv_heads : 0;
+  g.key_items = a.rows_k > 0 ? (a.rows_k / kRows + a.seqs) * a.kv_heads : 0;
+  FW_REQUIRE(query_items + g.key_items < (int64_t(1) << 31), FW_ERR_SHAPE, "prompt_attention_grad: too many tiles");
+  if (query_items + g.key_items == 0) return FW_OK;
+  if (a.rows_q > 0) {
+    cudaError_t e = launch(prompt_delta_kernel<T>, dim3(kDeltaBlocks), dim3(256), 0, s, false, g);
+    const int rc = launch_status(e, "prompt_attention_grad delta");
+    if (rc) return rc;
+  }
+  CUtensorMap tq{}, td{}, tk{}, tv{};
+  int rc = FW_OK;
+  if (a.rows_q > 0) {
+    rc = make_rows_map(&tq, Type16<T>::kMap, q.ptr, a.rows_q, a.heads, q.token, q.head, 1, kStep);
+    if (!rc) rc = make_rows_map(&td, Type16<T>::kMap, d.ptr, a.rows_q, a.heads, d.token, d.head, 1, kStep);
+  }
+  if (!rc && a.rows_k > 0) {
+    rc = make_rows_map(&tk, Type16<T>::kMap, k.ptr, a.rows_k, a.kv_heads, k.token, k.head, 1, kStep);
+    if (!rc) rc = make_rows_map(&tv, Type16<T>::kMap, v.ptr, a.rows_k, a.kv_heads, v.token, v.head, 1, kStep);
+  }
+  if (rc) return rc;
+  if (a.rows_q == 0) tq = tk, td = tv;  // nothing is read through them
+  if (a.rows_k == 0) tk = tq, tv = td;
+  auto kern = prompt_grad_kernel<T>;
+  cudaError_t e = ensure_smem(kern, kGradSmem);
+  if (e == cudaSuccess)
+    e = launch(kern, dim3(static_cast<unsigned>(g.key_items + query_items)), dim3(kFwdThreads), kGradSmem, s,
+               a.rows_q > 0, tq, td, tk, tv, g);
+  return launch_status(e, "prompt_attention_grad");
+}
+
+static int64_t grad_stat_rows(int64_t rows_q, int seqs) {  // room for a step's copy behind the last row
+  return (rows_q + 3) / 4 * 4 + 4 * static_cast<int64_t>(seqs) + 4 + kStep;
 }
 
 static int check_rows(const char* what, const char* name, const fw_rows_t& x, int heads, int64_t rows) {
@@ -565,6 +1005,73 @@ int fw_prompt_attention(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t*
   a.part_lse = a.part_o + static_cast<int64_t>(a.splits) * rows_q * heads * 64;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == FW_F16 ? run_prompt<half>(*q, *k, *v, a, s) : run_prompt<__nv_bfloat16>(*q, *k, *v, a, s);
+}
+
+int fw_prompt_attention_grad_workspace(int64_t rows_q, int64_t rows_k, int seqs, int heads, int kv_heads,
+                                       int64_t* bytes) {
+  FW_REQUIRE(bytes != nullptr, FW_ERR_NULL, "prompt_attention_grad_workspace: bytes is NULL");
+  int rc = check_prompt("prompt_attention_grad", bytes, bytes, seqs, rows_q, rows_k, heads, kv_heads, 1.f, FW_F16);
+  if (rc) return rc;
+  *bytes = kDeltaBlocks * 4 + heads * grad_stat_rows(rows_q, seqs) * 8;
+  return FW_OK;
+}
+
+int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t* v, const fw_rows_t* out,
+                             const fw_rows_t* dout, const float* lse, const int64_t* cu_q, const int64_t* cu_k,
+                             int seqs, int64_t rows_q, int64_t rows_k, int heads, int kv_heads, float scale, int causal,
+                             int dtype, const fw_rows_t* dq, const fw_rows_t* dk, const fw_rows_t* dv, void* workspace,
+                             int64_t workspace_bytes, fw_stream_t stream) {
+  const char* what = "prompt_attention_grad";
+  FW_REQUIRE(q && k && v && out && dout && dq && dk && dv, FW_ERR_NULL,
+             "%s: q, k, v, out, dout, dq, dk and dv are required", what);
+  int rc = check_prompt(what, cu_q, cu_k, seqs, rows_q, rows_k, heads, kv_heads, scale, dtype);
+  if (!rc) rc = check_rows(what, "q", *q, heads, rows_q);
+  if (!rc) rc = check_rows(what, "k", *k, kv_heads, rows_k);
+  if (!rc) rc = check_rows(what, "v", *v, kv_heads, rows_k);
+  if (!rc) rc = check_rows(what, "out", *out, heads, rows_q);
+  if (!rc) rc = check_rows(what, "dout", *dout, heads, rows_q);
+  if (!rc) rc = check_rows(what, "dq", *dq, heads, rows_q);
+  if (!rc) rc = check_rows(what, "dk", *dk, kv_heads, rows_k);
+  if (!rc) rc = check_rows(what, "dv", *dv, kv_heads, rows_k);
+  if (rc) return rc;
+  int64_t need = 0;
+  rc = fw_prompt_attention_grad_workspace(rows_q, rows_k, seqs, heads, kv_heads, &need);
+  if (rc) return rc;
+  if (seqs == 0) return FW_OK;
+  FW_REQUIRE(lse || rows_q == 0, FW_ERR_NULL, "%s: lse is required", what);
+  FW_REQUIRE(workspace && aligned16(workspace), FW_ERR_ALIGN, "%s: a 16-byte aligned workspace is required", what);
+  FW_REQUIRE(workspace_bytes >= need, FW_ERR_SHAPE, "%s: workspace too small (%lld of %lld bytes)", what,
+             static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  GradArgs g{};
+  PromptArgs& a = g.p;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.seqs = seqs;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.group = heads / kv_heads;
+  a.tokens = kRows / a.group;
+  a.rows_q = rows_q;
+  a.rows_k = rows_k;
+  a.scale_log2 = scale * kLog2;
+  a.causal = causal != 0;
+  a.splits = 1;
+  a.lse = const_cast<float*>(lse);
+  g.q = q->ptr, g.q_token = q->token, g.q_head = q->head;
+  g.k = k->ptr, g.k_token = k->token, g.k_head = k->head;
+  g.v = v->ptr, g.v_token = v->token, g.v_head = v->head;
+  g.o = out->ptr, g.o_token = out->token, g.o_head = out->head;
+  g.dout = dout->ptr, g.d_token = dout->token, g.d_head = dout->head;
+  g.dq = dq->ptr, g.dq_token = dq->token, g.dq_head = dq->head;
+  g.dk = dk->ptr, g.dk_token = dk->token, g.dk_head = dk->head;
+  g.dv = dv->ptr, g.dv_token = dv->token, g.dv_head = dv->head;
+  g.largest = static_cast<float*>(workspace);
+  g.stat = reinterpret_cast<float2*>(g.largest + kDeltaBlocks);
+  g.stat_rows = grad_stat_rows(rows_q, seqs);
+  g.scale = scale;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == FW_F16 ? run_prompt_grad<half>(*q, *k, *v, *dout, g, s)
+                         : run_prompt_grad<__nv_bfloat16>(*q, *k, *v, *dout, g, s);
 }
 
 }  // extern "C"

@@ -72,6 +72,13 @@ __device__ __forceinline__ void tc_store32(uint32_t taddr, const uint32_t (&r)[3
       FW_R8(r, 0), FW_R8(r, 8), FW_R8(r, 16), FW_R8(r, 24)
       : "memory");
 }
+__device__ __forceinline__ void tc_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      FW_R8(r, 0), FW_R8(r, 8)
+      : "memory");
+}
 #undef FW_R8
 __device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

@@ -389,6 +389,24 @@ class Ext:
                       _ptr(lse), _ptr(cu_q), _ptr(cu_k), seqs, rows_q, rows_k, heads, kv_heads, float(scale),
                       int(bool(causal)), _DTYPES[q.dtype], _ptr(ws), ws.numel(), _stream())
 
+    def prompt_attention_grad_workspace(self, rows_q, rows_k, seqs, heads, kv_heads):
+        return _workspace_bytes('fw_prompt_attention_grad_workspace', rows_q, rows_k, seqs, heads, kv_heads)
+
+    def prompt_attention_grad(self, q, k, v, out, dout, lse, cu_q, cu_k, scale, dq, dk, dv, causal=True, ws=None):
+        """Gradient of prompt_attention: dq like q, dk and dv like k and v, for dout, from the forward's out and lse."""
+        rows_q, rows_k, heads, kv_heads, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
+        rq, ro, rd, rdq = (self._rows(t, q, rows_q, heads, name)
+                           for t, name in ((q, 'q'), (out, 'out'), (dout, 'dout'), (dq, 'dq')))
+        rk, rv, rdk, rdv = (self._rows(t, q, rows_k, kv_heads, name)
+                            for t, name in ((k, 'k'), (v, 'v'), (dk, 'dk'), (dv, 'dv')))
+        self._check_rows(lse, heads * rows_q, q, 'lse')
+        ref = ctypes.byref
+        with _On(q.device):
+            ws = _workspace(ws, self.prompt_attention_grad_workspace(rows_q, rows_k, seqs, heads, kv_heads), q.device)
+            _lib.call('fw_prompt_attention_grad', ref(rq), ref(rk), ref(rv), ref(ro), ref(rd), _ptr(lse), _ptr(cu_q),
+                      _ptr(cu_k), seqs, rows_q, rows_k, heads, kv_heads, float(scale), int(bool(causal)),
+                      _DTYPES[q.dtype], ref(rdq), ref(rdk), ref(rdv), _ptr(ws), ws.numel(), _stream())
+
     def _check_loss(self, h, w, targets):
         _check(h.dtype in (torch.float16, torch.bfloat16), 'h must be fp16 or bf16')
         _check_typed(h, h, 'h')

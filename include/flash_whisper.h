@@ -431,6 +431,20 @@ int fw_prompt_attention(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t*
                         fw_stream_t stream);
 int fw_prompt_attention_workspace(int64_t rows_q, int64_t rows_k, int seqs, int heads, int kv_heads, int64_t* bytes);
 
+/* Gradient of fw_prompt_attention: dq, dk and dv for dout (all as the forward's rows), from its out and lse.
+ * dk and dv are summed over the heads of a group in a fixed order (no atomics: results do not vary from run
+ * to run). Every row of a sequence is written (0 where nothing is seen), rows of no sequence are left as
+ * they are and what they hold reaches no result. Between the products, the probabilities and their
+ * gradients are rounded to 16 bits (in fp16 scaled by powers of two, so that small gradients keep their
+ * bits); sums are fp32. */
+int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t* v, const fw_rows_t* out,
+                             const fw_rows_t* dout, const float* lse, const int64_t* cu_q, const int64_t* cu_k,
+                             int seqs, int64_t rows_q, int64_t rows_k, int heads, int kv_heads, float scale, int causal,
+                             int dtype, const fw_rows_t* dq, const fw_rows_t* dk, const fw_rows_t* dv, void* workspace,
+                             int64_t workspace_bytes, fw_stream_t stream);
+int fw_prompt_attention_grad_workspace(int64_t rows_q, int64_t rows_k, int seqs, int heads, int kv_heads,
+                                       int64_t* bytes);
+
 /* Softmax cross entropy of rows h [n, hidden] over the vocabulary matrix w [vocab, hidden] (the tied LM
  * head), in pieces of the vocabulary on tcgen05; the logits are never stored. With z = h . w^T (fp32):
  * lse[i] = log sum_v exp(z[i, v]), loss[i] = lse[i] - z[i, targets[i]] (minus the log probability of the

@@ -110,3 +110,66 @@ def test_lm_head_loss_grad_scratch_is_bounded():
     ext = Ext()
     assert ext.lm_head_loss_grad_workspace(8192, 51866, 1280) < 200 << 20
     assert ext.lm_head_loss_grad_workspace(65536, 51866, 1280) < 65536 * 51866  # half a byte a logit
+
+
+def _rows(ptr=256, token=640, head=64):
+    return ctypes.byref(_lib.Rows(ptr, token, head))
+
+
+def _attn(**changed):
+    a = dict(q=_rows(), k=_rows(), v=_rows(), out=_rows(), lse=P, cu_q=P, cu_k=P, seqs=2, rows_q=100, rows_k=100,
+             heads=10, kv_heads=10, scale=0.125, causal=1, dtype=0, ws=P, ws_bytes=1 << 40)
+    assert set(changed) <= set(a)
+    a.update(changed)
+    return (*a.values(), None)
+
+
+def _attn_grad(**changed):
+    a = dict(q=_rows(), k=_rows(), v=_rows(), out=_rows(), dout=_rows(), lse=P, cu_q=P, cu_k=P, seqs=2, rows_q=100,
+             rows_k=100, heads=10, kv_heads=10, scale=0.125, causal=1, dtype=0, dq=_rows(), dk=_rows(), dv=_rows(),
+             ws=P, ws_bytes=1 << 40)
+    assert set(changed) <= set(a)
+    a.update(changed)
+    return (*a.values(), None)
+
+
+@pytest.mark.parametrize('changed,status,text', [
+    (dict(q=None), 1, 'required'), (dict(k=_rows(ptr=0)), 1, 'k is required'), (dict(cu_k=None), 1, 'cu_q and cu_k'),
+    (dict(seqs=-1), 2, 'bad sizes'), (dict(rows_k=1 << 30), 2, 'bad sizes'), (dict(kv_heads=3), 2, 'multiple of kv_heads'),
+    (dict(heads=0), 2, 'multiple of kv_heads'), (dict(heads=1290, kv_heads=10), 2, 'at most 128 times'),
+    (dict(scale=0.0), 4, 'positive'), (dict(scale=-1.0), 4, 'positive'), (dict(scale=float('nan')), 4, 'positive'),
+    (dict(scale=float('inf')), 4, 'positive'), (dict(dtype=2), 4, 'dtype'), (dict(v=_rows(ptr=264)), 3, '16 bytes'),
+    (dict(q=_rows(token=644)), 3, 'multiple of 8'), (dict(k=_rows(head=32)), 2, 'overlapping'),
+    (dict(v=_rows(token=64, head=64)), 2, 'overlapping'), (dict(k=_rows(token=-640)), 2, 'overlapping'),
+])
+def test_prompt_attention_refuses(changed, status, text):
+    _refused('fw_prompt_attention', _attn(**changed), status, text)
+    _refused('fw_prompt_attention_grad', _attn_grad(**changed), status, text)
+
+
+def test_prompt_attention_refuses_small_workspaces():
+    _refused('fw_prompt_attention', _attn(rows_q=2, ws_bytes=10, rows_k=4096, heads=1, kv_heads=1), 2, 'workspace too')
+    _refused('fw_prompt_attention', _attn(rows_q=2, ws=None, rows_k=4096, heads=1, kv_heads=1), 3, 'workspace')
+    _refused('fw_prompt_attention_grad', _attn_grad(ws_bytes=10), 2, 'workspace too')
+    _refused('fw_prompt_attention_grad', _attn_grad(ws=None), 3, 'workspace')
+    _refused('fw_prompt_attention_grad', _attn_grad(lse=None), 1, 'lse')
+    _refused('fw_prompt_attention_grad', _attn_grad(dk=_rows(ptr=8)), 3, 'dk must start')
+
+
+def test_prompt_wrappers_refuse():
+    ext = Ext()
+    q, cu = torch.zeros(4, 2, 64, dtype=torch.float16), torch.tensor([0, 4])
+    with pytest.raises(RuntimeError, match='cu_q must be contiguous CUDA int64'):
+        ext.prompt_attention(q, q, q, q, cu, cu, 0.1)
+    with pytest.raises(RuntimeError, match='q must be fp16 or bf16'):
+        ext.prompt_attention(q.float(), q, q, q, cu, cu, 0.1)
+    with pytest.raises(RuntimeError, match='multiple of kv_heads'):
+        ext.prompt_attention_grad(q, torch.zeros(4, 3, 64), q, q, q, q, cu, cu, 0.1, q, q, q)
+    with pytest.raises(RuntimeError, match='rows, heads, 64'):
+        ext.prompt_attention(q[0], q, q, q, cu, cu, 0.1)
+    assert ext.prompt_attention_workspace(11173, 11173, 6, 32, 8) == 0  # enough query tiles: no key splits
+    assert ext.prompt_attention_workspace(1, 4096, 1, 1, 1) > 0  # one token: the keys are split
+
+
+def test_rows_struct_matches_header():
+    assert ctypes.sizeof(_lib.Rows) == 24 and _lib.Rows.token.offset == 8 and _lib.Rows.head.offset == 16
