@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
   const int tiles = tile_count<kKind>(a);
@@ -206,37 +206,36 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {  // the whole warp runs the loop, one lane issues
       int it = 0, local = 0;
       bool ok = true;
       for (int t = first; t < tiles && ok; t += pairs, ++local) {
         const Tile x = tile_at<kKind>(a, t);
         const int buf = local & 1;
-        if (local >= 2 && !mbar_wait(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u)) {
-          loss_flag(FW_DEVERR_TIMEOUT);
-          ok = false;
-        }
+        if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
         tc_fence_after();
         const uint32_t d = tmem + buf * kBN;
         for (int kb = 0; kb < x.kbs && ok; ++kb, ++it) {
           const int s = it % kStages;
-          if (!mbar_wait(&full_bar[s], (it / kStages) & 1u)) {
-            loss_flag(FW_DEVERR_TIMEOUT);
-            ok = false;
-            break;
-          }
+          ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u);
+          if (!ok) break;
           tc_fence_after();
           const uint32_t at = base + s * kStageBytes;
-          if (kKind != kGrads)
-            mma_block<T, false, false>(d, at, kb == 0);
-          else if (x.dh)
-            mma_block<T, false, true>(d, at, kb == 0);
-          else
-            mma_block<T, true, true>(d, at, kb == 0);
-          tc_commit_pair(&empty_bar[s]);
+          if (elect_one()) {
+            if (kKind != kGrads)
+              mma_block<T, false, false>(d, at, kb == 0);
+            else if (x.dh)
+              mma_block<T, false, true>(d, at, kb == 0);
+            else
+              mma_block<T, true, true>(d, at, kb == 0);
+            tc_commit_pair(&empty_bar[s]);
+          }
+          __syncwarp();
         }
-        tc_commit_pair(&acc_full[buf]);
+        if (elect_one()) tc_commit_pair(&acc_full[buf]);
+        __syncwarp();
       }
+      if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
     }
   } else {
     // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns

@@ -5,8 +5,7 @@
 //   sees the last key)        lse_i = log sum_j exp s_ij        o_i = sum_j exp(s_ij - lse_i) v_j
 // A query that sees no key has o = 0 and lse = -inf.
 //
-// Forward (prompt_attn_kernel): a CTA takes two tiles of 128 query rows of one sequence and one key head. The rows of
-// a tile are (token, head of the group) pairs, tokens major, so that one read of K and V serves the whole group and a
+// Forward (prompt_attn_kernel): a CTA takes 128 query rows of one sequence and one key head. The rows of a tile are (token, head of the group) pairs, tokens major, so that one read of K and V serves the whole group and a
 // single token of a grouped model still fills several rows. S = Q K^T and O += P V run on tcgen05 with S, P and O in
 // tensor memory (P, 16 bits, is the A operand from there: it never passes through shared memory); one thread owns a
 // row, so maximum and sum need no exchange. S has a buffer of its own besides P: the next block's Q K^T runs while the
@@ -26,9 +25,9 @@ __device__ __forceinline__ void prompt_flag(unsigned bits) { atomicOr(&g_fw_dev_
 constexpr float kLog2 = 1.4426950408889634f;
 constexpr int kRows = 128;  // query rows of a tile, keys of a block
 constexpr uint32_t kTileBytes = kRows * 64 * 2;  // 16 KB
-constexpr int kKvStages = 3;
-constexpr int kFwdSmem = 2 * kTileBytes + 2 * kKvStages * kTileBytes + 1024;
-constexpr int kFwdThreads = 32 * 10;  // 4 + 4 softmax warps (one tile each), MMA, TMA
+constexpr int kKStages = 3, kVStages = 2;  // 97 KB with Q: two CTAs an SM
+constexpr int kFwdSmem = (1 + kKStages + kVStages) * kTileBytes + 1024;
+constexpr int kFwdThreads = 32 * 6;  // 4 softmax warps, products, loads
 
 struct PromptArgs {
   const int64_t *cu_q, *cu_k;  // [seqs + 1]
@@ -43,7 +42,7 @@ struct PromptArgs {
   float *part_o, *part_lse;     // splits > 1: [splits][rows_q][heads][64], [splits][heads][rows_q]
 };
 
-// Where a work item lies: a pair of query tiles of one sequence.
+// Where a work item lies: a tile of one sequence.
 struct Item {
   int64_t q0, k0;  // first rows of the sequence
   int lq, lk;
@@ -93,45 +92,48 @@ __device__ __forceinline__ Item find_item(const int64_t* cu_a, const int64_t* cu
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
+__global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
                                                                      const __grid_constant__ CUtensorMap tmK,
                                                                      const __grid_constant__ CUtensorMap tmV,
                                                                      PromptArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_q, full_k[kKvStages], empty_k[kKvStages], full_v[kKvStages],
-      empty_v[kKvStages], landed_v, s_full[2], s_free[2], p_full[2], o_done[2];
+  __shared__ __align__(8) uint64_t bar_q, full_k[kKStages], empty_k[kKStages], full_v[kVStages],
+      empty_v[kVStages], landed_v, s_full, s_free, p_full, o_done;
   __shared__ uint32_t tmem_base_sh;
   __shared__ Item s_item;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  uint8_t* ks = smem + 2 * kTileBytes;
-  uint8_t* vs = ks + kKvStages * kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ks = smem + kTileBytes;
+  uint8_t* vs = ks + kKStages * kTileBytes;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
 
   // blockIdx.x = (item * kv_heads + key head) * splits + split
   const int split = blockIdx.x % a.splits;
   const int kvh = blockIdx.x / a.splits % a.kv_heads;
-  if (warp == 8) tmem_alloc(&tmem_base_sh, 512);
-  if (warp == 9) {
-    const Item it = find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, 2 * a.tokens,
+  if (warp == 4) {
+    tmem_alloc(&tmem_base_sh, 256);
+    tmem_relinquish();
+  }
+  if (warp == 5) {
+    const Item it = find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens,
                               blockIdx.x / a.splits / a.kv_heads, lane);
     if (lane == 0) {
       s_item = it;
       mbar_init(&bar_q, 1);
       mbar_init(&landed_v, 1);
-      for (int i = 0; i < kKvStages; ++i) {
+      for (int i = 0; i < kKStages; ++i) {
         mbar_init(&full_k[i], 1);
         mbar_init(&empty_k[i], 1);
+      }
+      for (int i = 0; i < kVStages; ++i) {
         mbar_init(&full_v[i], 1);
         mbar_init(&empty_v[i], 1);
       }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1);  // scores of the tile's next block are in tensor memory
-        mbar_init(&s_free[i], 4);  // its softmax warps have read them
-        mbar_init(&p_full[i], 4);  // P is in tensor memory
-        mbar_init(&o_done[i], 1);  // P V has been added to O
-      }
+      mbar_init(&s_full, 1);  // scores of the next block are in tensor memory
+      mbar_init(&s_free, 4);  // the softmax warps have read them
+      mbar_init(&p_full, 4);  // P is in tensor memory
+      mbar_init(&o_done, 1);  // P V has been added to O
       mbar_fence_init();
       tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(&tmK);
@@ -141,51 +143,38 @@ __global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base_sh;
-  Item it = s_item;
+  const uint32_t tmem = tmem_base_sh;  // columns: S 0, P 128, O 192
+  const Item it = s_item;
   if (it.tile >= 0) {
-    // Causal: the items of a sequence from its end, so that the longest start first.
-    const int items = (it.lq + 2 * a.tokens - 1) / (2 * a.tokens);
-    const int tile = a.causal ? items - 1 - it.tile : it.tile;
+    // Causal: the tiles of a sequence from its end, so that the longest start first.
+    const int items = (it.lq + a.tokens - 1) / a.tokens;
+    const int tok = (a.causal ? items - 1 - it.tile : it.tile) * a.tokens;  // the tile's first token
     const int shift = it.lk - it.lq;
-    int tok[2], blocks[2];  // first token of each tile; key blocks that it sees
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      tok[t] = (2 * tile + t) * a.tokens;
-      const int last = min(it.lq, tok[t] + a.tokens) - 1;  // its last token
-      const int seen = tok[t] >= it.lq ? 0 : a.causal ? max(0, min(it.lk, last + shift + 1)) : it.lk;
-      blocks[t] = (seen + kRows - 1) / kRows;
-    }
-    const int all = max(blocks[0], blocks[1]);
+    const int last = min(it.lq, tok + a.tokens) - 1;
+    const int all = ((a.causal ? max(0, last + shift + 1) : it.lk) + kRows - 1) / kRows;  // key blocks that it sees
     const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
     const int cnt = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - j0;
-    const int nt[2] = {max(0, min(cnt, blocks[0] - j0)), max(0, min(cnt, blocks[1] - j0))};
 
-    if (warp == 9) {
+    if (warp == 5) {
       // ---- loads
       if (lane == 0 && cnt > 0) {
-        const uint32_t bytes = static_cast<uint32_t>(a.tokens * a.group) * 128;
-        mbar_arrive_expect_tx(&bar_q, nt[1] > 0 ? 2 * bytes : bytes);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (t == 0 || nt[1] > 0)
-            tma_load_3d(smem + t * kTileBytes, &tmQ, &bar_q, 0, kvh * a.group, static_cast<int>(it.q0 + tok[t]));
+        mbar_arrive_expect_tx(&bar_q, static_cast<uint32_t>(a.tokens * a.group) * 128);
+        tma_load_3d(smem, &tmQ, &bar_q, 0, kvh * a.group, static_cast<int>(it.q0 + tok));
       }
       bool ok = true;
       for (int jj = 0; jj < cnt && ok; ++jj) {
-        const int s = jj % kKvStages;
-        const uint32_t ph = ((jj / kKvStages) & 1u) ^ 1u;
+        const int s = jj % kKStages, sv = jj % kVStages;
         const int key = (j0 + jj) * kRows, row = static_cast<int>(it.k0) + key, valid = it.lk - key;
-        uint8_t* vdst = vs + s * kTileBytes;
+        uint8_t* vdst = vs + sv * kTileBytes;
         if (lane == 0) {
-          if (jj >= kKvStages) ok = mbar_wait(&empty_k[s], ph);
+          if (jj >= kKStages) ok = mbar_wait(&empty_k[s], ((jj / kKStages) & 1u) ^ 1u);
           if (ok) {
             mbar_arrive_expect_tx(&full_k[s], kTileBytes);
             tma_load_3d(ks + s * kTileBytes, &tmK, &full_k[s], 0, kvh, row);
-            if (jj >= kKvStages) ok = mbar_wait(&empty_v[s], ph);
+            if (jj >= kVStages) ok = mbar_wait(&empty_v[sv], ((jj / kVStages) & 1u) ^ 1u);
           }
           if (ok) {
-            uint64_t* bar = valid >= kRows ? &full_v[s] : &landed_v;
+            uint64_t* bar = valid >= kRows ? &full_v[sv] : &landed_v;
             mbar_arrive_expect_tx(bar, kTileBytes);
             tma_load_3d(vdst, &tmV, bar, 0, kvh, row);
           }
@@ -199,78 +188,72 @@ __global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __gri
             reinterpret_cast<uint4*>(vdst)[i] = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full_v[s]);
+          if (lane == 0) mbar_arrive(&full_v[sv]);
         }
         if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
-    } else if (warp == 8) {
-      // ---- products
-      if (lane == 0 && cnt > 0) {
+    } else if (warp == 4) {
+      // ---- products (the whole warp runs the loop, one lane issues)
+      if (cnt > 0) {
         constexpr uint32_t idesc_s = make_idesc(kRows, kRows, Type16<T>::kBf16, false, false);
         constexpr uint32_t idesc_o = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
-        bool ok = mbar_wait(&bar_q, 0);
+        const uint64_t qd = sw128_desc(base);
+        bool ok = mbar_wait_warp(&bar_q, 0);
         for (int jj = -1; jj < cnt && ok; ++jj) {
           if (jj + 1 < cnt) {  // S of the next block
-            const int s = (jj + 1) % kKvStages;
-            ok = mbar_wait(&full_k[s], ((jj + 1) / kKvStages) & 1u);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!ok || jj + 1 >= nt[t]) continue;
-              if (jj >= 0) ok = mbar_wait(&s_free[t], jj & 1u);
-              tc_fence_after();
-              const uint64_t qd = sw128_desc(base + t * kTileBytes);
-              const uint64_t kd = sw128_desc(base + (2 + s) * kTileBytes);
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc_mma_f16(tmem + t * 128, qd + 2 * kk, kd + 2 * kk, idesc_s, kk != 0 ? 1u : 0u);
-              tc_commit(&s_full[t]);
-            }
-            tc_commit(&empty_k[s]);
-          }
-          if (jj < 0 || !ok) continue;
-          const int s = jj % kKvStages;
-          ok = mbar_wait(&full_v[s], (jj / kKvStages) & 1u);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok || jj >= nt[t]) continue;
-            ok = mbar_wait(&p_full[t], jj & 1u);
+            const int s = (jj + 1) % kKStages;
+            ok = mbar_wait_warp(&full_k[s], ((jj + 1) / kKStages) & 1u);
+            if (ok && jj >= 0) ok = mbar_wait_warp(&s_free, jj & 1u);
+            if (!ok) break;
             tc_fence_after();
-            const uint64_t vd = sw128_mn_desc(base + (2 + kKvStages + s) * kTileBytes, kTileBytes);
+            const uint64_t kd = sw128_desc(base + (1 + s) * kTileBytes);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) tc_mma_f16(tmem, qd + 2 * kk, kd + 2 * kk, idesc_s, kk != 0 ? 1u : 0u);
+              tc_commit(&s_full);
+              tc_commit(&empty_k[s]);
+            }
+            __syncwarp();
+          }
+          if (jj < 0) continue;
+          const int s = jj % kVStages;
+          ok = mbar_wait_warp(&full_v[s], (jj / kVStages) & 1u) && mbar_wait_warp(&p_full, jj & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = sw128_mn_desc(base + (1 + kKStages + s) * kTileBytes, kTileBytes);
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
-              tc_mma_ta(tmem + 256 + t * 64, tmem + 384 + t * 64 + 8 * kk, vd + 128 * kk, idesc_o,
-                        jj != 0 || kk != 0 ? 1u : 0u);
-            tc_commit(&o_done[t]);
+              tc_mma_ta(tmem + 192, tmem + 128 + 8 * kk, vd + 128 * kk, idesc_o, jj != 0 || kk != 0 ? 1u : 0u);
+            tc_commit(&o_done);
+            tc_commit(&empty_v[s]);
           }
-          tc_commit(&empty_v[s]);
+          __syncwarp();
         }
-        if (!ok) prompt_flag(FW_DEVERR_TIMEOUT);
+        if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
     } else {
       // ---- softmax: thread = row
-      const int t = warp >> 2;
-      const int r = (warp & 3) * 32 + lane;
-      const int n = nt[t];
-      const int token = tok[t] + r / a.group, head = kvh * a.group + r % a.group;
+      const int r = warp * 32 + lane;
+      const int token = tok + r / a.group, head = kvh * a.group + r % a.group;
       const bool live = r < a.tokens * a.group && token < it.lq;
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int limit = a.causal ? min(it.lk - 1, token + shift) : it.lk - 1;  // the last key that it sees
-      const int safe = a.causal ? min(it.lk - 1, tok[t] + shift) : it.lk - 1;  // that every row of the tile sees
-      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 64, tp = tmem + lanes + 384 + t * 64;
+      const int safe = a.causal ? min(it.lk - 1, tok + shift) : it.lk - 1;     // that every row of the tile sees
+      const uint32_t ts = tmem + (static_cast<uint32_t>(warp * 32) << 16), tp = ts + 128, to = ts + 192;
       const float c = a.scale_log2;
       float top = -INFINITY, sum = 0.f;
       bool ok = true;
-      for (int jj = 0; jj < n; ++jj) {
-        ok = mbar_wait_warp(&s_full[t], jj & 1u);
+      for (int jj = 0; jj < cnt; ++jj) {
+        ok = mbar_wait_warp(&s_full, jj & 1u);
         if (!ok) break;
         if (!warp_live) {  // no row of this warp counts: whatever P holds in its lanes stays in them
           // not before the other warps' arrivals of the block before have been used up
-          ok = jj == 0 || mbar_wait_warp(&o_done[t], (jj - 1) & 1u);
+          ok = jj == 0 || mbar_wait_warp(&o_done, (jj - 1) & 1u);
           if (!ok) break;
           if (lane == 0) {
-            mbar_arrive(&s_free[t]);
-            mbar_arrive(&p_full[t]);
+            mbar_arrive(&s_free);
+            mbar_arrive(&p_full);
           }
           continue;
         }
@@ -281,7 +264,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __gri
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
+        if (lane == 0) mbar_arrive(&s_free);
         const int key = (j0 + jj) * kRows;
         if (key + kRows - 1 > safe) {
 #pragma unroll
@@ -290,62 +273,62 @@ __global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __gri
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[i >> 5][i & 31]));
+        for (int i = 0; i < 128; i += 2)
+          mx[(i >> 1) & 3] = fmaxf(fmaxf(mx[(i >> 1) & 3], __uint_as_float(x[i >> 5][i & 31])),
+                                   __uint_as_float(x[i >> 5][(i + 1) & 31]));
         const float cand = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
         const bool move = cand > top + 8.f || (top == -INFINITY && cand > top);
-        bool waited = jj == 0;
+        if (jj > 0) {  // P of the block before has been read, O is complete
+          ok = mbar_wait_warp(&o_done, (jj - 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+        }
         if (__any_sync(0xffffffffu, move)) {
           const float next = move ? cand : top;
-          const float f = top == -INFINITY ? 0.f : ex2(top - next);
-          sum *= move ? f : 1.f;
+          const float f = !move ? 1.f : top == -INFINITY ? 0.f : ex2(top - next);
+          sum *= f;
           top = next;
           if (jj > 0) {
-            ok = mbar_wait_warp(&o_done[t], (jj - 1) & 1u);
-            if (!ok) break;
-            waited = true;
-            tc_fence_after();
-            uint32_t o[32];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              tc_load32(to + 32 * i, o);
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[16];
+              tc_ld16(to + 16 * i, o);
               tc_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
+              for (int k = 0; k < 16; ++k)
                 if (move) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tc_store32(to + 32 * i, o);
+              tc_store16(to + 16 * i, o);
             }
           }
         }
         const float off = top == -INFINITY ? 0.f : -top;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[2][32];
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const float e0 = ex2(fmaf(__uint_as_float(x[i >> 4][(2 * i) & 31]), c, off));
-          const float e1 = ex2(fmaf(__uint_as_float(x[i >> 4][(2 * i + 1) & 31]), c, off));
-          acc[i & 1] += e0;
-          acc[2 + (i & 1)] += e1;
-          p[i >> 5][i & 31] = Type16<T>::pack(e0, e1);
+        for (int h = 0; h < 4; ++h) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = fma2(make_float2(__uint_as_float(x[h][2 * i]), __uint_as_float(x[h][2 * i + 1])),
+                            make_float2(c, c), make_float2(off, off));
+            e = make_float2(ex2(e.x), ex2(e.y));
+            acc[i & 1] = add2(acc[i & 1], e);
+            p[i] = Type16<T>::pack(e.x, e.y);
+          }
+          tc_store16(tp + 16 * h, p);
         }
-        sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-        if (!waited) {  // P of the previous block has been read
-          ok = mbar_wait_warp(&o_done[t], (jj - 1) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-        }
-        tc_store32(tp, p[0]);
-        tc_store32(tp + 32, p[1]);
+        acc[0] = add2(acc[0], acc[1]);
+        sum += acc[0].x + acc[0].y;
         tc_wait_store();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full);
       }
-      if (ok && n > 0 && warp_live) ok = mbar_wait_warp(&o_done[t], (n - 1) & 1u);
+      if (ok && cnt > 0 && warp_live) ok = mbar_wait_warp(&o_done, (cnt - 1) & 1u);
       if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       if (ok && warp_live) {
         tc_fence_after();
         uint32_t o[2][32];
-        if (n > 0) {
+        if (cnt > 0) {
           tc_load32(to, o[0]);
           tc_load32(to + 32, o[1]);
           tc_wait_ld();
@@ -385,10 +368,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) prompt_attn_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, 512);
-  }
+  if (warp == 4) tmem_dealloc(tmem, 256);
 }
 
 // Joins the key splits of a (row, head), one warp each: o = sum_s exp(lse_s - lse) o_s.
@@ -438,7 +418,7 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 //
 //   delta_i = do_i . o_i      p_ij = exp(s_ij - lse_i)      ds_ij = p_ij (do_i . v_j - delta_i)
 //   dv_j = sum_i p_ij do_i    dk_j = scale sum_i ds_ij q_i  dq_i = scale sum_j ds_ij k_j
-// (dv and dk summed over the heads of the group). prompt_delta_kernel writes {lse log2 e, delta} per row;
+// (dv and dk summed over the heads of the group). prompt_delta_kernel writes what both need of lse and delta per row;
 // prompt_grad_kernel has CTAs of two roles, which share one pipeline, so that nothing is summed by atomics and
 // results do not vary: a key role owns 128 keys of a key head and walks the queries (64 tokens of one head a step), a
 // query role owns 128 (token, head) rows and walks the keys (64 a step). The probabilities are computed in both.
@@ -455,6 +435,7 @@ constexpr uint32_t kStepBytes = kStep * 64 * 2;  // 8 KB
 constexpr int kGradStages = 6;
 constexpr uint32_t kGradStage = 2 * kStepBytes;
 constexpr int kGradSmem = kGradStages * kGradStage + 1024;
+constexpr int kGradThreads = 32 * 18;  // 16 softmax warps, products, loads
 constexpr int kDeltaBlocks = 592;
 
 struct GradArgs {
@@ -463,7 +444,7 @@ struct GradArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, d_token, d_head;
   void *dq, *dk, *dv;
   int64_t dq_token, dq_head, dk_token, dk_head, dv_token, dv_head;
-  float2* stat;       // [heads][stat_rows]: {lse log2 e, delta}; a sequence's rows start at stat_start()
+  float2* stat;       // [heads][stat_rows]: {log2 of P's factor - lse log2 e, -delta}; sequences from stat_start() on
   int64_t stat_rows;
   float* largest;     // [kDeltaBlocks]: largest finite |do| each block met
   int64_t key_items;  // CTAs of the key role
@@ -480,6 +461,7 @@ __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
   const PromptArgs& a = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t units = a.rows_q * a.heads;
+  constexpr float kP = Type16<T>::kBf16 ? 0.f : 8.f;  // log2 of the factor that P carries
   float big = 0.f;
   for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; u0 < units; u0 += static_cast<int64_t>(gridDim.x) * 32) {
     const int64_t u = u0 + (lane >> 3);
@@ -517,7 +499,7 @@ __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if (mine && (lane & 7) == 0)
-      g.stat[head * g.stat_rows + stat_start(q0, seq) + row - q0] = make_float2(a.lse[head * a.rows_q + row] * kLog2, dot);
+      g.stat[head * g.stat_rows + stat_start(q0, seq) + row - q0] = make_float2(kP - a.lse[head * a.rows_q + row] * kLog2, -dot);
   }
   big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
@@ -535,8 +517,68 @@ __device__ __forceinline__ float normalizer(float x) {
   return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
 }
 
+// One softmax warp's share of a CTA's steps: 32 of the 64 columns of every second step, P and dS over X and Y (those of
+// columns 32 h .. + 31 as 16 columns from 32 h on). [lo, hi): the columns of a step that count for this row, kKeys:
+// per-column statistics from the step's stage, else the row's own.
+struct GradRow {
+  int steps, per_head, begin;
+  int lo0, hi0;       // of the step at row 0: lo = lo0 - at, hi = hi0 - at
+  float off, del;     // of this row (query role): stat's two
+  float c, norm;
+};
+template <typename T, bool kKeys>
+__device__ __forceinline__ bool grad_steps(const GradRow& g, uint32_t tx, int set, int h, const float2 (*stat)[kStep],
+                                           uint64_t* x_full, uint64_t* p_full, int lane) {
+  int used = 0;
+  for (int j = set; j < g.steps; j += 2, ++used) {
+    if (!mbar_wait_warp(x_full, used & 1u)) return false;
+    tc_fence_after();
+    const int at = (g.begin + (kKeys ? j % g.per_head : j)) * kStep + 32 * h;
+    const float4* st = reinterpret_cast<const float4*>(&stat[j % kGradStages][32 * h]);
+    uint32_t x[32], y[32], p[16];
+    tc_load32(tx, x);
+    tc_load32(tx + 64, y);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float2 off = make_float2(g.off, g.off), del = make_float2(g.del, g.del);
+      if (kKeys) {
+        const float4 two = st[i >> 1];  // of two columns
+        off = make_float2(two.x, two.z);
+        del = make_float2(two.y, two.w);
+      }
+      const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(g.c, g.c), off);
+      const float2 pr = make_float2(ex2(e.x), ex2(e.y));
+      float2 d = add2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), del);
+      if (!Type16<T>::kBf16) d = mul2(d, make_float2(g.norm, g.norm));
+      d = mul2(d, pr);
+      x[i] = __float_as_uint(pr.x), x[i + 1] = __float_as_uint(pr.y);
+      y[i] = __float_as_uint(d.x), y[i + 1] = __float_as_uint(d.y);
+    }
+    const int lo = g.lo0 - at, hi = g.hi0 - at;
+    if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < lo || i >= hi) x[i] = y[i] = 0u;
+    }
+    if (kKeys) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+      tc_store16(tx, p);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+    tc_store16(tx + 64, p);
+    tc_wait_store();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(p_full);
+  }
+  return true;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kGradThreads, 1)
     prompt_grad_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmD,
                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GradArgs g) {
   extern __shared__ uint8_t smem_raw[];
@@ -544,18 +586,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], p_full[2], a_ready, done;
   __shared__ uint32_t tmem_base_sh;
   __shared__ Item s_item;
-  __shared__ float s_norm, s_row_norm[kRows];
+  __shared__ float s_norm, s_big[2][kRows];
   const PromptArgs& a = g.p;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const bool keys = blockIdx.x < g.key_items;  // the role
   const int64_t index = keys ? blockIdx.x : blockIdx.x - g.key_items;
   const int kvh = static_cast<int>(index % a.kv_heads);
 
-  if (warp == 8) tmem_alloc(&tmem_base_sh, 512);
-  if (warp == 9) {
+  if (warp == 16) tmem_alloc(&tmem_base_sh, 512);
+  if (warp == 17) {
     const Item it = keys ? find_item(a.cu_k, a.cu_q, a.rows_k, a.rows_q, a.seqs, kRows, index / a.kv_heads, lane)
                          : find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, index / a.kv_heads, lane);
     if (lane == 0) {
@@ -567,9 +609,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_init(&landed, 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&x_full[i], 1);  // X and Y of the set's next step are in tensor memory
-        mbar_init(&p_full[i], 4);  // P and dS are
+        mbar_init(&p_full[i], 8);  // P and dS are
       }
-      mbar_init(&a_ready, 8);
+      mbar_init(&a_ready, 16);
       mbar_init(&done, 1);
       mbar_fence_init();
       tma_prefetch_desc(keys ? &tmQ : &tmK);
@@ -577,7 +619,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   }
   pdl_wait();
-  if (warp == 8 && !Type16<T>::kBf16) {
+  if (warp == 16 && !Type16<T>::kBf16) {
     float m = 0.f;
     for (int i = lane; i < kDeltaBlocks; i += 32) m = fmaxf(m, g.largest[i]);
     m = warp_max(m);
@@ -612,7 +654,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       per_head = steps = ((a.causal ? max(0, min(it.lk, last + shift + 1)) : it.lk) + kStep - 1) / kStep;
     }
 
-    if (warp == 9) {
+    if (warp == 17) {
       // ---- loads
       bool ok = true;
       uint32_t cut = 0;  // tiles that end inside a step so far
@@ -649,174 +691,145 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
-    } else if (warp == 8) {
-      // ---- products
-      if (lane == 0 && steps > 0) {
+    } else if (warp == 16) {
+      // ---- products (the whole warp runs the loop, one lane issues)
+      if (steps > 0) {
         constexpr uint32_t idesc1 = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
         constexpr uint32_t idesc2 = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
-        bool ok = mbar_wait(&a_ready, 0);
+        bool ok = mbar_wait_warp(&a_ready, 0);
         tc_fence_after();
         for (int j = -1; j < steps && ok; ++j) {
           if (j + 1 < steps) {
             // X and Y of step j + 1, into the set that step j - 1 used: its second products were issued before
-            const int s = (j + 1) % kGradStages, set = (j + 1) & 1;
-            ok = mbar_wait(&full[s], ((j + 1) / kGradStages) & 1u);
+            const int s = (j + 1) % kGradStages;
+            const uint32_t set = tmem + ((j + 1) & 1) * 128;
+            ok = mbar_wait_warp(&full[s], ((j + 1) / kGradStages) & 1u);
             if (!ok) break;
             tc_fence_after();
             const uint64_t b1 = sw128_desc(base + s * kGradStage), b2 = sw128_desc(base + s * kGradStage + kStepBytes);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma_ta(tmem + set * 128, tmem + 384 + 8 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                tc_mma_ta(set, tmem + 384 + 8 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma_ta(tmem + set * 128 + 64, tmem + 416 + 8 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
-            tc_commit(&x_full[set]);
+              for (int kk = 0; kk < 4; ++kk)
+                tc_mma_ta(set + 64, tmem + 416 + 8 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+              tc_commit(&x_full[(j + 1) & 1]);
+            }
+            __syncwarp();
           }
           if (j < 0) continue;
-          const int s = j % kGradStages, set = j & 1;
-          ok = mbar_wait(&p_full[set], (j >> 1) & 1u);
+          const int s = j % kGradStages;
+          const uint32_t set = tmem + (j & 1) * 128;
+          ok = mbar_wait_warp(&p_full[j & 1], (j >> 1) & 1u);
           if (!ok) break;
           tc_fence_after();
           const uint64_t b1 = sw128_mn_desc(base + s * kGradStage, kStepBytes);
           const uint64_t b2 = sw128_mn_desc(base + s * kGradStage + kStepBytes, kStepBytes);
-          if (keys) {
+          if (elect_one()) {
+            if (keys) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc_mma_ta(tmem + 256, set + 32 * (kk >> 1) + 8 * (kk & 1), b2 + 128 * kk, idesc2,
+                          j != 0 || kk != 0 ? 1u : 0u);
+            }
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              tc_mma_ta(tmem + 256, tmem + set * 128 + 8 * kk, b2 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
+              tc_mma_ta(tmem + 320, set + 64 + 32 * (kk >> 1) + 8 * (kk & 1), b1 + 128 * kk, idesc2,
+                        j != 0 || kk != 0 ? 1u : 0u);
+            tc_commit(&empty[s]);
           }
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_ta(tmem + 320, tmem + set * 128 + 64 + 8 * kk, b1 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
-          tc_commit(&empty[s]);
+          __syncwarp();
         }
-        tc_commit(&done);
-        if (!ok) prompt_flag(FW_DEVERR_TIMEOUT);
+        if (elect_one()) tc_commit(&done);
+        if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
     } else {
-      // ---- softmax: thread = row of the A operands (both warpgroups), steps of its warpgroup's parity
-      const int wg = warp >> 2;
+      // ---- softmax: thread = row of the A operands; warps 4 g .. 4 g + 3 work on set g % 2, column half g / 2
+      const int grp = warp >> 2;
       const int r = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const int token = keys ? 0 : first + r / a.group;
       const int head = keys ? kvh : kvh * a.group + r % a.group;
       const bool live = keys ? first + r < it.lk : r < a.tokens * a.group && token < it.lq;
       const int64_t row = keys ? it.k0 + first + r : it.q0 + token;
-      float lse2 = 0.f, delta = 0.f;
-      // A1 (warpgroup 0) and A2 (warpgroup 1) into tensor memory
+      GradRow gr;
+      gr.off = gr.del = 0.f;
+      // the A operands into tensor memory: each warp group takes half the columns of A1 (0, 1) or A2 (2, 3)
       {
-        const T* src = static_cast<const T*>(keys ? (wg == 0 ? g.k : g.v) : (wg == 0 ? g.q : g.dout));
-        const int64_t ts = keys ? (wg == 0 ? g.k_token : g.v_token) : (wg == 0 ? g.q_token : g.d_token);
-        const int64_t hs = keys ? (wg == 0 ? g.k_head : g.v_head) : (wg == 0 ? g.q_head : g.d_head);
-        uint32_t x[32];
-        float big = 0.f;
+        const bool second = grp >= 2;
+        const T* src = static_cast<const T*>(keys ? (second ? g.v : g.k) : (second ? g.dout : g.q));
+        const int64_t ts = keys ? (second ? g.v_token : g.k_token) : (second ? g.d_token : g.q_token);
+        const int64_t hs = keys ? (second ? g.v_head : g.k_head) : (second ? g.d_head : g.q_head);
+        uint32_t x[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live) v = reinterpret_cast<const uint4*>(src + row * ts + head * hs)[i];
+          if (live) v = reinterpret_cast<const uint4*>(src + row * ts + head * hs)[4 * (grp & 1) + i];
           x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
         }
-        if (!Type16<T>::kBf16 && !keys && wg == 1) {
+        if (!Type16<T>::kBf16 && !keys && second) {
+          float big = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < 16; ++i) {
             const float2 v = Type16<T>::unpack(x[i]);
             if (fabsf(v.x) < INFINITY) big = fmaxf(big, fabsf(v.x));
             if (fabsf(v.y) < INFINITY) big = fmaxf(big, fabsf(v.y));
           }
-          s_row_norm[r] = normalizer(big);
+          s_big[grp & 1][r] = big;
         }
-        tc_store32(tmem + lanes + 384 + 32 * wg, x);
+        tc_store16(tmem + lanes + 384 + 16 * grp, x);
         tc_wait_store();
         if (!keys && live) {
           const float2 st = g.stat[head * g.stat_rows + stat_start(it.q0, it.seq) + token];
-          lse2 = st.x;
-          delta = st.y;
+          gr.off = st.x;
+          gr.del = st.y;
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&a_ready);
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // s_row_norm
-      constexpr float kP = Type16<T>::kBf16 ? 0.f : 8.f;  // log2 of the factor that P carries
-      const float norm = Type16<T>::kBf16 ? 1.f : 0.0625f * (keys ? s_norm : s_row_norm[r]);  // of dS besides P's
-      const int limit = keys ? 0 : a.causal ? min(it.lk - 1, token + shift) : it.lk - 1;
-      const float c = a.scale_log2;
-      const uint32_t tx = tmem + lanes + wg * 128;
-      bool ok = true;
-      int used = 0;
-      for (int j = wg; j < steps; j += 2, ++used) {
-        ok = mbar_wait_warp(&x_full[wg], used & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        const int at = (begin + (keys ? j % per_head : j)) * kStep;
-        const float2* st = s_stat[j % kGradStages];
-        // columns [lo, hi) of the step count for this row
-        int lo = 0, hi = kStep;
-        if (keys) {
-          hi = it.lq - at;
-          if (a.causal) lo = first + r - shift - at;
-        } else {
-          hi = limit + 1 - at;
-        }
-        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < kStep);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t x[32], y[32], p[16], d[16];
-          tc_load32(tx + 32 * h, x);
-          tc_load32(tx + 64 + 32 * h, y);
-          tc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float4 two = make_float4(lse2, delta, lse2, delta);
-            if (keys) two = *reinterpret_cast<const float4*>(&st[32 * h + i]);
-            float p0 = ex2(fmaf(__uint_as_float(x[i]), c, kP - two.x));
-            float p1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, kP - two.z));
-            float d0 = p0 * ((__uint_as_float(y[i]) - two.y) * norm);
-            float d1 = p1 * ((__uint_as_float(y[i + 1]) - two.w) * norm);
-            if (cut) {
-              const int k = 32 * h + i;
-              const bool in0 = k >= lo && k < hi, in1 = k + 1 >= lo && k + 1 < hi;
-              p0 = in0 ? p0 : 0.f, d0 = in0 ? d0 : 0.f;
-              p1 = in1 ? p1 : 0.f, d1 = in1 ? d1 : 0.f;
-            }
-            p[i >> 1] = Type16<T>::pack(p0, p1);
-            d[i >> 1] = Type16<T>::pack(d0, d1);
-          }
-          // over X and Y: columns 16 h .. + 15 hold what has been read (h = 0) or is in registers by now
-          if (keys) tc_store16(tx + 16 * h, p);
-          tc_store16(tx + 64 + 16 * h, d);
-        }
-        tc_wait_store();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[wg]);
+      asm volatile("bar.sync 1, 512;" ::: "memory");  // s_big
+      gr.steps = steps, gr.per_head = per_head, gr.begin = begin;
+      gr.c = a.scale_log2;
+      // the factor of dS besides P's
+      gr.norm = Type16<T>::kBf16 ? 1.f : 0.0625f * (keys ? s_norm : normalizer(fmaxf(s_big[0][r], s_big[1][r])));
+      const int set = grp & 1, h = grp >> 1;
+      const uint32_t tx = tmem + lanes + set * 128 + 32 * h;
+      bool ok;
+      if (keys) {
+        gr.hi0 = it.lq;
+        gr.lo0 = a.causal ? first + r - shift : 0;
+        ok = grad_steps<T, true>(gr, tx, set, h, s_stat, &x_full[set], &p_full[set], lane);
+      } else {
+        gr.lo0 = 0;
+        gr.hi0 = (a.causal ? min(it.lk - 1, token + shift) : it.lk - 1) + 1;
+        ok = grad_steps<T, false>(gr, tx, set, h, s_stat, &x_full[set], &p_full[set], lane);
       }
       if (ok && steps > 0) ok = mbar_wait_warp(&done, 0);
       if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
-      // ---- results: key role: warpgroup 0 dK, 1 dV; query role: warpgroup 0 dQ
-      if (ok && (keys || wg == 0)) {
+      // ---- results: 32 columns each of dK (groups 0, 1) and dV (2, 3), or of dQ (0, 1)
+      if (ok && (keys || grp < 2)) {
         tc_fence_after();
-        const bool dv = keys && wg == 1;
-        uint32_t x[2][32];
+        const bool dv = grp >= 2;
+        uint32_t x[32];
         if (steps > 0) {
-          tc_load32(tmem + lanes + (dv ? 256 : 320), x[0]);
-          tc_load32(tmem + lanes + (dv ? 288 : 352), x[1]);
+          tc_load32(tmem + lanes + (dv ? 256 : 320) + 32 * (grp & 1), x);
           tc_wait_ld();
         }
         if (live) {
           constexpr float kUnP = Type16<T>::kBf16 ? 1.f : 1.f / 256.f;
-          const float f = dv ? kUnP : g.scale * kUnP / norm;
+          const float f = dv ? kUnP : g.scale * kUnP / gr.norm;
           T* dst = static_cast<T*>(keys ? (dv ? g.dv : g.dk) : g.dq) +
                    row * (keys ? (dv ? g.dv_token : g.dk_token) : g.dq_token) +
-                   head * (keys ? (dv ? g.dv_head : g.dk_head) : g.dq_head);
+                   head * (keys ? (dv ? g.dv_head : g.dk_head) : g.dq_head) + 32 * (grp & 1);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int e = 8 * i + 2 * k;
-              w[k] = steps > 0 ? Type16<T>::pack(__uint_as_float(x[e >> 5][e & 31]) * f,
-                                                 __uint_as_float(x[e >> 5][(e & 31) + 1]) * f)
-                               : 0u;
+              w[k] = steps > 0 ? Type16<T>::pack(__uint_as_float(x[e]) * f, __uint_as_float(x[e + 1]) * f) : 0u;
             }
             reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -827,7 +840,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_relinquish();
     tmem_dealloc(tmem, 512);
   }
@@ -838,7 +851,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // Splits of the keys: none when the query tiles fill the SMs; else as many as make two CTAs an SM, up to one per key
 // block of an average sequence. From sizes only (the offsets are on the device).
 static int prompt_splits(int64_t rows_q, int64_t rows_k, int seqs, int kv_heads, int group) {
-  const int64_t items = (rows_q / (2 * (kRows / group)) + seqs) * kv_heads;  // at most
+  const int64_t items = (rows_q / (kRows / group) + seqs) * kv_heads;  // at most
   const int64_t blocks = seqs > 0 ? (rows_k / seqs + kRows - 1) / kRows : 1;
   int64_t s = items > 0 ? 2 * 148 / items : 1;
   if (s > blocks) s = blocks;
@@ -864,7 +877,7 @@ static int make_rows_map(CUtensorMap* m, CUtensorMapDataType type, const void* p
 template <typename T>
 static int run_prompt(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v, PromptArgs a, cudaStream_t s) {
   CUtensorMap tq, tk, tv;
-  const int64_t items = (a.rows_q / (2 * a.tokens) + a.seqs) * a.kv_heads * a.splits;
+  const int64_t items = (a.rows_q / a.tokens + a.seqs) * a.kv_heads * a.splits;
   FW_REQUIRE(items < (int64_t(1) << 31), FW_ERR_SHAPE, "prompt_attention: too many query tiles");
   // no keys at all: any valid address serves, nothing is read through it
   const bool keys = a.rows_k > 0;
@@ -912,7 +925,7 @@ static int run_prompt_grad(const fw_rows_t& q, const fw_rows_t& k, const fw_rows
   auto kern = prompt_grad_kernel<T>;
   cudaError_t e = ensure_smem(kern, kGradSmem);
   if (e == cudaSuccess)
-    e = launch(kern, dim3(static_cast<unsigned>(g.key_items + query_items)), dim3(kFwdThreads), kGradSmem, s,
+    e = launch(kern, dim3(static_cast<unsigned>(g.key_items + query_items)), dim3(kGradThreads), kGradSmem, s,
                a.rows_q > 0, tq, td, tk, tv, g);
   return launch_status(e, "prompt_attention_grad");
 }
