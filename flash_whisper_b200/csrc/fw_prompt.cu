@@ -424,18 +424,21 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 // query role owns 128 (token, head) rows and walks the keys (64 a step). The probabilities are computed in both.
 //   first products:   X = A1 B1^T, Y = A2 B2^T       key role: A = K, V   B = Q, dO;    query role: A = Q, dO  B = K, V
 //   second products:  key role: dV += P^T dO, dK += dS^T Q;      query role: dQ += dS K
-// The A operands stay in tensor memory for the CTA's whole life, and P and dS are written over X and Y as the A
-// operands of the second products; from shared memory comes only a step's B tile pair, which serves both products
-// (K-major in the first, MN-major in the second). Two sets of X and Y: one softmax warpgroup works on each, the even
-// and the odd steps, while the tensor core works on the other.
+// Each step's B tile pair serves both products (K-major in the first, MN-major in the second). X and Y, and P and dS as
+// the A operands of the second products, are in tensor memory, two sets of each: eight softmax warps work on the even
+// and eight on the odd steps, half a step apart, so that the exponentials of one group run while the other waits, loads
+// and stores. As soon as a step's X and Y are in registers the first products of the step after the next are issued
+// into them, by a warp of its own (a third one issues the second products: one warp for both was busy for longer than
+// the exponentials take). A1 and A2 stay for the CTA's whole life, in shared memory in the key role (tensor memory is
+// full) and in tensor memory in the query role.
 // fp16 range: P is kept times 2^8, and dS times 2^4 over the power of two of the largest |do| (of the row in the query
 // role, of the call in the key role), so that gradients of any size keep their bits; bf16 needs neither.
 constexpr int kStep = 64;                        // B rows of a step
 constexpr uint32_t kStepBytes = kStep * 64 * 2;  // 8 KB
-constexpr int kGradStages = 6;
+constexpr int kGradStages = 8;
 constexpr uint32_t kGradStage = 2 * kStepBytes;
-constexpr int kGradSmem = kGradStages * kGradStage + 1024;
-constexpr int kGradThreads = 32 * 18;  // 16 softmax warps, products, loads
+constexpr int kGradSmem = 2 * kTileBytes + kGradStages * kGradStage + 1024;
+constexpr int kGradThreads = 32 * 19;  // 16 softmax warps, loads, first products, second products
 constexpr int kDeltaBlocks = 592;
 
 struct GradArgs {
@@ -444,7 +447,9 @@ struct GradArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, d_token, d_head;
   void *dq, *dk, *dv;
   int64_t dq_token, dq_head, dk_token, dk_head, dv_token, dv_head;
-  float2* stat;       // [heads][stat_rows]: {log2 of P's factor - lse log2 e, -delta}; sequences from stat_start() on
+  // [heads][stat_rows]: log2 of P's factor - lse log2 e, and -delta, four rows of the first and then of the second at a
+  // time; a sequence's rows start at stat_start()
+  float* stat;
   int64_t stat_rows;
   float* largest;     // [kDeltaBlocks]: largest finite |do| each block met
   int64_t key_items;  // CTAs of the key role
@@ -453,6 +458,10 @@ struct GradArgs {
 
 // First row of sequence `seq` in stat: a multiple of 4 (16 bytes at least), behind the previous sequence's rows.
 __device__ __forceinline__ int64_t stat_start(int64_t q0, int seq) { return ((q0 + 3) / 4 + seq) * 4; }
+
+__device__ __forceinline__ float* stat_at(const GradArgs& g, int head, int64_t row) {
+  return g.stat + (head * g.stat_rows + row / 4 * 4) * 2 + row % 4;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
@@ -498,8 +507,11 @@ __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
     }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (mine && (lane & 7) == 0)
-      g.stat[head * g.stat_rows + stat_start(q0, seq) + row - q0] = make_float2(kP - a.lse[head * a.rows_q + row] * kLog2, -dot);
+    if (mine && (lane & 7) == 0) {
+      float* st = stat_at(g, head, stat_start(q0, seq) + row - q0);
+      st[0] = kP - a.lse[head * a.rows_q + row] * kLog2;
+      st[4] = -dot;
+    }
   }
   big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
@@ -517,62 +529,78 @@ __device__ __forceinline__ float normalizer(float x) {
   return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
 }
 
-// One softmax warp's share of a CTA's steps: 32 of the 64 columns of every second step, P and dS over X and Y (those of
-// columns 32 h .. + 31 as 16 columns from 32 h on). [lo, hi): the columns of a step that count for this row, kKeys:
-// per-column statistics from the step's stage, else the row's own.
+// One softmax warp's share of a CTA's steps: 32 of the 64 columns of every second step. kKeys: the statistics are per
+// column, from the step's stage, else the row's own.
 struct GradRow {
   int steps, per_head, begin;
-  int lo0, hi0;       // of the step at row 0: lo = lo0 - at, hi = hi0 - at
+  int lo0, hi0;       // columns [lo0, hi0) of the whole walk count for this row
   float off, del;     // of this row (query role): stat's two
   float c, norm;
+  uint32_t tx, tp;    // tensor memory: X (Y 64 columns on), P (dS 32 columns on) of this warp's set, half and lanes
+  uint64_t *x_full, *x_free, *p_full, *p_free, *full;
 };
 template <typename T, bool kKeys>
-__device__ __forceinline__ bool grad_steps(const GradRow& g, uint32_t tx, int set, int h, const float2 (*stat)[kStep],
-                                           uint64_t* x_full, uint64_t* p_full, int lane) {
+__device__ __forceinline__ bool grad_steps(const GradRow& g, int set, int h, const float (*stat)[2 * kStep], int lane) {
   int used = 0;
   for (int j = set; j < g.steps; j += 2, ++used) {
-    if (!mbar_wait_warp(x_full, used & 1u)) return false;
+    const int s = j % kGradStages;
+    if (kKeys && !mbar_wait_warp(g.full + s, (j / kGradStages) & 1u)) return false;  // the statistics
+    if (!mbar_wait_warp(g.x_full, used & 1u)) return false;
     tc_fence_after();
-    const int at = (g.begin + (kKeys ? j % g.per_head : j)) * kStep + 32 * h;
-    const float4* st = reinterpret_cast<const float4*>(&stat[j % kGradStages][32 * h]);
-    uint32_t x[32], y[32], p[16];
-    tc_load32(tx, x);
-    tc_load32(tx + 64, y);
+    uint32_t x[32], y[32];
+    tc_load32(g.tx, x);
+    tc_load32(g.tx + 64, y);
     tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float2 off = make_float2(g.off, g.off), del = make_float2(g.del, g.del);
-      if (kKeys) {
-        const float4 two = st[i >> 1];  // of two columns
-        off = make_float2(two.x, two.z);
-        del = make_float2(two.y, two.w);
-      }
-      const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(g.c, g.c), off);
-      const float2 pr = make_float2(ex2(e.x), ex2(e.y));
-      float2 d = add2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), del);
-      if (!Type16<T>::kBf16) d = mul2(d, make_float2(g.norm, g.norm));
-      d = mul2(d, pr);
-      x[i] = __float_as_uint(pr.x), x[i + 1] = __float_as_uint(pr.y);
-      y[i] = __float_as_uint(d.x), y[i + 1] = __float_as_uint(d.y);
-    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(g.x_free);
+    const int at = (g.begin + (kKeys ? j % g.per_head : j)) * kStep + 32 * h;
     const int lo = g.lo0 - at, hi = g.hi0 - at;
-    if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
+    const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 32);
+    const float4* st = reinterpret_cast<const float4*>(&stat[s][64 * h]);
+    const float2 c2 = make_float2(g.c, g.c), n2 = make_float2(g.norm, g.norm);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {  // four columns at a time
+      float4 off = make_float4(g.off, g.off, g.off, g.off), del = make_float4(g.del, g.del, g.del, g.del);
+      if (kKeys) {
+        off = st[2 * q];
+        del = st[2 * q + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = 4 * q + 2 * i;
+        const float2 e = fma2(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), c2,
+                              i == 0 ? make_float2(off.x, off.y) : make_float2(off.z, off.w));
+        const float2 p = make_float2(ex2(e.x), ex2(e.y));
+        float2 d = add2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])),
+                        i == 0 ? make_float2(del.x, del.y) : make_float2(del.z, del.w));
+        if (!Type16<T>::kBf16) d = mul2(d, n2);
+        d = mul2(d, p);
+        x[k] = __float_as_uint(p.x), x[k + 1] = __float_as_uint(p.y);
+        y[k] = __float_as_uint(d.x), y[k + 1] = __float_as_uint(d.y);
+      }
+    }
+    if (cut) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (i < lo || i >= hi) x[i] = y[i] = 0u;
     }
-    if (kKeys) {
+    uint32_t p[16], d[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
-      tc_store16(tx, p);
+    for (int i = 0; i < 16; ++i) {
+      if (kKeys) p[i] = Type16<T>::pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+      d[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
-    tc_store16(tx + 64, p);
+    if (used > 0) {  // the second products of two steps before have read P and dS
+      if (!mbar_wait_warp(g.p_free, (used - 1) & 1u)) return false;
+      tc_fence_after();
+    }
+    if (kKeys) tc_store16(g.tp, p);
+    tc_store16(g.tp + 32, d);
     tc_wait_store();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(p_full);
+    if (lane == 0) mbar_arrive(g.p_full);
   }
   return true;
 }
@@ -582,15 +610,16 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     prompt_grad_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmD,
                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GradArgs g) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(16) float2 s_stat[kGradStages][kStep];
-  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], p_full[2], a_ready, done;
+  __shared__ __align__(16) float s_stat[kGradStages][2 * kStep];
+  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], x_free[2], p_full[2],
+      p_free[2], a_ready, done;
   __shared__ uint32_t tmem_base_sh;
   __shared__ Item s_item;
   __shared__ float s_norm, s_big[2][kRows];
   const PromptArgs& a = g.p;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
+  uint8_t* stages = smem_raw + (base - raw) + 2 * kTileBytes;  // behind A1 and A2 of the key role
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const bool keys = blockIdx.x < g.key_items;  // the role
   const int64_t index = keys ? blockIdx.x : blockIdx.x - g.key_items;
@@ -609,9 +638,11 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       mbar_init(&landed, 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&x_full[i], 1);  // X and Y of the set's next step are in tensor memory
-        mbar_init(&p_full[i], 8);  // P and dS are
+        mbar_init(&x_free[i], 8);  // its warps have read them
+        mbar_init(&p_full[i], 8);  // P and dS are in tensor memory
+        mbar_init(&p_free[i], 1);  // the second products have read them
       }
-      mbar_init(&a_ready, 16);
+      mbar_init(&a_ready, keys ? 1 : 16);
       mbar_init(&done, 1);
       mbar_fence_init();
       tma_prefetch_desc(keys ? &tmQ : &tmK);
@@ -656,6 +687,13 @@ __global__ void __launch_bounds__(kGradThreads, 1)
 
     if (warp == 17) {
       // ---- loads
+      if (keys && lane == 0 && steps > 0) {  // A1 = K, A2 = V; rows behind the sequence are rows of no result
+        mbar_arrive_expect_tx(&a_ready, 2 * kTileBytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          tma_load_3d(stages - 2 * kTileBytes + i * kStepBytes, i < 2 ? &tmK : &tmV, &a_ready, 0, kvh,
+                      static_cast<int>(it.k0) + first + (i & 1) * kStep);
+      }
       bool ok = true;
       uint32_t cut = 0;  // tiles that end inside a step so far
       for (int j = 0; j < steps && ok; ++j) {
@@ -664,7 +702,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const int at = (begin + (keys ? j % per_head : j)) * kStep;
         const int valid = (keys ? it.lq : it.lk) - at;
         const int row = static_cast<int>(keys ? it.q0 : it.k0) + at;
-        uint8_t* dst = smem + s * kGradStage;
+        uint8_t* dst = stages + s * kGradStage;
         if (lane == 0) {
           if (j >= kGradStages) ok = mbar_wait(&empty[s], ((j / kGradStages) & 1u) ^ 1u);
           if (ok) {
@@ -673,7 +711,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
             tma_load_3d(dst, keys ? &tmQ : &tmK, bar, 0, head, row);
             tma_load_3d(dst + kStepBytes, keys ? &tmD : &tmV, bar, 0, head, row);
             if (keys)
-              bulk_g2s(s_stat[s], g.stat + head * g.stat_rows + stat_start(it.q0, it.seq) + at, kStep * 8, bar);
+              bulk_g2s(s_stat[s], stat_at(g, head, stat_start(it.q0, it.seq) + at), kStep * 8, bar);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -692,52 +730,61 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
     } else if (warp == 16) {
-      // ---- products (the whole warp runs the loop, one lane issues)
+      // ---- first products (the whole warp runs the loop, one lane issues)
       if (steps > 0) {
-        constexpr uint32_t idesc1 = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
-        constexpr uint32_t idesc2 = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
+        constexpr uint32_t idesc = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+        const uint64_t a1 = sw128_desc(base), a2 = a1 + (kTileBytes >> 4);
         bool ok = mbar_wait_warp(&a_ready, 0);
-        tc_fence_after();
-        for (int j = -1; j < steps && ok; ++j) {
-          if (j + 1 < steps) {
-            // X and Y of step j + 1, into the set that step j - 1 used: its second products were issued before
-            const int s = (j + 1) % kGradStages;
-            const uint32_t set = tmem + ((j + 1) & 1) * 128;
-            ok = mbar_wait_warp(&full[s], ((j + 1) / kGradStages) & 1u);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t b1 = sw128_desc(base + s * kGradStage), b2 = sw128_desc(base + s * kGradStage + kStepBytes);
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc_mma_ta(set, tmem + 384 + 8 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc_mma_ta(set + 64, tmem + 416 + 8 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
-              tc_commit(&x_full[(j + 1) & 1]);
-            }
-            __syncwarp();
-          }
-          if (j < 0) continue;
+        for (int j = 0; j < steps && ok; ++j) {
           const int s = j % kGradStages;
-          const uint32_t set = tmem + (j & 1) * 128;
-          ok = mbar_wait_warp(&p_full[j & 1], (j >> 1) & 1u);
+          const uint32_t x = tmem + (j & 1) * 128;
+          ok = mbar_wait_warp(&full[s], (j / kGradStages) & 1u);
+          if (ok && j >= 2) ok = mbar_wait_warp(&x_free[j & 1], ((j >> 1) & 1u) ^ 1u);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t b1 = sw128_mn_desc(base + s * kGradStage, kStepBytes);
-          const uint64_t b2 = sw128_mn_desc(base + s * kGradStage + kStepBytes, kStepBytes);
+          const uint64_t b1 = sw128_desc(base + 2 * kTileBytes + s * kGradStage), b2 = b1 + (kStepBytes >> 4);
           if (elect_one()) {
             if (keys) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                tc_mma_ta(tmem + 256, set + 32 * (kk >> 1) + 8 * (kk & 1), b2 + 128 * kk, idesc2,
-                          j != 0 || kk != 0 ? 1u : 0u);
-            }
+              for (int kk = 0; kk < 4; ++kk) {
+                tc_mma_f16(x, a1 + 2 * kk, b1 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                tc_mma_f16(x + 64, a2 + 2 * kk, b2 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+              }
+            } else {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma_ta(tmem + 320, set + 64 + 32 * (kk >> 1) + 8 * (kk & 1), b1 + 128 * kk, idesc2,
-                        j != 0 || kk != 0 ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk) {
+                tc_mma_ta(x, tmem + 256 + 8 * kk, b1 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                tc_mma_ta(x + 64, tmem + 320 + 8 * kk, b2 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+              }
+            }
+            tc_commit(&x_full[j & 1]);
+          }
+          __syncwarp();
+        }
+        if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
+      }
+    } else if (warp == 18) {
+      // ---- second products
+      if (steps > 0) {
+        constexpr uint32_t idesc = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
+        bool ok = true;
+        for (int j = 0; j < steps && ok; ++j) {
+          const int s = j % kGradStages;
+          const uint32_t p = tmem + 256 + (j & 1) * 64;
+          // the B tiles have landed for the first products; this warp's own view of them
+          ok = mbar_wait_warp(&full[s], (j / kGradStages) & 1u) && mbar_wait_warp(&p_full[j & 1], (j >> 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b1 = sw128_mn_desc(base + 2 * kTileBytes + s * kGradStage, kStepBytes),
+                         b2 = b1 + (kStepBytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              if (keys) tc_mma_ta(tmem + 384, p + 8 * kk, b2 + 128 * kk, idesc, j != 0 || kk != 0 ? 1u : 0u);
+              tc_mma_ta(tmem + 448, p + 32 + 8 * kk, b1 + 128 * kk, idesc, j != 0 || kk != 0 ? 1u : 0u);
+            }
             tc_commit(&empty[s]);
+            tc_commit(&p_free[j & 1]);
           }
           __syncwarp();
         }
@@ -755,20 +802,19 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       const int64_t row = keys ? it.k0 + first + r : it.q0 + token;
       GradRow gr;
       gr.off = gr.del = 0.f;
-      // the A operands into tensor memory: each warp group takes half the columns of A1 (0, 1) or A2 (2, 3)
-      {
+      if (!keys) {
+        // the A operands into tensor memory: each warp group takes half the columns of A1 = Q (0, 1) or A2 = dO (2, 3)
         const bool second = grp >= 2;
-        const T* src = static_cast<const T*>(keys ? (second ? g.v : g.k) : (second ? g.dout : g.q));
-        const int64_t ts = keys ? (second ? g.v_token : g.k_token) : (second ? g.d_token : g.q_token);
-        const int64_t hs = keys ? (second ? g.v_head : g.k_head) : (second ? g.d_head : g.q_head);
+        const T* src = static_cast<const T*>(second ? g.dout : g.q) + row * (second ? g.d_token : g.q_token) +
+                       head * (second ? g.d_head : g.q_head);
         uint32_t x[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live) v = reinterpret_cast<const uint4*>(src + row * ts + head * hs)[4 * (grp & 1) + i];
+          if (live) v = reinterpret_cast<const uint4*>(src)[4 * (grp & 1) + i];
           x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
         }
-        if (!Type16<T>::kBf16 && !keys && second) {
+        if (!Type16<T>::kBf16 && second) {
           float big = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -778,12 +824,12 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           }
           s_big[grp & 1][r] = big;
         }
-        tc_store16(tmem + lanes + 384 + 16 * grp, x);
+        tc_store16(tmem + lanes + (second ? 320 : 256) + 16 * (grp & 1), x);
         tc_wait_store();
-        if (!keys && live) {
-          const float2 st = g.stat[head * g.stat_rows + stat_start(it.q0, it.seq) + token];
-          gr.off = st.x;
-          gr.del = st.y;
+        if (live) {
+          const float* st = stat_at(g, head, stat_start(it.q0, it.seq) + token);
+          gr.off = st[0];
+          gr.del = st[4];
         }
         tc_fence_before();
         __syncwarp();
@@ -795,16 +841,19 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       // the factor of dS besides P's
       gr.norm = Type16<T>::kBf16 ? 1.f : 0.0625f * (keys ? s_norm : normalizer(fmaxf(s_big[0][r], s_big[1][r])));
       const int set = grp & 1, h = grp >> 1;
-      const uint32_t tx = tmem + lanes + set * 128 + 32 * h;
+      gr.tx = tmem + lanes + set * 128 + 32 * h;
+      gr.tp = tmem + lanes + 256 + set * 64 + 16 * h;
+      gr.x_full = &x_full[set], gr.x_free = &x_free[set], gr.p_full = &p_full[set], gr.p_free = &p_free[set];
+      gr.full = full;
       bool ok;
       if (keys) {
         gr.hi0 = it.lq;
         gr.lo0 = a.causal ? first + r - shift : 0;
-        ok = grad_steps<T, true>(gr, tx, set, h, s_stat, &x_full[set], &p_full[set], lane);
+        ok = grad_steps<T, true>(gr, set, h, s_stat, lane);
       } else {
         gr.lo0 = 0;
         gr.hi0 = (a.causal ? min(it.lk - 1, token + shift) : it.lk - 1) + 1;
-        ok = grad_steps<T, false>(gr, tx, set, h, s_stat, &x_full[set], &p_full[set], lane);
+        ok = grad_steps<T, false>(gr, set, h, s_stat, lane);
       }
       if (ok && steps > 0) ok = mbar_wait_warp(&done, 0);
       if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
@@ -814,7 +863,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         const bool dv = grp >= 2;
         uint32_t x[32];
         if (steps > 0) {
-          tc_load32(tmem + lanes + (dv ? 256 : 320) + 32 * (grp & 1), x);
+          tc_load32(tmem + lanes + (dv ? 384 : 448) + 32 * (grp & 1), x);
           tc_wait_ld();
         }
         if (live) {
@@ -1079,7 +1128,7 @@ int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_ro
   g.dk = dk->ptr, g.dk_token = dk->token, g.dk_head = dk->head;
   g.dv = dv->ptr, g.dv_token = dv->token, g.dv_head = dv->head;
   g.largest = static_cast<float*>(workspace);
-  g.stat = reinterpret_cast<float2*>(g.largest + kDeltaBlocks);
+  g.stat = g.largest + kDeltaBlocks;
   g.stat_rows = grad_stat_rows(rows_q, seqs);
   g.scale = scale;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
