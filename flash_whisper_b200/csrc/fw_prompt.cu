@@ -420,25 +420,22 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 //   dv_j = sum_i p_ij do_i    dk_j = scale sum_i ds_ij q_i  dq_i = scale sum_j ds_ij k_j
 // (dv and dk summed over the heads of the group). prompt_delta_kernel writes what both need of lse and delta per row;
 // prompt_grad_kernel has CTAs of two roles, which share one pipeline, so that nothing is summed by atomics and
-// results do not vary: a key role owns 128 keys of a key head and walks the queries (64 tokens of one head a step), a
-// query role owns 128 (token, head) rows and walks the keys (64 a step). The probabilities are computed in both.
+// results do not vary: a key role owns 128 keys of a key head and walks the queries (128 tokens of one head a step), a
+// query role owns 128 (token, head) rows and walks the keys (128 a step). The probabilities are computed in both.
 //   first products:   X = A1 B1^T, Y = A2 B2^T       key role: A = K, V   B = Q, dO;    query role: A = Q, dO  B = K, V
 //   second products:  key role: dV += P^T dO, dK += dS^T Q;      query role: dQ += dS K
-// Each step's B tile pair serves both products (K-major in the first, MN-major in the second). X and Y, and P and dS as
-// the A operands of the second products, are in tensor memory, two sets of each: eight softmax warps work on the even
-// and eight on the odd steps, half a step apart, so that the exponentials of one group run while the other waits, loads
-// and stores. As soon as a step's X and Y are in registers the first products of the step after the next are issued
-// into them, by a warp of its own (a third one issues the second products: one warp for both was busy for longer than
-// the exponentials take). A1 and A2 stay for the CTA's whole life, in shared memory in the key role (tensor memory is
-// full) and in tensor memory in the query role.
+// Each step's B tile pair serves both products (K-major in the first, MN-major in the second). X, twice, and Y are in
+// tensor memory; P and dS, the A operands of the second products, are written over X. 16 softmax warps (32 rows x 32
+// columns each) compute a step's exponentials from X while the tensor core is still at the step before's second
+// products and this step's Y, and need Y only then: a step's hand-overs hide behind the exponentials. A1 and A2 stay for
+// the CTA's whole life, in shared memory in the key role (tensor memory is full) and in tensor memory in the query role.
 // fp16 range: P is kept times 2^8, and dS times 2^4 over the power of two of the largest |do| (of the row in the query
 // role, of the call in the key role), so that gradients of any size keep their bits; bf16 needs neither.
-constexpr int kStep = 64;                        // B rows of a step
-constexpr uint32_t kStepBytes = kStep * 64 * 2;  // 8 KB
-constexpr int kGradStages = 8;
-constexpr uint32_t kGradStage = 2 * kStepBytes;
+constexpr int kStep = 128;  // B rows of a step
+constexpr int kGradStages = 4;
+constexpr uint32_t kGradStage = 2 * kTileBytes;
 constexpr int kGradSmem = 2 * kTileBytes + kGradStages * kGradStage + 1024;
-constexpr int kGradThreads = 32 * 19;  // 16 softmax warps, loads, first products, second products
+constexpr int kGradThreads = 32 * 18;  // 16 softmax warps, products, loads
 constexpr int kDeltaBlocks = 592;
 
 struct GradArgs {
@@ -529,74 +526,84 @@ __device__ __forceinline__ float normalizer(float x) {
   return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
 }
 
-// One softmax warp's share of a CTA's steps: 32 of the 64 columns of every second step. kKeys: the statistics are per
-// column, from the step's stage, else the row's own.
+// One softmax warp's share of a CTA's steps: 32 of the 128 columns. kKeys: the statistics are per column, from the
+// step's stage, else the row's own.
 struct GradRow {
   int steps, per_head, begin;
-  int lo0, hi0;       // columns [lo0, hi0) of the whole walk count for this row
-  float off, del;     // of this row (query role): stat's two
+  int lo0, hi0;     // columns [lo0, hi0) of the whole walk count for this row
+  float off, del;   // of this row (query role): stat's two
   float c, norm;
-  uint32_t tx, tp;    // tensor memory: X (Y 64 columns on), P (dS 32 columns on) of this warp's set, half and lanes
-  uint64_t *x_full, *x_free, *p_full, *p_free, *full;
+  uint32_t tx, ty;  // tensor memory: X (the second one 128 columns on) and Y, this warp's columns and lanes
+  uint64_t *x_full, *y_full, *p_full, *full;
 };
 template <typename T, bool kKeys>
-__device__ __forceinline__ bool grad_steps(const GradRow& g, int set, int h, const float (*stat)[2 * kStep], int lane) {
-  int used = 0;
-  for (int j = set; j < g.steps; j += 2, ++used) {
+__device__ __forceinline__ bool grad_steps(const GradRow& g, int h, const float (*stat)[2 * kStep], int lane) {
+  const float2 c2 = make_float2(g.c, g.c), n2 = make_float2(g.norm, g.norm);
+  int block = 0;  // j % per_head in the key role
+  for (int j = 0; j < g.steps; ++j) {
     const int s = j % kGradStages;
-    if (kKeys && !mbar_wait_warp(g.full + s, (j / kGradStages) & 1u)) return false;  // the statistics
-    if (!mbar_wait_warp(g.x_full, used & 1u)) return false;
+    const uint32_t tx = g.tx + 128 * (j & 1);
+    // the statistics have landed for the first products; this thread's own view of them
+    const uint32_t there = kKeys ? mbar_test(g.full + s, (j / kGradStages) & 1u) : 1u;
+    if (!mbar_wait_warp(g.x_full + (j & 1), (j >> 1) & 1u)) return false;
+    if (kKeys && !mbar_wait_tested(there, g.full + s, (j / kGradStages) & 1u)) return false;
     tc_fence_after();
-    uint32_t x[32], y[32];
-    tc_load32(g.tx, x);
-    tc_load32(g.tx + 64, y);
+    uint32_t x[32], y[32], p[16];
+    tc_load32(tx, x);
     tc_wait_ld();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(g.x_free);
-    const int at = (g.begin + (kKeys ? j % g.per_head : j)) * kStep + 32 * h;
+    const int at = (g.begin + block) * kStep + 32 * h;
+    if (++block == g.per_head && kKeys) block = 0;
     const int lo = g.lo0 - at, hi = g.hi0 - at;
     const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 32);
     const float4* st = reinterpret_cast<const float4*>(&stat[s][64 * h]);
-    const float2 c2 = make_float2(g.c, g.c), n2 = make_float2(g.norm, g.norm);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {  // four columns at a time
-      float4 off = make_float4(g.off, g.off, g.off, g.off), del = make_float4(g.del, g.del, g.del, g.del);
-      if (kKeys) {
-        off = st[2 * q];
-        del = st[2 * q + 1];
-      }
+      float4 off = make_float4(g.off, g.off, g.off, g.off);
+      if (kKeys) off = st[2 * q];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int k = 4 * q + 2 * i;
         const float2 e = fma2(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), c2,
                               i == 0 ? make_float2(off.x, off.y) : make_float2(off.z, off.w));
-        const float2 p = make_float2(ex2(e.x), ex2(e.y));
-        float2 d = add2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])),
-                        i == 0 ? make_float2(del.x, del.y) : make_float2(del.z, del.w));
-        if (!Type16<T>::kBf16) d = mul2(d, n2);
-        d = mul2(d, p);
-        x[k] = __float_as_uint(p.x), x[k + 1] = __float_as_uint(p.y);
-        y[k] = __float_as_uint(d.x), y[k + 1] = __float_as_uint(d.y);
+        x[k] = __float_as_uint(ex2(e.x)), x[k + 1] = __float_as_uint(ex2(e.y));
       }
     }
     if (cut) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i < lo || i >= hi) x[i] = y[i] = 0u;
+        if (i < lo || i >= hi) x[i] = 0u;
     }
-    uint32_t p[16], d[16];
+    if (kKeys) {  // P over the X that this warp has read
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (kKeys) p[i] = Type16<T>::pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
-      d[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+      for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+      tc_store16(tx, p);
     }
-    if (used > 0) {  // the second products of two steps before have read P and dS
-      if (!mbar_wait_warp(g.p_free, (used - 1) & 1u)) return false;
-      tc_fence_after();
+    if (!mbar_wait_warp(g.y_full, j & 1u)) return false;
+    tc_fence_after();
+    tc_load32(g.ty, y);
+    tc_wait_ld();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      float4 del = make_float4(g.del, g.del, g.del, g.del);
+      if (kKeys) del = st[2 * q + 1];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = 4 * q + 2 * i;
+        float2 d = add2(make_float2(__uint_as_float(y[k]), __uint_as_float(y[k + 1])),
+                        i == 0 ? make_float2(del.x, del.y) : make_float2(del.z, del.w));
+        if (!Type16<T>::kBf16) d = mul2(d, n2);
+        d = mul2(d, make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+        y[k] = __float_as_uint(d.x), y[k + 1] = __float_as_uint(d.y);
+      }
     }
-    if (kKeys) tc_store16(g.tp, p);
-    tc_store16(g.tp + 32, d);
+    if (cut) {  // 0 x what a foreign row gave may be NaN
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < lo || i >= hi) y[i] = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+    tc_store16(tx + 16, p);
     tc_wait_store();
     tc_fence_before();
     __syncwarp();
@@ -611,8 +618,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, GradArgs g) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) float s_stat[kGradStages][2 * kStep];
-  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], x_free[2], p_full[2],
-      p_free[2], a_ready, done;
+  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], y_full, p_full, a_ready,
+      done;
   __shared__ uint32_t tmem_base_sh;
   __shared__ Item s_item;
   __shared__ float s_norm, s_big[2][kRows];
@@ -636,12 +643,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         mbar_init(&empty[i], 1);
       }
       mbar_init(&landed, 1);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&x_full[i], 1);  // X and Y of the set's next step are in tensor memory
-        mbar_init(&x_free[i], 8);  // its warps have read them
-        mbar_init(&p_full[i], 8);  // P and dS are in tensor memory
-        mbar_init(&p_free[i], 1);  // the second products have read them
-      }
+      mbar_init(&x_full[0], 1);  // X of an even or odd step is in tensor memory
+      mbar_init(&x_full[1], 1);
+      mbar_init(&y_full, 1);     // Y is
+      mbar_init(&p_full, 16);    // P and dS are, and Y has been read
       mbar_init(&a_ready, keys ? 1 : 16);
       mbar_init(&done, 1);
       mbar_fence_init();
@@ -690,9 +695,9 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       if (keys && lane == 0 && steps > 0) {  // A1 = K, A2 = V; rows behind the sequence are rows of no result
         mbar_arrive_expect_tx(&a_ready, 2 * kTileBytes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          tma_load_3d(stages - 2 * kTileBytes + i * kStepBytes, i < 2 ? &tmK : &tmV, &a_ready, 0, kvh,
-                      static_cast<int>(it.k0) + first + (i & 1) * kStep);
+        for (int i = 0; i < 2; ++i)
+          tma_load_3d(stages - (2 - i) * kTileBytes, i == 0 ? &tmK : &tmV, &a_ready, 0, kvh,
+                      static_cast<int>(it.k0) + first);
       }
       bool ok = true;
       uint32_t cut = 0;  // tiles that end inside a step so far
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
             uint64_t* bar = valid >= kStep ? &full[s] : &landed;
             mbar_arrive_expect_tx(bar, kGradStage + (keys ? kStep * 8 : 0));
             tma_load_3d(dst, keys ? &tmQ : &tmK, bar, 0, head, row);
-            tma_load_3d(dst + kStepBytes, keys ? &tmD : &tmV, bar, 0, head, row);
+            tma_load_3d(dst + kTileBytes, keys ? &tmD : &tmV, bar, 0, head, row);
             if (keys)
               bulk_g2s(s_stat[s], stat_at(g, head, stat_start(it.q0, it.seq) + at), kStep * 8, bar);
           }
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           ++cut;
           for (int i = valid * 8 + lane; i < kStep * 8; i += 32) {
             reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-            reinterpret_cast<uint4*>(dst + kStepBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+            reinterpret_cast<uint4*>(dst + kTileBytes)[i] = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_proxy_async_shared();
           __syncwarp();
@@ -730,61 +735,52 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
     } else if (warp == 16) {
-      // ---- first products (the whole warp runs the loop, one lane issues)
+      // ---- products (the whole warp runs the loop, one lane issues)
       if (steps > 0) {
-        constexpr uint32_t idesc = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+        constexpr uint32_t idesc1 = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+        constexpr uint32_t idesc2 = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
         const uint64_t a1 = sw128_desc(base), a2 = a1 + (kTileBytes >> 4);
         bool ok = mbar_wait_warp(&a_ready, 0);
-        for (int j = 0; j < steps && ok; ++j) {
-          const int s = j % kGradStages;
-          const uint32_t x = tmem + (j & 1) * 128;
-          ok = mbar_wait_warp(&full[s], (j / kGradStages) & 1u);
-          if (ok && j >= 2) ok = mbar_wait_warp(&x_free[j & 1], ((j >> 1) & 1u) ^ 1u);
+        for (int j = -2; j < steps && ok; ++j) {
+          if (j >= 0) ok = mbar_wait_warp(&p_full, j & 1u);
+          if (ok && j + 2 < steps) ok = mbar_wait_warp(&full[(j + 2) % kGradStages], ((j + 2) / kGradStages) & 1u);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t b1 = sw128_desc(base + 2 * kTileBytes + s * kGradStage), b2 = b1 + (kStepBytes >> 4);
           if (elect_one()) {
-            if (keys) {
+            if (j + 1 >= 0 && j + 1 < steps) {  // Y of the next step: the last one has been read
+              const uint64_t b2 = sw128_desc(base + 2 * kTileBytes + (j + 1) % kGradStages * kGradStage + kTileBytes);
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
-                tc_mma_f16(x, a1 + 2 * kk, b1 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-                tc_mma_f16(x + 64, a2 + 2 * kk, b2 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                if (keys)
+                  tc_mma_f16(tmem + 256, a2 + 2 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+                else
+                  tc_mma_ta(tmem + 256, tmem + 416 + 8 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
               }
-            } else {
+              tc_commit(&y_full);
+            }
+            const uint32_t x = tmem + 128 * (j & 1);
+            if (j >= 0) {
+              const uint64_t b1 = sw128_mn_desc(base + 2 * kTileBytes + j % kGradStages * kGradStage, kTileBytes),
+                             b2 = b1 + (kTileBytes >> 4);
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk) {  // warp group g left its 32 columns of P and dS from 32 g and 32 g + 16 on
+                const uint32_t p = x + 32 * (kk >> 1) + 8 * (kk & 1);
+                if (keys) tc_mma_ta(tmem + 384, p, b2 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
+                tc_mma_ta(tmem + 448, p + 16, b1 + 128 * kk, idesc2, j != 0 || kk != 0 ? 1u : 0u);
+              }
+              tc_commit(&empty[j % kGradStages]);
+            }
+            if (j + 2 < steps) {  // X of the step after the next, over P and dS of this one
+              const uint64_t b1 = sw128_desc(base + 2 * kTileBytes + (j + 2) % kGradStages * kGradStage);
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
-                tc_mma_ta(x, tmem + 256 + 8 * kk, b1 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
-                tc_mma_ta(x + 64, tmem + 320 + 8 * kk, b2 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+                if (keys)
+                  tc_mma_f16(x, a1 + 2 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+                else
+                  tc_mma_ta(x, tmem + 384 + 8 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
               }
+              tc_commit(&x_full[j & 1]);
             }
-            tc_commit(&x_full[j & 1]);
-          }
-          __syncwarp();
-        }
-        if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
-      }
-    } else if (warp == 18) {
-      // ---- second products
-      if (steps > 0) {
-        constexpr uint32_t idesc = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
-        bool ok = true;
-        for (int j = 0; j < steps && ok; ++j) {
-          const int s = j % kGradStages;
-          const uint32_t p = tmem + 256 + (j & 1) * 64;
-          // the B tiles have landed for the first products; this warp's own view of them
-          ok = mbar_wait_warp(&full[s], (j / kGradStages) & 1u) && mbar_wait_warp(&p_full[j & 1], (j >> 1) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t b1 = sw128_mn_desc(base + 2 * kTileBytes + s * kGradStage, kStepBytes),
-                         b2 = b1 + (kStepBytes >> 4);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (keys) tc_mma_ta(tmem + 384, p + 8 * kk, b2 + 128 * kk, idesc, j != 0 || kk != 0 ? 1u : 0u);
-              tc_mma_ta(tmem + 448, p + 32 + 8 * kk, b1 + 128 * kk, idesc, j != 0 || kk != 0 ? 1u : 0u);
-            }
-            tc_commit(&empty[s]);
-            tc_commit(&p_free[j & 1]);
           }
           __syncwarp();
         }
@@ -792,7 +788,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
       }
     } else {
-      // ---- softmax: thread = row of the A operands; warps 4 g .. 4 g + 3 work on set g % 2, column half g / 2
+      // ---- softmax: thread = row of the A operands; warps 4 g .. 4 g + 3 work on columns 32 g .. + 31 of a step
       const int grp = warp >> 2;
       const int r = (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -824,7 +820,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
           }
           s_big[grp & 1][r] = big;
         }
-        tc_store16(tmem + lanes + (second ? 320 : 256) + 16 * (grp & 1), x);
+        tc_store16(tmem + lanes + 384 + 16 * grp, x);
         tc_wait_store();
         if (live) {
           const float* st = stat_at(g, head, stat_start(it.q0, it.seq) + token);
@@ -840,20 +836,19 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       gr.c = a.scale_log2;
       // the factor of dS besides P's
       gr.norm = Type16<T>::kBf16 ? 1.f : 0.0625f * (keys ? s_norm : normalizer(fmaxf(s_big[0][r], s_big[1][r])));
-      const int set = grp & 1, h = grp >> 1;
-      gr.tx = tmem + lanes + set * 128 + 32 * h;
-      gr.tp = tmem + lanes + 256 + set * 64 + 16 * h;
-      gr.x_full = &x_full[set], gr.x_free = &x_free[set], gr.p_full = &p_full[set], gr.p_free = &p_free[set];
+      gr.tx = tmem + lanes + 32 * grp;
+      gr.ty = tmem + lanes + 256 + 32 * grp;
+      gr.x_full = x_full, gr.y_full = &y_full, gr.p_full = &p_full;
       gr.full = full;
       bool ok;
       if (keys) {
         gr.hi0 = it.lq;
         gr.lo0 = a.causal ? first + r - shift : 0;
-        ok = grad_steps<T, true>(gr, set, h, s_stat, lane);
+        ok = grad_steps<T, true>(gr, grp, s_stat, lane);
       } else {
         gr.lo0 = 0;
         gr.hi0 = (a.causal ? min(it.lk - 1, token + shift) : it.lk - 1) + 1;
-        ok = grad_steps<T, false>(gr, set, h, s_stat, lane);
+        ok = grad_steps<T, false>(gr, grp, s_stat, lane);
       }
       if (ok && steps > 0) ok = mbar_wait_warp(&done, 0);
       if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);

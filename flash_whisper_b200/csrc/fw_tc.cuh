@@ -137,6 +137,24 @@ __device__ __forceinline__ bool elect_one() {
 // This thread's warp index as a value that the compiler knows to be the same in the whole warp.
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0); }
 
+// Whether a phase is complete, without waiting; the answer is only used once it is needed.
+__device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, unsigned parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
+}
+// mbar_wait_warp where mbar_test has been asked before: one vote if the phase was complete in every lane.
+__device__ __forceinline__ bool mbar_wait_tested(uint32_t tested, uint64_t* bar, unsigned parity) {
+  if (__all_sync(0xffffffffu, tested != 0)) return true;
+  return mbar_wait_warp(bar, parity);
+}
+
 // ---- CTA pairs ---------------------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {  // one warp of each CTA
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
