@@ -90,7 +90,8 @@ int fw_device_error(unsigned int* bits, int clear) {
   if (e != cudaSuccess) return fw::set_error(FW_ERR_LAUNCH, "fw_device_error: %s", cudaGetErrorString(e));
   *bits = fw::read_decode_errors(clear != 0) | fw::read_logmel_errors(clear != 0) |
           fw::read_encoder_errors(clear != 0) | fw::read_embed_errors(clear != 0) |
-          fw::read_loss_errors(clear != 0) | fw::read_prompt_errors(clear != 0);
+          fw::read_loss_errors(clear != 0) | fw::read_prompt_errors(clear != 0) |
+          fw::read_prompt_grad_errors(clear != 0);
   return FW_OK;
 }
 

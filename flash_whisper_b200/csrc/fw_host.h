@@ -54,6 +54,7 @@ unsigned int read_encoder_errors(bool clear);
 unsigned int read_embed_errors(bool clear);
 unsigned int read_loss_errors(bool clear);
 unsigned int read_prompt_errors(bool clear);
+unsigned int read_prompt_grad_errors(bool clear);
 
 }  // namespace fw
 
