@@ -12,10 +12,15 @@
 //   second products:  key item: dV += P^T dO, dK += dS^T Q;      query item: dQ += dS K
 // A1 and A2 stay in shared memory for the item, each step's B tile pair serves both products (K-major in the first,
 // MN-major in the second). X, twice, and Y are in tensor memory; P and dS, the A operands of the second products, are
-// written over X. 16 softmax warps (32 rows x 32 columns each) compute a step's exponentials from X while the tensor
-// core is still at the step before's second products and this step's Y, and need Y only then: a step's hand-overs hide
-// behind the exponentials. Steps run on across items: the loads and the first products of the next item start while the
-// results of the last one are read out (one CTA per item spent 8 us outside of its steps).
+// written over X. 16 softmax warps (32 rows x 32 columns each) compute a step's exponentials from X and need Y only after
+// them; Y of the next step is issued, by a warp of its own, as soon as Y has been read, and the second products and X of
+// the step after the next once P and dS are there: a step's hand-overs hide behind the exponentials. Steps run on across
+// items: the loads and the first products of the next item start while the results of the last one are read out (with one
+// CTA per item 24 CTAs an SM spent 8 us each outside of their steps).
+// Tried and slower (six sequences up to 4096, 32 heads on 8; this: 622 us): steps of 64 with two sets of X and Y and 8
+// warps on each (693), all products from one warp (674: its waits add to the products' time), A in tensor memory with P
+// and dS over Y (715), the two halves of the warps taking turns at the exponentials (667), a quarter of the exponentials
+// as polynomials on the FMA pipe (no change).
 // fp16 range: P is kept times 2^8, and dS times 2^4 over the power of two of the largest |do| (of the row in a query
 // item, of the call in a key item), so that gradients of any size keep their bits; bf16 needs neither.
 #include "fw_prompt.cuh"
@@ -26,7 +31,7 @@ constexpr int kStep = 128;  // B rows of a step
 constexpr int kGradStages = 4;
 constexpr uint32_t kGradStage = 2 * kTileBytes;
 constexpr int kGradSmem = 4 * kTileBytes + kGradStages * kGradStage + 1024;  // two pairs of A, the stages
-constexpr int kGradThreads = 32 * 18;                                       // 16 softmax warps, products, loads
+constexpr int kGradThreads = 32 * 19;  // 16 softmax warps, X and second products, loads, Y
 constexpr int kDeltaBlocks = 592;
 constexpr int kRing = 4;  // items known ahead; the first products look two steps, so at most two items, ahead
 
@@ -135,7 +140,7 @@ struct GradRow {
   float off, del;   // of this row (query role): stat's two
   float c, norm;
   uint32_t tx, ty;  // tensor memory: X (the second one 128 columns on) and Y, this warp's columns and lanes
-  uint64_t *x_full, *y_full, *p_full, *full;
+  uint64_t *x_full, *y_full, *y_free, *p_full, *full;
 };
 template <typename T, bool kKeys>
 __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, const float (*stat)[2 * kStep], int lane) {
@@ -156,6 +161,8 @@ __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, c
     if (++block == g.per_head && kKeys) block = 0;
     const int lo = g.lo0 - at, hi = g.hi0 - at;
     const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < 32);
+    uint32_t keep = 0;  // bit i: column i counts
+    if (cut && hi > 0 && lo < 32) keep = (0xffffffffu >> (32 - min(hi, 32))) & (0xffffffffu << max(lo, 0));
     const float4* st = reinterpret_cast<const float4*>(&stat[s][64 * h]);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {  // four columns at a time
@@ -172,7 +179,7 @@ __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, c
     if (cut) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i < lo || i >= hi) x[i] = 0u;
+        if (!(keep & (1u << i))) x[i] = 0u;
     }
     if (kKeys) {  // P over the X that this warp has read
 #pragma unroll
@@ -183,6 +190,9 @@ __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, c
     tc_fence_after();
     tc_load32(g.ty, y);
     tc_wait_ld();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(g.y_free);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       float4 del = make_float4(g.del, g.del, g.del, g.del);
@@ -200,7 +210,7 @@ __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, c
     if (cut) {  // 0 x what a foreign row gave may be NaN
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i < lo || i >= hi) y[i] = 0u;
+        if (!(keep & (1u << i))) y[i] = 0u;
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = Type16<T>::pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
@@ -257,7 +267,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                        const __grid_constant__ CUtensorMap tmQa, const __grid_constant__ CUtensorMap tmDa, GradArgs g) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) float s_stat[kGradStages][2 * kStep];
-  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], y_full, p_full, a_full[2],
+  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], y_full, y_free, p_full, a_full[2],
       a_free[2], done, item_full[kRing], item_free[kRing];
   __shared__ uint32_t tmem_base_sh;
   __shared__ GradItem s_item[kRing];
@@ -281,14 +291,15 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x_full[i], 1);  // X of an even or odd step is in tensor memory
       mbar_init(&a_full[i], 1);  // A1 and A2 of an even or odd item have landed
-      mbar_init(&a_free[i], 1);  // its first products are done
+      mbar_init(&a_free[i], 2);  // its X and its Y are done
     }
     mbar_init(&y_full, 1);   // Y is in tensor memory
-    mbar_init(&p_full, 16);  // P and dS are, and Y has been read
+    mbar_init(&y_free, 16);  // it has been read
+    mbar_init(&p_full, 16);  // P and dS are in tensor memory
     mbar_init(&done, 1);     // an item's results are
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_free[i], 17);  // every role but the loads has read the entry for the last time
+      mbar_init(&item_free[i], 18);  // every role but the loads has read the entry for the last time
     }
     mbar_fence_init();
   }
@@ -413,48 +424,36 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     }
     if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
   } else if (warp == 16) {
-    // ---- products (the whole warp runs the loop, one lane issues): per step Y of the next one, the second products,
-    // X of the one after the next
-    constexpr uint32_t idesc1 = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
-    constexpr uint32_t idesc2 = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
+    // ---- second products, and X of the step after the next over their P and dS (the whole warp runs the loop, one lane
+    // issues)
+    constexpr uint32_t idesc_x = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+    constexpr uint32_t idesc_o = make_idesc(kRows, 64, Type16<T>::kBf16, false, true);
     const uint32_t b_base = base + 4 * kTileBytes;
-    GradCursor cx, cy, cs;
+    GradCursor cx, cs;
     bool ok = true;
     for (int j = -2; ok; ++j) {
+      const uint32_t x = tmem + 128 * (j & 1);
       if (j >= 0) {
         ok = cs.next(s_item, item_full);
         if (!ok || cs.end) break;
         ok = mbar_wait_warp(&p_full, j & 1u);
-      }
-      if (ok && j >= -1 && !cy.end) ok = cy.next(s_item, item_full);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t x = tmem + 128 * (j & 1);
-      if (elect_one()) {
-        if (j >= -1 && !cy.end) {  // Y of step j + 1: the last one has been read
-          const uint64_t a2 = sw128_desc(base + (cy.item & 1) * 2 * kTileBytes + kTileBytes);
-          const uint64_t b2 = sw128_desc(b_base + (j + 1) % kGradStages * kGradStage + kTileBytes);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(tmem + 256, a2 + 2 * kk, b2 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
-          tc_commit(&y_full);
-          if (cy.last) tc_commit(&a_free[cy.item & 1]);
-        }
-        if (j >= 0) {
-          const uint64_t b1 = sw128_mn_desc(b_base + j % kGradStages * kGradStage, kTileBytes),
-                         b2 = b1 + (kTileBytes >> 4);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t b1 = sw128_mn_desc(b_base + j % kGradStages * kGradStage, kTileBytes),
+                       b2 = b1 + (kTileBytes >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {  // warp group g left its 32 columns of P and dS from 32 g and 32 g + 16 on
             const uint32_t p = x + 32 * (kk >> 1) + 8 * (kk & 1);
-            if (cs.keys) tc_mma_ta(tmem + 384, p, b2 + 128 * kk, idesc2, !cs.fresh || kk != 0 ? 1u : 0u);
-            tc_mma_ta(tmem + 448, p + 16, b1 + 128 * kk, idesc2, !cs.fresh || kk != 0 ? 1u : 0u);
+            if (cs.keys) tc_mma_ta(tmem + 384, p, b2 + 128 * kk, idesc_o, !cs.fresh || kk != 0 ? 1u : 0u);
+            tc_mma_ta(tmem + 448, p + 16, b1 + 128 * kk, idesc_o, !cs.fresh || kk != 0 ? 1u : 0u);
           }
           tc_commit(&empty[j % kGradStages]);
           if (cs.last) tc_commit(&done);
         }
+        __syncwarp();
+        if (cs.last && lane == 0) mbar_arrive(&item_free[cs.item % kRing]);
       }
-      __syncwarp();
-      if (j >= 0 && cs.last && lane == 0) mbar_arrive(&item_free[cs.item % kRing]);
       if (cx.end) continue;
       ok = cx.next(s_item, item_full);
       if (!ok || cx.end) continue;
@@ -462,14 +461,41 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       if (ok) ok = mbar_wait_warp(&full[(j + 2) % kGradStages], ((j + 2) / kGradStages) & 1u);
       if (!ok) break;
       tc_fence_after();
-      if (elect_one()) {  // X of step j + 2, over P and dS of step j
-        const uint64_t a1 = sw128_desc(base + (cx.item & 1) * 2 * kTileBytes);
-        const uint64_t b1 = sw128_desc(b_base + (j + 2) % kGradStages * kGradStage);
+      const uint64_t a1 = sw128_desc(base + (cx.item & 1) * 2 * kTileBytes);
+      const uint64_t b1 = sw128_desc(b_base + (j + 2) % kGradStages * kGradStage);
+      if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) tc_mma_f16(x, a1 + 2 * kk, b1 + 2 * kk, idesc1, kk != 0 ? 1u : 0u);
+        for (int kk = 0; kk < 4; ++kk) tc_mma_f16(x, a1 + 2 * kk, b1 + 2 * kk, idesc_x, kk != 0 ? 1u : 0u);
         tc_commit(&x_full[j & 1]);
+        if (cx.last) tc_commit(&a_free[cx.item & 1]);
       }
       __syncwarp();
+    }
+    if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
+  } else if (warp == 18) {
+    // ---- Y
+    constexpr uint32_t idesc = make_idesc(kRows, kStep, Type16<T>::kBf16, false, false);
+    GradCursor c;
+    bool ok = true;
+    while (true) {
+      ok = c.next(s_item, item_full);
+      if (!ok || c.end) break;
+      const int j = c.step, s = j % kGradStages;
+      if (c.fresh) ok = mbar_wait_warp(&a_full[c.item & 1], (c.item >> 1) & 1u);
+      if (ok) ok = mbar_wait_warp(&full[s], (j / kGradStages) & 1u);
+      if (ok && j > 0) ok = mbar_wait_warp(&y_free, (j - 1) & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t a2 = sw128_desc(base + (c.item & 1) * 2 * kTileBytes + kTileBytes);
+      const uint64_t b2 = sw128_desc(base + 4 * kTileBytes + s * kGradStage + kTileBytes);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) tc_mma_f16(tmem + 256, a2 + 2 * kk, b2 + 2 * kk, idesc, kk != 0 ? 1u : 0u);
+        tc_commit(&y_full);
+        if (c.last) tc_commit(&a_free[c.item & 1]);
+      }
+      __syncwarp();
+      if (c.last && lane == 0) mbar_arrive(&item_free[c.item % kRing]);
     }
     if (!ok && lane == 0) prompt_flag(FW_DEVERR_TIMEOUT);
   } else {
@@ -507,7 +533,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       }
       gr.tx = tmem + lanes + 32 * grp;
       gr.ty = tmem + lanes + 256 + 32 * grp;
-      gr.x_full = x_full, gr.y_full = &y_full, gr.p_full = &p_full;
+      gr.x_full = x_full, gr.y_full = &y_full, gr.y_free = &y_free, gr.p_full = &p_full;
       gr.full = full;
       if (keys) {
         gr.hi0 = it.lq;
