@@ -28,17 +28,23 @@ FW_DEFINE_ERROR_WORD();
 __device__ __forceinline__ void loss_flag(unsigned bits) { atomicOr(&g_fw_dev_error, bits); }
 
 constexpr int kBM = 256, kBN = 256, kBK = 64;  // tile of a CTA pair
-constexpr int kStages = 6;
 constexpr uint32_t kHalfBytes = 128 * kBK * 2;  // a CTA's share of A (or B) per stage: 16 KB
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-constexpr int kLossSmem = kStages * kStageBytes + 1024;
 constexpr int kEpiWarps = 8;
+constexpr uint32_t kOutBytes = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes on their way to global memory
 constexpr int kLossThreads = 32 * (2 + kEpiWarps);
 constexpr int kMGroup = 32;  // row tiles that run against a vocabulary tile before the next one: h stays in L2
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kStats, kDz, kGrads };  // what a launch computes
+constexpr int stages_of(int kind) { return kind == kStats ? 6 : 5; }
+constexpr int smem_of(int kind) {
+  return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : kEpiWarps * kOutBytes) + 1024;
+}
+// The tensor core's fp32 additions truncate, which over a contraction of 1280 leaves logits 2e-6 short. For the loss, an
+// fp32 result, it adds up kSegment k blocks at a time and the epilogue adds those rounding to nearest.
+constexpr int kSegment = 4;
 
 struct LossArgs {
   int n, hidden, width;      // rows, hidden size, columns of this launch's vocabulary piece
@@ -132,11 +138,13 @@ __device__ __forceinline__ void mma_block(uint32_t d, uint32_t a_addr, bool fres
     tc_mma_pair(d, ad + kk * (kAMn ? 128 : 2), bd + kk * (kBMn ? 128 : 2), idesc, fresh && kk == 0 ? 0u : 1u);
 }
 
-// tmA, tmB: the operands of kStats, kDz and of kGrads' dh; tmA2, tmB2: of kGrads' dW.
+// tmA, tmB: the operands of kStats, kDz and of kGrads' dh; tmA2, tmB2: of kGrads' dW. tmOut: dz or dW, tmPart: dh's sums.
 template <int kKind, typename T>
 __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
     loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2, LossArgs a) {
+                     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
+                     const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmPart, LossArgs a) {
+  constexpr int kStages = stages_of(kKind);
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base_sh;
@@ -209,45 +217,51 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
     if (rank == 0) {  // the whole warp runs the loop, one lane issues
       int it = 0, local = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += pairs, ++local) {
+      for (int t = first; t < tiles && ok; t += pairs) {
         const Tile x = tile_at<kKind>(a, t);
-        const int buf = local & 1;
-        if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
-        tc_fence_after();
-        const uint32_t d = tmem + buf * kBN;
-        for (int kb = 0; kb < x.kbs && ok; ++kb, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u);
-          if (!ok) break;
+        const int segment = kKind == kStats ? kSegment : x.kbs;
+        for (int kb0 = 0; kb0 < x.kbs && ok; kb0 += segment, ++local) {
+          const int buf = local & 1;
+          if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
           tc_fence_after();
-          const uint32_t at = base + s * kStageBytes;
-          if (elect_one()) {
-            if (kKind != kGrads)
-              mma_block<T, false, false>(d, at, kb == 0);
-            else if (x.dh)
-              mma_block<T, false, true>(d, at, kb == 0);
-            else
-              mma_block<T, true, true>(d, at, kb == 0);
-            tc_commit_pair(&empty_bar[s]);
+          const uint32_t d = tmem + buf * kBN;
+          const int kb1 = min(x.kbs, kb0 + segment);
+          for (int kb = kb0; kb < kb1 && ok; ++kb, ++it) {
+            const int s = it % kStages;
+            ok = mbar_wait_warp(&full_bar[s], (it / kStages) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t at = base + s * kStageBytes;
+            if (elect_one()) {
+              if (kKind != kGrads)
+                mma_block<T, false, false>(d, at, kb == kb0);
+              else if (x.dh)
+                mma_block<T, false, true>(d, at, kb == kb0);
+              else
+                mma_block<T, true, true>(d, at, kb == kb0);
+              tc_commit_pair(&empty_bar[s]);
+            }
+            __syncwarp();
           }
+          if (elect_one()) tc_commit_pair(&acc_full[buf]);
           __syncwarp();
         }
-        if (elect_one()) tc_commit_pair(&acc_full[buf]);
-        __syncwarp();
       }
       if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
     }
   } else {
     // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns
-    // 128 ((w - 2) / 4) .. + 127.
+    // 128 ((w - 2) / 4) .. + 127. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128 bytes, 128-byte
+    // swizzle) to tensor stores: 16 bytes a thread straight to rows 2560 bytes apart took three times as long.
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t drained = cluster_map(&acc_empty[0], 0);
+    uint8_t* out = smem + kStages * kStageBytes + (warp - 2) * kOutBytes;
     bool failed = false;
     int local = 0;
-    for (int t = first; t < tiles; t += pairs, ++local) {
+    for (int t = first; t < tiles && !failed; t += pairs) {
       const Tile x = tile_at<kKind>(a, t);
-      const int buf = local & 1;
-      const int row = x.m0 + 128 * static_cast<int>(rank) + q * 32 + lane;
+      const int row0 = x.m0 + 128 * static_cast<int>(rank) + q * 32;  // the warp's first row
+      const int row = row0 + lane;
       const int c0 = x.n0 + 128 * part;
       int64_t target = -1;  // relative to this launch's vocabulary piece
       float neg_lse = 0.f;
@@ -258,101 +272,149 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
         target = tg - a.v0;
         if (kKind == kDz) neg_lse = -a.lse[row] * kLog2e;
       }
-      if (failed || !mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
-        if (!failed) loss_flag(FW_DEVERR_TIMEOUT);
+      if (kKind == kStats) {
+        float z[128];
+        for (int kb0 = 0; kb0 < x.kbs; kb0 += kSegment, ++local) {
+          const int buf = local & 1;
+          if (!mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
+            failed = true;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + 128 * part;
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t r[16];
+            tc_ld16(d + c, r);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[c + j] = kb0 == 0 ? __uint_as_float(r[j]) : z[c + j] + __uint_as_float(r[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(drained + 8 * buf);
+        }
+        if (failed) break;
+        if (c0 + 128 > a.width) {  // columns behind the vocabulary count as -inf
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (c0 + j >= a.width) z[j] = -INFINITY;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], z[j]);
+        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (target >= c0 && target < c0 + 128) {
+          const int at = static_cast<int>(target) - c0;
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if (j == at) a.target_logit[row] = z[j];
+        }
+        const float off = m == -INFINITY ? 0.f : -m * kLog2e;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j & 3] += ex2(fmaf(z[j], kLog2e, off));
+        if (row < a.n)
+          a.stats[static_cast<int64_t>(2 * (x.n0 / kBN) + part) * a.n + row] =
+              make_float2(m, (acc[0] + acc[1]) + (acc[2] + acc[3]));
+        __syncwarp();
+        continue;
+      }
+      const int buf = local & 1;
+      if (!mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
         failed = true;
         break;
       }
+      ++local;
       tc_fence_after();
       const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + 128 * part;
-      float top = -INFINITY, sum = 0.f;
+      const bool wide = kKind == kGrads && x.dh;  // fp32 rows of 32 columns, else 16-bit rows of 64
+      const bool direct = kKind == kGrads && !x.dh && a.accumulate;
+      const float f = kKind == kGrads && !x.dh ? *a.gmax / a.dz_scale : 1.f;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
         uint32_t r[32];
         tc_load32(d + c, r);
         tc_wait_ld();
         const int col = c0 + c;
-        if (kKind == kStats) {
-          if (col + 32 > a.width) {  // columns behind the vocabulary count as -inf
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col + j >= a.width) r[j] = 0xff800000u;
-          }
-          float m = top;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) m = fmaxf(m, __uint_as_float(r[j]));
-          const float off = m == -INFINITY ? 0.f : -m * kLog2e;
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[j & 3] += ex2(fmaf(__uint_as_float(r[j]), kLog2e, off));
-          sum = fmaf(sum, ex2(fmaf(top, kLog2e, off)), (acc[0] + acc[1]) + (acc[2] + acc[3]));
-          top = m;
-          if (target >= col && target < col + 32) {
-            const int at = static_cast<int>(target) - col;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j == at) a.target_logit[row] = __uint_as_float(r[j]);
-          }
-        } else if (kKind == kDz && row < a.n) {
+        if (kKind == kDz) {
           const int at = target >= col && target < col + 32 ? static_cast<int>(target) - col : -1;
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.dz) + static_cast<int64_t>(row) * a.ld_dz + col);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const float p = ex2(fmaf(__uint_as_float(r[j]), kLog2e, neg_lse)) - (j == at ? 1.f : 0.f);
             r[j] = __float_as_uint(kept ? p * a.dz_scale : 0.f);
           }
+        } else if (!wide) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            dst[j] = make_uint4(Type16<T>::pack(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1])),
-                                Type16<T>::pack(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3])),
-                                Type16<T>::pack(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5])),
-                                Type16<T>::pack(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7])));
-        } else if (kKind == kGrads && x.dh && row < a.n) {
-          float* dst = a.part + (static_cast<int64_t>(x.split) * a.n + row) * a.hidden + col;
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+        }
+        if (direct) {  // dW added to what is there
+          if (row < a.width) {
+            uint4* dst =
+                reinterpret_cast<uint4*>(static_cast<T*>(a.dw) + (static_cast<int64_t>(a.v0) + row) * a.hidden + col);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            if (col + j >= a.hidden) break;
-            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
-                                   __uint_as_float(r[j + 3]));
-            float4* at = reinterpret_cast<float4*>(dst + j);
-            if (!a.first_piece) {
-              const float4 o = *at;
-              v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
-            }
-            *at = v;
-          }
-        } else if (kKind == kGrads && !x.dh && row < a.width) {
-          const float f = *a.gmax / a.dz_scale;
-          uint4* dst =
-              reinterpret_cast<uint4*>(static_cast<T*>(a.dw) + (static_cast<int64_t>(a.v0) + row) * a.hidden + col);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (col + 8 * j >= a.hidden) break;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[8 * j + i]) * f;
-            if (a.accumulate) {
+            for (int j = 0; j < 4; ++j) {
+              if (col + 8 * j >= a.hidden) break;
               const uint4 o = dst[j];
               const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+              uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float2 u = Type16<T>::unpack(ow[i]);
-                v[2 * i] += u.x;
-                v[2 * i + 1] += u.y;
+                w[i] = Type16<T>::pack(__uint_as_float(r[8 * j + 2 * i]) + u.x, __uint_as_float(r[8 * j + 2 * i + 1]) + u.y);
               }
+              dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            dst[j] = make_uint4(Type16<T>::pack(v[0], v[1]), Type16<T>::pack(v[2], v[3]), Type16<T>::pack(v[4], v[5]),
-                                Type16<T>::pack(v[6], v[7]));
+          }
+          __syncwarp();
+          continue;
+        }
+        const bool first_half = wide || c % 64 == 0;
+        if (first_half) {  // the last store has read the buffer
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
+        }
+        uint8_t* mine = out + lane * 128;
+        if (wide) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(mine + ((j ^ (lane & 7)) << 4)) =
+                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int chunk = (c % 64) / 8 + j;
+            *reinterpret_cast<uint4*>(mine + ((chunk ^ (lane & 7)) << 4)) =
+                make_uint4(Type16<T>::pack(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1])),
+                           Type16<T>::pack(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3])),
+                           Type16<T>::pack(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5])),
+                           Type16<T>::pack(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7])));
+          }
+        }
+        if (wide || c % 64 == 32) {
+          fence_proxy_async_shared();
+          __syncwarp();
+          // rows and columns behind the end of a partly covered box are not written
+          const int at = wide ? col : col - 32;
+          const int rows = kKind == kDz || wide ? a.n : a.width, cols = kKind == kDz ? a.width : a.hidden;
+          if (lane == 0 && row0 < rows && at < cols) {
+            if (!wide)
+              tma_store_2d(&tmOut, out, at, row0);
+            else if (a.first_piece)
+              tma_store_3d(&tmPart, out, at, row0, x.split);
+            else
+              tma_add_3d(&tmPart, out, at, row0, x.split);
+            tma_store_commit();
           }
         }
         __syncwarp();  // the next load is a warp-wide instruction
       }
-      if (kKind == kStats && row < a.n)
-        a.stats[static_cast<int64_t>(2 * (x.n0 / kBN) + part) * a.n + row] = make_float2(top, sum);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(drained + 8 * buf);
     }
+    if (kKind != kStats && lane == 0) tma_store_wait();
+    if (failed && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
   }
 
   tc_fence_before();
@@ -363,7 +425,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
 }
 
 // Joins the (max, sum) of all half tiles of a row: 32 rows per CTA (lanes), the half tiles over its warps.
-constexpr int kCombineThreads = 512;
+constexpr int kCombineThreads = 1024;
 __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const float2* __restrict__ stats, int halves,
                                                                        int n, const int64_t* __restrict__ targets,
                                                                        int64_t ignore, int vocab, float* loss,
@@ -375,7 +437,7 @@ __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const flo
   const int row = blockIdx.x * 32 + lane;
   float top = -INFINITY, sum = 0.f;
   if (row < n) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < halves; i += kWarps) {
       const float2 v = stats[static_cast<int64_t>(i) * n + row];
       const float m = fmaxf(top, v.x), off = m == -INFINITY ? 0.f : -m * kLog2e;
@@ -538,15 +600,32 @@ static int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* ptr, i
   return FW_OK;
 }
 
+// 3-D map over fp32 sums [splits][n][hidden]; boxes of 32 x 32.
+static int make_part_map(CUtensorMap* m, const void* ptr, int hidden, int n, int splits) {
+  EncodeTiledFn enc = tensor_map_encode_fn();
+  if (!enc) return set_error(FW_ERR_LAUNCH, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(hidden), static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(splits)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(hidden) * 4, static_cast<cuuint64_t>(hidden) * 4 * n};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FW_ERR_ARG, "lm_head_loss: tensor map encode failed (%d)", static_cast<int>(r));
+  return FW_OK;
+}
+
 template <int kKind, typename T>
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ta2, const CUtensorMap& tb2,
-                       const LossArgs& a, int tiles, cudaStream_t s, bool pdl) {
+                       const CUtensorMap& tout, const CUtensorMap& tpart, const LossArgs& a, int tiles, cudaStream_t s,
+                       bool pdl) {
+  constexpr int kLossSmem = smem_of(kKind);
   auto kern = loss_gemm_kernel<kKind, T>;
   cudaError_t e = ensure_smem(kern, kLossSmem);
   if (e == cudaSuccess) {
     const int pairs = num_sms() / 2;
     e = launch(kern, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kLossThreads), kLossSmem, s, pdl, ta, tb, ta2,
-               tb2, a);
+               tb2, tout, tpart, a);
   }
   return launch_status(e, "lm_head_loss");
 }
@@ -569,7 +648,7 @@ static int run_loss(const void* h, const void* w, const int64_t* targets, float*
   a.targets = targets;
   a.stats = static_cast<float2*>(ws);
   a.target_logit = loss;  // replaced by the loss when the halves are joined
-  rc = launch_gemm<kStats, T>(ta, tb, ta, tb, a, a.m_tiles * a.n_tiles, s, false);
+  rc = launch_gemm<kStats, T>(ta, tb, ta, tb, ta, ta, a, a.m_tiles * a.n_tiles, s, false);
   if (rc) return rc;
   cudaError_t e = launch(loss_combine_kernel, dim3((n + 31) / 32), dim3(kCombineThreads), 0, s, true,
                          static_cast<const float2*>(a.stats), 2 * l.n_tiles, n, targets, ignore, vocab, loss, lse);
@@ -593,9 +672,10 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
                          dim3(256), 0, s, false, static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden, scaled,
                          gmax);
   int rc = launch_status(e, "lm_head_loss_grad scale");
-  CUtensorMap ta, tb, ga, gb, ga2, gb2;
+  CUtensorMap ta, tb, ga, gb, ga2, gb2, tz, tw, tp;
   if (!rc) rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
   if (!rc) rc = make_map(&gb2, Type16<T>::kMap, scaled, hidden, n, hidden, 64);
+  if (!rc) rc = make_part_map(&tp, part, hidden, n, l.splits);
   for (int p = 0; p < l.pieces && !rc; ++p) {
     const int v0 = p * l.width, width = vocab - v0 < l.width ? vocab - v0 : l.width;
     const T* wp = static_cast<const T*>(w) + static_cast<int64_t>(v0) * hidden;
@@ -603,6 +683,10 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     if (!rc) rc = make_map(&ga, Type16<T>::kMap, dz, width, n, l.width, 128);
     if (!rc) rc = make_map(&gb, Type16<T>::kMap, wp, hidden, width, hidden, 64);
     if (!rc) rc = make_map(&ga2, Type16<T>::kMap, dz, width, n, l.width, 64);
+    if (!rc) rc = make_map(&tz, Type16<T>::kMap, dz, width, n, l.width, 32);
+    if (!rc && dw != nullptr)
+      rc = make_map(&tw, Type16<T>::kMap, static_cast<T*>(dw) + static_cast<int64_t>(v0) * hidden, hidden, width, hidden, 32);
+    if (!rc && dw == nullptr) tw = tz;  // not used
     if (rc) return rc;
     LossArgs a{};
     a.n = n;
@@ -618,7 +702,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     a.dz = dz;
     a.ld_dz = l.width;
     a.dz_scale = dz_scale;
-    rc = launch_gemm<kDz, T>(ta, tb, ta, tb, a, a.m_tiles * a.n_tiles, s, true);
+    rc = launch_gemm<kDz, T>(ta, tb, ta, tb, tz, tz, a, a.m_tiles * a.n_tiles, s, true);
     if (rc) return rc;
     a.m_tiles = dw != nullptr ? (width + kBM - 1) / kBM : 0;
     a.n_tiles = (hidden + kBN - 1) / kBN;
@@ -629,7 +713,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     a.gmax = gmax;
     a.first_piece = p == 0;
     a.accumulate = accumulate;
-    rc = launch_gemm<kGrads, T>(ga, gb, ga2, gb2, a, (a.dh_m_tiles * a.splits + a.m_tiles) * a.n_tiles, s, true);
+    rc = launch_gemm<kGrads, T>(ga, gb, ga2, gb2, tw, tp, a, (a.dh_m_tiles * a.splits + a.m_tiles) * a.n_tiles, s, true);
   }
   if (rc || dh == nullptr) return rc;
   e = launch(loss_dh_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, true,
