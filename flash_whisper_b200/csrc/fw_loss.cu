@@ -42,9 +42,14 @@ constexpr int stages_of(int kind) { return kind == kStats ? 6 : 5; }
 constexpr int smem_of(int kind) {
   return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : kEpiWarps * kOutBytes) + 1024;
 }
-// The tensor core's fp32 additions truncate, which over a contraction of 1280 leaves logits 2e-6 short. For the loss, an
-// fp32 result, it adds up kSegment k blocks at a time and the epilogue adds those rounding to nearest.
-constexpr int kSegment = 4;
+// The tensor core's fp32 additions truncate: 80 of them leave logits 1.3e-6 of their size short. For the loss, an fp32
+// result, it adds up at most 10 k blocks (40 additions) at a time, and the epilogue adds those segments rounding to
+// nearest. A segment takes the tensor core longer than a tile's exponentials take the epilogue, so it never waits
+// (segments of 4 left it idle for a fifth of the time).
+constexpr int kSegment = 10;
+__host__ __device__ constexpr int segment_of(int kbs) {
+  return (kbs + (kbs + kSegment - 1) / kSegment - 1) / ((kbs + kSegment - 1) / kSegment);
+}
 
 struct LossArgs {
   int n, hidden, width;      // rows, hidden size, columns of this launch's vocabulary piece
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       bool ok = true;
       for (int t = first; t < tiles && ok; t += pairs) {
         const Tile x = tile_at<kKind>(a, t);
-        const int segment = kKind == kStats ? kSegment : x.kbs;
+        const int segment = kKind == kStats ? segment_of(x.kbs) : x.kbs;
         for (int kb0 = 0; kb0 < x.kbs && ok; kb0 += segment, ++local) {
           const int buf = local & 1;
           if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
@@ -274,7 +279,8 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       }
       if (kKind == kStats) {
         float z[128];
-        for (int kb0 = 0; kb0 < x.kbs; kb0 += kSegment, ++local) {
+        const int segment = segment_of(x.kbs);
+        for (int kb0 = 0; kb0 < x.kbs; kb0 += segment, ++local) {
           const int buf = local & 1;
           if (!mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
             failed = true;
@@ -300,23 +306,27 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
           for (int j = 0; j < 128; ++j)
             if (c0 + j >= a.width) z[j] = -INFINITY;
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], z[j]);
-        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], z[j]), z[j + 1]);
         if (target >= c0 && target < c0 + 128) {
           const int at = static_cast<int>(target) - c0;
 #pragma unroll
           for (int j = 0; j < 128; ++j)
             if (j == at) a.target_logit[row] = z[j];
         }
-        const float off = m == -INFINITY ? 0.f : -m * kLog2e;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        // the maximum in powers of two, rounded once: the sum is relative to exactly this number
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+        const float off = top == -INFINITY ? 0.f : -top;
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int j = 0; j < 128; ++j) acc[j & 3] += ex2(fmaf(z[j], kLog2e, off));
+        for (int j = 0; j < 128; j += 2) {
+          const float2 e = fma2(make_float2(z[j], z[j + 1]), make_float2(kLog2e, kLog2e), make_float2(off, off));
+          acc[(j >> 1) & 1] = add2(acc[(j >> 1) & 1], make_float2(ex2(e.x), ex2(e.y)));
+        }
+        acc[0] = add2(acc[0], acc[1]);
         if (row < a.n)
-          a.stats[static_cast<int64_t>(2 * (x.n0 / kBN) + part) * a.n + row] =
-              make_float2(m, (acc[0] + acc[1]) + (acc[2] + acc[3]));
+          a.stats[static_cast<int64_t>(2 * (x.n0 / kBN) + part) * a.n + row] = make_float2(top, acc[0].x + acc[0].y);
         __syncwarp();
         continue;
       }
@@ -424,7 +434,8 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// Joins the (max, sum) of all half tiles of a row: 32 rows per CTA (lanes), the half tiles over its warps.
+// Joins the (max, sum) of all half tiles of a row, both in powers of two, so that the differences of maxima are exact:
+// 32 rows per CTA (lanes), the half tiles over its warps.
 constexpr int kCombineThreads = 1024;
 __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const float2* __restrict__ stats, int halves,
                                                                        int n, const int64_t* __restrict__ targets,
@@ -440,8 +451,8 @@ __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const flo
 #pragma unroll 8
     for (int i = warp; i < halves; i += kWarps) {
       const float2 v = stats[static_cast<int64_t>(i) * n + row];
-      const float m = fmaxf(top, v.x), off = m == -INFINITY ? 0.f : -m * kLog2e;
-      sum = sum * ex2(fmaf(top, kLog2e, off)) + v.y * ex2(fmaf(v.x, kLog2e, off));
+      const float m = fmaxf(top, v.x), off = m == -INFINITY ? 0.f : -m;
+      sum = sum * ex2(top + off) + v.y * ex2(v.x + off);
       top = m;
     }
   }
@@ -451,11 +462,11 @@ __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const flo
   float m = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_part[w][lane].x);
-  const float off = m == -INFINITY ? 0.f : -m * kLog2e;
+  const float off = m == -INFINITY ? 0.f : -m;
   float s = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) s += s_part[w][lane].y * ex2(fmaf(s_part[w][lane].x, kLog2e, off));
-  const float l = m + logf(s);
+  for (int w = 0; w < kWarps; ++w) s += s_part[w][lane].y * ex2(s_part[w][lane].x + off);
+  const float l = m == -INFINITY ? logf(s) : fmaf(m, kLn2, logf(s));
   const int64_t t = targets[row];
   const bool bad = t != ignore && (t < 0 || t >= vocab);
   if (bad) loss_flag(FW_DEVERR_BAD_INDEX);
