@@ -42,13 +42,14 @@ constexpr int stages_of(int kind) { return kind == kStats ? 6 : 5; }
 constexpr int smem_of(int kind) {
   return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : kEpiWarps * kOutBytes) + 1024;
 }
-// The tensor core's fp32 additions truncate: 80 of them leave logits 1.3e-6 of their size short. For the loss, an fp32
-// result, it adds up at most 10 k blocks (40 additions) at a time, and the epilogue adds those segments rounding to
-// nearest. A segment takes the tensor core longer than a tile's exponentials take the epilogue, so it never waits
-// (segments of 4 left it idle for a fifth of the time).
-constexpr int kSegment = 10;
+// The tensor core's fp32 additions truncate: the 80 of a contraction of 1280 leave logits 1.3e-6 (bf16) or 2.4e-6 (fp16)
+// of their size short. For the loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
+// those segments rounding to nearest: below 8e-7 for any contraction. The tensor core is at the next segment meanwhile;
+// shorter ones leave it idle during a tile's exponentials (16381 rows: none 1265 us, 10 1355, 7 1466, 4 1850).
+template <typename T>
 __host__ __device__ constexpr int segment_of(int kbs) {
-  return (kbs + (kbs + kSegment - 1) / kSegment - 1) / ((kbs + kSegment - 1) / kSegment);
+  constexpr int most = Type16<T>::kBf16 ? 10 : 7;
+  return (kbs + (kbs + most - 1) / most - 1) / ((kbs + most - 1) / most);
 }
 
 struct LossArgs {
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       bool ok = true;
       for (int t = first; t < tiles && ok; t += pairs) {
         const Tile x = tile_at<kKind>(a, t);
-        const int segment = kKind == kStats ? segment_of(x.kbs) : x.kbs;
+        const int segment = kKind == kStats ? segment_of<T>(x.kbs) : x.kbs;
         for (int kb0 = 0; kb0 < x.kbs && ok; kb0 += segment, ++local) {
           const int buf = local & 1;
           if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       }
       if (kKind == kStats) {
         float z[128];
-        const int segment = segment_of(x.kbs);
+        const int segment = segment_of<T>(x.kbs);
         for (int kb0 = 0; kb0 < x.kbs; kb0 += segment, ++local) {
           const int buf = local & 1;
           if (!mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u)) {
