@@ -30,17 +30,18 @@ __device__ __forceinline__ void loss_flag(unsigned bits) { atomicOr(&g_fw_dev_er
 constexpr int kBM = 256, kBN = 256, kBK = 64;  // tile of a CTA pair
 constexpr uint32_t kHalfBytes = 128 * kBK * 2;  // a CTA's share of A (or B) per stage: 16 KB
 constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-constexpr int kEpiWarps = 8;
 constexpr uint32_t kOutBytes = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes on their way to global memory
-constexpr int kLossThreads = 32 * (2 + kEpiWarps);
 constexpr int kMGroup = 32;  // row tiles that run against a vocabulary tile before the next one: h stays in L2
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kStats, kDz, kGrads };  // what a launch computes
-constexpr int stages_of(int kind) { return kind == kStats ? 6 : 5; }
+constexpr int stages_of(int kind) { return kind == kStats ? 6 : kind == kDz ? 5 : 4; }
+// Epilogue warps: twice as many where the products are short (dW of few rows) and the epilogue has little to compute.
+constexpr int epi_warps(int kind) { return kind == kGrads ? 16 : 8; }
+constexpr int threads_of(int kind) { return 32 * (2 + epi_warps(kind)); }
 constexpr int smem_of(int kind) {
-  return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : kEpiWarps * kOutBytes) + 1024;
+  return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : epi_warps(kind) * kOutBytes) + 1024;
 }
 // The tensor core's fp32 additions truncate: the 80 of a contraction of 1280 leave logits 1.3e-6 (bf16) or 2.4e-6 (fp16)
 // of their size short. For the loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
@@ -146,7 +147,7 @@ __device__ __forceinline__ void mma_block(uint32_t d, uint32_t a_addr, bool fres
 
 // tmA, tmB: the operands of kStats, kDz and of kGrads' dh; tmA2, tmB2: of kGrads' dW. tmOut: dz or dW, tmPart: dh's sums.
 template <int kKind, typename T>
-__global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1)
     loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
                      const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmPart, LossArgs a) {
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * kEpiWarps);  // leader's: both CTAs' epilogue warps have drained the buffer
+      mbar_init(&acc_empty[b], 2 * epi_warps(kKind));  // leader's: both CTAs' epilogue warps have drained the buffer
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
@@ -257,10 +258,11 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
     }
   } else {
     // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns
-    // 128 ((w - 2) / 4) .. + 127. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128 bytes, 128-byte
+    // kCols ((w - 2) / 4) .. + kCols - 1. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128 bytes, 128-byte
     // swizzle) to tensor stores: 16 bytes a thread straight to rows 2560 bytes apart took three times as long.
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t drained = cluster_map(&acc_empty[0], 0);
+    constexpr int kCols = 2 * 4 * 128 / epi_warps(kKind);  // columns of a warp
     uint8_t* out = smem + kStages * kStageBytes + (warp - 2) * kOutBytes;
     bool failed = false;
     int local = 0;
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       const Tile x = tile_at<kKind>(a, t);
       const int row0 = x.m0 + 128 * static_cast<int>(rank) + q * 32;  // the warp's first row
       const int row = row0 + lane;
-      const int c0 = x.n0 + 128 * part;
+      const int c0 = x.n0 + kCols * part;
       int64_t target = -1;  // relative to this launch's vocabulary piece
       float neg_lse = 0.f;
       bool kept = false;
@@ -338,12 +340,12 @@ __global__ void __launch_bounds__(kLossThreads, 1) __cluster_dims__(2, 1, 1)
       }
       ++local;
       tc_fence_after();
-      const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + 128 * part;
+      const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + kCols * part;
       const bool wide = kKind == kGrads && x.dh;  // fp32 rows of 32 columns, else 16-bit rows of 64
       const bool direct = kKind == kGrads && !x.dh && a.accumulate;
       const float f = kKind == kGrads && !x.dh ? *a.gmax / a.dz_scale : 1.f;
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
+      for (int c = 0; c < kCols; c += 32) {
         uint32_t r[32];
         tc_load32(d + c, r);
         tc_wait_ld();
@@ -636,7 +638,7 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   cudaError_t e = ensure_smem(kern, kLossSmem);
   if (e == cudaSuccess) {
     const int pairs = num_sms() / 2;
-    e = launch(kern, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(kLossThreads), kLossSmem, s, pdl, ta, tb, ta2,
+    e = launch(kern, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(threads_of(kKind)), kLossSmem, s, pdl, ta, tb, ta2,
                tb2, tout, tpart, a);
   }
   return launch_status(e, "lm_head_loss");
