@@ -16,6 +16,7 @@ stream. There is no CPU path: without a CUDA tensor the checks fail.
 """
 
 import ctypes
+import functools
 
 import torch
 
@@ -46,48 +47,60 @@ def _check_cuda(t, dtype, name, what):
 
 
 _DTYPES = {torch.float16: _lib.FW_F16, torch.bfloat16: _lib.FW_BF16, torch.float32: _lib.FW_F32}
+_HALF_TYPES = (torch.float16, torch.bfloat16)
 
 
-def _check_typed(t, like, name):
-    """A contiguous CUDA tensor of like's type on like's device."""
-    if not (t.is_cuda and t.is_contiguous() and t.dtype == like.dtype and t.device == like.device):
-        raise RuntimeError(f'{name} must be contiguous CUDA {str(like.dtype)[6:]} on {like.device}')
+# The whole-transcript operators' checks and calls. They cost as much as a small operator takes on the GPU, so messages
+# are made only where they are raised, devices are compared by index, and pointers are passed as plain integers.
+def _check_typed(t, dtype, dev, name):
+    """A contiguous tensor of this type on CUDA device `dev`."""
+    if t.dtype is not dtype or dev < 0 or t.get_device() != dev or not t.is_contiguous():
+        where = f'on cuda:{dev}' if dev >= 0 else 'on a CUDA device'
+        raise RuntimeError(f'{name} must be contiguous CUDA {str(dtype)[6:]} {where}')
 
 
-def _check_ints(t, n, like, name):
-    if not (t.is_cuda and t.is_contiguous() and t.dtype == torch.long and t.numel() == n and t.device == like.device):
-        raise RuntimeError(f'{name} must be contiguous CUDA int64 [{n}] on {like.device}')
+def _check_ints(t, n, dev, name):
+    if t.dtype is not torch.long or dev < 0 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f'{name} must be contiguous CUDA int64 [{n}] on cuda:{dev}')
 
 
-class _On:
-    """Makes `device` current for the calls within (nothing to do where it is already)."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _check_fp32(t, n, dev, name):
+    if t.dtype is not torch.float32 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f'{name} must be contiguous CUDA fp32 [{n}] on cuda:{dev}')
 
 
+@functools.lru_cache(maxsize=1024)
 def _workspace_bytes(name, *sizes):
     need = ctypes.c_int64(0)
-    _lib.call(name, *map(int, sizes), ctypes.byref(need))
+    _lib.call(name, *sizes, ctypes.byref(need))
     return need.value
 
 
-def _workspace(ws, need, device):
-    """The caller's scratch after a check of its size, or (None) scratch of the current stream."""
+def _workspace(ws, need, dev):
+    """The caller's scratch after a check of its size, or (None) scratch of the device's current stream."""
     if ws is None:
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    if not (ws.is_cuda and ws.is_contiguous() and ws.dtype == torch.uint8 and ws.device == device
-            and ws.numel() >= need):
-        raise RuntimeError(f'ws must be contiguous CUDA uint8 on {device} of at least {need} bytes')
+        return torch.empty(need, dtype=torch.uint8, device=f'cuda:{dev}') if need else None
+    if (ws.dtype is not torch.uint8 or ws.get_device() != dev or ws.numel() < need or not ws.is_contiguous()):
+        raise RuntimeError(f'ws must be contiguous CUDA uint8 on cuda:{dev} of at least {need} bytes')
     return ws
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _size(ws):
+    return 0 if ws is None else ws.numel()
+
+
+def _call_on(dev, name, *args):
+    """Calls fw_<name> on device `dev`, whichever is current, and its current stream."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch.cuda.current_device() == dev:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
 
 
 class Ext:
@@ -311,150 +324,147 @@ class Ext:
     # scratch of at least the matching *_workspace bytes; without it scratch is allocated on that stream.
     def embed_scaled(self, embed, ids, out, scale=1.0, pos_embed=None, positions=None):
         """out[i] = embed[ids[i]] * scale (+ pos_embed[positions[i]]) in fp16, bf16 or fp32."""
-        _check(embed.dtype in _DTYPES, 'embed must be fp16, bf16 or fp32')
-        _check_typed(embed, embed, 'embed')
-        _check_typed(out, embed, 'out')
-        n = ids.numel()
-        _check_ints(ids, n, embed, 'ids')
+        dtype, dev, n = embed.dtype, embed.get_device(), ids.numel()
+        _check(dtype in _DTYPES, 'embed must be fp16, bf16 or fp32')
+        _check_typed(embed, dtype, dev, 'embed')
+        _check_typed(out, dtype, dev, 'out')
+        _check_ints(ids, n, dev, 'ids')
         _check(embed.dim() == 2 and embed.numel() > 0, 'embed must be [vocab, hidden]')
         vocab, hidden = embed.shape
         _check((pos_embed is None) == (positions is None), 'pos_embed and positions must be given together')
         max_pos = 0
         if pos_embed is not None:
-            _check_typed(pos_embed, embed, 'pos_embed')
-            _check_ints(positions, n, embed, 'positions')
+            _check_typed(pos_embed, dtype, dev, 'pos_embed')
+            _check_ints(positions, n, dev, 'positions')
             _check(pos_embed.dim() == 2 and pos_embed.size(1) == hidden and pos_embed.numel() > 0,
                    'pos_embed must be [max_pos, hidden]')
             max_pos = pos_embed.size(0)
         _check(out.numel() == n * hidden, 'embed_scaled: out must be [n, hidden]')
-        with _On(embed.device):
-            _lib.call('fw_embed_scaled', _ptr(embed), _ptr(pos_embed), _ptr(ids), _ptr(positions), _ptr(out), n, vocab,
-                      max_pos, hidden, float(scale), _DTYPES[embed.dtype], _stream())
+        _call_on(dev, 'fw_embed_scaled', embed.data_ptr(), _address(pos_embed), ids.data_ptr(), _address(positions),
+                 out.data_ptr(), n, vocab, max_pos, hidden, scale, _DTYPES[dtype])
 
     def embed_grad_workspace(self, n, hidden):
-        return _workspace_bytes('fw_embed_grad_workspace', n, hidden)
+        return _workspace_bytes('fw_embed_grad_workspace', int(n), int(hidden))
 
     def embed_grad(self, dout, ids, dembed, scale=1.0, padding_idx=-1, accumulate=False, ws=None):
         """dembed[v] = (dembed[v] if accumulate) + scale * sum of dout[i] over ids[i] == v != padding_idx, summed in
         fp32 in the order of i. With ids = positions and scale 1 it is the position table's gradient."""
-        _check(dembed.dtype in _DTYPES, 'dembed must be fp16, bf16 or fp32')
-        _check_typed(dembed, dembed, 'dembed')
-        _check_typed(dout, dembed, 'dout')
-        n = ids.numel()
-        _check_ints(ids, n, dembed, 'ids')
+        dtype, dev, n = dembed.dtype, dembed.get_device(), ids.numel()
+        _check(dtype in _DTYPES, 'dembed must be fp16, bf16 or fp32')
+        _check_typed(dembed, dtype, dev, 'dembed')
+        _check_typed(dout, dtype, dev, 'dout')
+        _check_ints(ids, n, dev, 'ids')
         _check(dembed.dim() == 2 and dembed.numel() > 0, 'dembed must be [vocab, hidden]')
         vocab, hidden = dembed.shape
         _check(dout.numel() == n * hidden, 'embed_grad: dout must be [n, hidden]')
-        with _On(dembed.device):
-            ws = _workspace(ws, self.embed_grad_workspace(n, hidden), dembed.device)
-            _lib.call('fw_embed_grad', _ptr(dout), _ptr(ids), _ptr(dembed), n, vocab, hidden, float(scale),
-                      int(padding_idx), int(bool(accumulate)), _DTYPES[dembed.dtype], _ptr(ws), ws.numel(), _stream())
+        ws = _workspace(ws, self.embed_grad_workspace(n, hidden), dev)
+        _call_on(dev, 'fw_embed_grad', dout.data_ptr(), ids.data_ptr(), dembed.data_ptr(), n, vocab, hidden, scale,
+                 padding_idx, 1 if accumulate else 0, _DTYPES[dtype], _address(ws), _size(ws))
 
     @staticmethod
-    def _rows(t, like, rows, heads, name):
-        """[rows, heads, 64] of like's type, strided over rows and heads, as a C descriptor."""
-        if not (t.is_cuda and t.dtype == like.dtype and t.device == like.device and t.dim() == 3
-                and t.shape == (rows, heads, HEAD_DIM) and (t.stride(2) == 1 or t.numel() == 0)):
-            raise RuntimeError(f'{name} must be CUDA {str(like.dtype)[6:]} [{rows}, {heads}, {HEAD_DIM}] on '
-                               f'{like.device}, its last dimension contiguous')
+    def _rows(t, dtype, dev, shape, name):
+        """[rows, heads, 64] of this type, strided over rows and heads, as a C descriptor."""
+        if (t.dtype is not dtype or t.get_device() != dev or t.shape != shape
+                or (t.stride(2) != 1 and t.numel() > 0)):
+            raise RuntimeError(f'{name} must be CUDA {str(dtype)[6:]} [{shape[0]}, {shape[1]}, {shape[2]}] on '
+                               f'cuda:{dev}, its last dimension contiguous')
+        token, head, _ = t.stride()
         # a dimension of one element has no stride of its own
-        head = t.stride(1) if heads > 1 else HEAD_DIM
-        return _lib.Rows(t.data_ptr(), t.stride(0) if rows > 1 else heads * head, head)
+        if shape[1] <= 1:
+            head = HEAD_DIM
+        return _lib.Rows(t.data_ptr(), token if shape[0] > 1 else shape[1] * head, head)
 
     def _check_prompt(self, q, k, v, cu_q, cu_k):
-        _check(q.dtype in (torch.float16, torch.bfloat16), 'q must be fp16 or bf16')
+        _check(q.dtype in _HALF_TYPES, 'q must be fp16 or bf16')
         _check(q.dim() == 3 and k.dim() == 3, 'q and k must be [rows, heads, 64]')
-        (rows_q, heads), (rows_k, kv_heads) = q.shape[:2], k.shape[:2]
+        rows_q, heads, _ = q.shape
+        rows_k, kv_heads, _ = k.shape
         _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, 'heads must be a multiple of kv_heads')
-        seqs = max(cu_q.numel() - 1, 0)
-        _check_ints(cu_q, seqs + 1, q, 'cu_q')
-        _check_ints(cu_k, seqs + 1, q, 'cu_k')
-        return rows_q, rows_k, heads, kv_heads, seqs
+        dev, seqs = q.get_device(), max(cu_q.numel() - 1, 0)
+        _check_ints(cu_q, seqs + 1, dev, 'cu_q')
+        _check_ints(cu_k, seqs + 1, dev, 'cu_k')
+        return dev, (rows_q, heads, HEAD_DIM), (rows_k, kv_heads, HEAD_DIM), seqs
 
     def prompt_attention_workspace(self, rows_q, rows_k, seqs, heads, kv_heads):
-        return _workspace_bytes('fw_prompt_attention_workspace', rows_q, rows_k, seqs, heads, kv_heads)
+        return _workspace_bytes('fw_prompt_attention_workspace', int(rows_q), int(rows_k), int(seqs), int(heads),
+                                int(kv_heads))
 
     def prompt_attention(self, q, k, v, out, cu_q, cu_k, scale, causal=True, lse=None, ws=None):
         """Attention over packed sequences: q, out [rows_q, heads, 64], k, v [rows_k, kv_heads, 64] (fp16 or bf16, rows
         and heads strided); sequence b has the rows cu_q[b]:cu_q[b + 1] and cu_k[b]:cu_k[b + 1] (int64). causal: the
         last query sees the last key. lse: fp32 [heads, rows_q] or None."""
-        rows_q, rows_k, heads, kv_heads, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
-        rq, ro = self._rows(q, q, rows_q, heads, 'q'), self._rows(out, q, rows_q, heads, 'out')
-        rk, rv = self._rows(k, q, rows_k, kv_heads, 'k'), self._rows(v, q, rows_k, kv_heads, 'v')
+        dev, like_q, like_k, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
+        dtype, ref = q.dtype, ctypes.byref
+        rq, ro = self._rows(q, dtype, dev, like_q, 'q'), self._rows(out, dtype, dev, like_q, 'out')
+        rk, rv = self._rows(k, dtype, dev, like_k, 'k'), self._rows(v, dtype, dev, like_k, 'v')
+        rows_q, heads, rows_k, kv_heads = like_q[0], like_q[1], like_k[0], like_k[1]
         if lse is not None:
-            self._check_rows(lse, heads * rows_q, q, 'lse')
-        with _On(q.device):
-            ws = _workspace(ws, self.prompt_attention_workspace(rows_q, rows_k, seqs, heads, kv_heads), q.device)
-            _lib.call('fw_prompt_attention', ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), ctypes.byref(ro),
-                      _ptr(lse), _ptr(cu_q), _ptr(cu_k), seqs, rows_q, rows_k, heads, kv_heads, float(scale),
-                      int(bool(causal)), _DTYPES[q.dtype], _ptr(ws), ws.numel(), _stream())
+            _check_fp32(lse, heads * rows_q, dev, 'lse')
+        ws = _workspace(ws, self.prompt_attention_workspace(rows_q, rows_k, seqs, heads, kv_heads), dev)
+        _call_on(dev, 'fw_prompt_attention', ref(rq), ref(rk), ref(rv), ref(ro), _address(lse), cu_q.data_ptr(),
+                 cu_k.data_ptr(), seqs, rows_q, rows_k, heads, kv_heads, scale, 1 if causal else 0, _DTYPES[dtype],
+                 _address(ws), _size(ws))
 
     def prompt_attention_grad_workspace(self, rows_q, rows_k, seqs, heads, kv_heads):
-        return _workspace_bytes('fw_prompt_attention_grad_workspace', rows_q, rows_k, seqs, heads, kv_heads)
+        return _workspace_bytes('fw_prompt_attention_grad_workspace', int(rows_q), int(rows_k), int(seqs), int(heads),
+                                int(kv_heads))
 
     def prompt_attention_grad(self, q, k, v, out, dout, lse, cu_q, cu_k, scale, dq, dk, dv, causal=True, ws=None):
         """Gradient of prompt_attention: dq like q, dk and dv like k and v, for dout, from the forward's out and lse."""
-        rows_q, rows_k, heads, kv_heads, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
-        rq, ro, rd, rdq = (self._rows(t, q, rows_q, heads, name)
+        dev, like_q, like_k, seqs = self._check_prompt(q, k, v, cu_q, cu_k)
+        dtype, ref = q.dtype, ctypes.byref
+        rq, ro, rd, rdq = (self._rows(t, dtype, dev, like_q, name)
                            for t, name in ((q, 'q'), (out, 'out'), (dout, 'dout'), (dq, 'dq')))
-        rk, rv, rdk, rdv = (self._rows(t, q, rows_k, kv_heads, name)
+        rk, rv, rdk, rdv = (self._rows(t, dtype, dev, like_k, name)
                             for t, name in ((k, 'k'), (v, 'v'), (dk, 'dk'), (dv, 'dv')))
-        self._check_rows(lse, heads * rows_q, q, 'lse')
-        ref = ctypes.byref
-        with _On(q.device):
-            ws = _workspace(ws, self.prompt_attention_grad_workspace(rows_q, rows_k, seqs, heads, kv_heads), q.device)
-            _lib.call('fw_prompt_attention_grad', ref(rq), ref(rk), ref(rv), ref(ro), ref(rd), _ptr(lse), _ptr(cu_q),
-                      _ptr(cu_k), seqs, rows_q, rows_k, heads, kv_heads, float(scale), int(bool(causal)),
-                      _DTYPES[q.dtype], ref(rdq), ref(rdk), ref(rdv), _ptr(ws), ws.numel(), _stream())
+        rows_q, heads, rows_k, kv_heads = like_q[0], like_q[1], like_k[0], like_k[1]
+        _check_fp32(lse, heads * rows_q, dev, 'lse')
+        ws = _workspace(ws, self.prompt_attention_grad_workspace(rows_q, rows_k, seqs, heads, kv_heads), dev)
+        _call_on(dev, 'fw_prompt_attention_grad', ref(rq), ref(rk), ref(rv), ref(ro), ref(rd), lse.data_ptr(),
+                 cu_q.data_ptr(), cu_k.data_ptr(), seqs, rows_q, rows_k, heads, kv_heads, scale, 1 if causal else 0,
+                 _DTYPES[dtype], ref(rdq), ref(rdk), ref(rdv), _address(ws), _size(ws))
 
     def _check_loss(self, h, w, targets):
-        _check(h.dtype in (torch.float16, torch.bfloat16), 'h must be fp16 or bf16')
-        _check_typed(h, h, 'h')
-        _check_typed(w, h, 'w')
+        dtype, dev = h.dtype, h.get_device()
+        _check(dtype in _HALF_TYPES, 'h must be fp16 or bf16')
+        _check_typed(h, dtype, dev, 'h')
+        _check_typed(w, dtype, dev, 'w')
         _check(h.dim() == 2 and w.dim() == 2 and w.size(1) == h.size(1) and w.size(0) > 0 and w.size(1) > 0,
                'h must be [n, hidden], w [vocab, hidden]')
-        _check_ints(targets, h.size(0), h, 'targets')
-        return h.size(0), w.size(0), h.size(1)
+        _check_ints(targets, h.size(0), dev, 'targets')
+        return dev, h.size(0), w.size(0), h.size(1)
 
     def lm_head_loss_workspace(self, n, vocab):
-        return _workspace_bytes('fw_lm_head_loss_workspace', n, vocab)
+        return _workspace_bytes('fw_lm_head_loss_workspace', int(n), int(vocab))
 
     def lm_head_loss(self, h, w, targets, loss, lse, ignore_index=-100, ws=None):
         """loss[i] = lse[i] - h[i] . w[targets[i]] (0 where targets[i] == ignore_index), lse[i] = log sum_v
         exp(h[i] . w[v]), both fp32 [n]; h, w fp16 or bf16. The logits are never stored."""
-        n, vocab, hidden = self._check_loss(h, w, targets)
-        for t, name in ((loss, 'loss'), (lse, 'lse')):
-            self._check_rows(t, n, h, name)
-        with _On(h.device):
-            ws = _workspace(ws, self.lm_head_loss_workspace(n, vocab), h.device)
-            _lib.call('fw_lm_head_loss', _ptr(h), _ptr(w), _ptr(targets), _ptr(loss), _ptr(lse), n, vocab, hidden,
-                      int(ignore_index), _DTYPES[h.dtype], _ptr(ws), ws.numel(), _stream())
-
-    @staticmethod
-    def _check_rows(t, n, like, name):
-        if not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == n
-                and t.device == like.device):
-            raise RuntimeError(f'{name} must be contiguous CUDA fp32 [{n}] on {like.device}')
+        dev, n, vocab, hidden = self._check_loss(h, w, targets)
+        _check_fp32(loss, n, dev, 'loss')
+        _check_fp32(lse, n, dev, 'lse')
+        ws = _workspace(ws, self.lm_head_loss_workspace(n, vocab), dev)
+        _call_on(dev, 'fw_lm_head_loss', h.data_ptr(), w.data_ptr(), targets.data_ptr(), loss.data_ptr(),
+                 lse.data_ptr(), n, vocab, hidden, ignore_index, _DTYPES[h.dtype], _address(ws), _size(ws))
 
     def lm_head_loss_grad_workspace(self, n, vocab, hidden):
-        return _workspace_bytes('fw_lm_head_loss_grad_workspace', n, vocab, hidden)
+        return _workspace_bytes('fw_lm_head_loss_grad_workspace', int(n), int(vocab), int(hidden))
 
     def lm_head_loss_grad(self, h, w, targets, lse, g, dh, dw, ignore_index=-100, accumulate=False, ws=None):
         """Gradient of sum_i g[i] loss[i] of lm_head_loss: dh like h, dw like w (either may be None); accumulate adds
         to dw. lse is lm_head_loss's, g fp32 [n]."""
-        n, vocab, hidden = self._check_loss(h, w, targets)
-        for t, name in ((lse, 'lse'), (g, 'g')):
-            self._check_rows(t, n, h, name)
+        dev, n, vocab, hidden = self._check_loss(h, w, targets)
+        _check_fp32(lse, n, dev, 'lse')
+        _check_fp32(g, n, dev, 'g')
         for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
             if t is not None:
-                _check_typed(t, like, name)
+                _check_typed(t, h.dtype, dev, name)
                 _check(t.shape == like.shape, 'dh must be shaped like h, dw like w')
         _check(dh is not None or dw is not None, 'at least one of dh and dw is required')
-        with _On(h.device):
-            ws = _workspace(ws, self.lm_head_loss_grad_workspace(n, vocab, hidden), h.device)
-            _lib.call('fw_lm_head_loss_grad', _ptr(h), _ptr(w), _ptr(targets), _ptr(lse), _ptr(g), _ptr(dh), _ptr(dw),
-                      n, vocab, hidden, int(ignore_index), int(bool(accumulate)), _DTYPES[h.dtype], _ptr(ws),
-                      ws.numel(), _stream())
+        ws = _workspace(ws, self.lm_head_loss_grad_workspace(n, vocab, hidden), dev)
+        _call_on(dev, 'fw_lm_head_loss_grad', h.data_ptr(), w.data_ptr(), targets.data_ptr(), lse.data_ptr(),
+                 g.data_ptr(), _address(dh), _address(dw), n, vocab, hidden, ignore_index, 1 if accumulate else 0,
+                 _DTYPES[h.dtype], _address(ws), _size(ws))
 
     def decoder_step(self, desc, steps=1):
         _lib.call('fw_decoder_step', ctypes.byref(desc), int(steps), _stream())
