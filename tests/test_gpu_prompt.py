@@ -125,35 +125,37 @@ def test_prompt_attention_layouts(ext):
 
 
 @pytest.mark.parametrize('tokens', [True, False])
-def test_prompt_attention_neighbours_and_tails(ext, tokens):
+@pytest.mark.parametrize('behind', [2, 40])
+def test_prompt_attention_neighbours_and_tails(ext, tokens, behind):
     """Rows before the first and behind the last sequence hold NaN and stay as they are; a neighbour's NaN and
-    infinities reach no other sequence."""
+    infinities reach no other sequence: the others' bits are those of a call of the same sizes without any. (How many
+    rows there are chooses between the kernels, so sizes are kept alike.)"""
     lk = [130, 61, 200]
     lq = [1, 1, 1] if tokens else lk
     q, k, v = _make(lq, lk, 4, 2, 'bf16', fused=False)
-    cq, ck = _cu(lq), _cu(lk)
-    want, lse = torch.empty_like(q), torch.empty(4, sum(lq), device='cuda')
-    ext.prompt_attention(q, k, v, want, cq, ck, 0.2, lse=lse)
+    cq, ck = _cu(lq) + 5, _cu(lk) + 5
 
     def padded(x, fill):
-        return torch.cat([torch.full_like(x[:5], fill).expand(5, -1, -1) if x.size(0) >= 5 else
-                          torch.full((5, *x.shape[1:]), fill, dtype=x.dtype, device='cuda'), x,
-                          torch.full((40, *x.shape[1:]), fill, dtype=x.dtype, device='cuda')])
+        return torch.cat([torch.full((n, *x.shape[1:]), fill, dtype=x.dtype, device='cuda') if n else x
+                          for n in (5, 0, behind)])
+
+    want, lse = torch.empty_like(padded(q, 0.0)), torch.empty(4, sum(lq) + 5 + behind, device='cuda')
+    ext.prompt_attention(padded(q, 0.0), padded(k, 0.0), padded(v, 0.0), want, cq, ck, 0.2, lse=lse)
+    end = 5 + sum(lq)
+    _check(q, k, v, want[5:end], lse[:, 5:end], lq, lk, 0.2, True)
 
     nan = float('nan')
     q2, k2, v2 = padded(q, nan), padded(k, nan), padded(v, nan)
-    a, b = int(ck[1]) + 5, int(ck[2]) + 5
+    a, b = int(ck[1]), int(ck[2])
     k2[a:b], v2[a:b] = nan, float('inf')  # the whole middle sequence
     out = torch.full_like(q2, 7.0)
     lse2 = torch.full((4, q2.size(0)), 7.0, device='cuda')
-    ext.prompt_attention(q2, k2, v2, out, cq + 5, ck + 5, 0.2, lse=lse2)
-    end = 5 + sum(lq)
+    ext.prompt_attention(q2, k2, v2, out, cq, ck, 0.2, lse=lse2)
     assert bool((out[:5] == 7).all() and (out[end:] == 7).all() and (lse2[:, :5] == 7).all() and (lse2[:, end:] == 7).all())
     for i in (0, 2):
         rows = slice(int(cq[i]), int(cq[i + 1]))
-        moved = slice(rows.start + 5, rows.stop + 5)
-        assert torch.equal(out[moved], want[rows]) and torch.equal(lse2[:, moved], lse[:, rows])
-    assert bool(out[int(cq[1]) + 5:int(cq[2]) + 5].isnan().all())
+        assert torch.equal(out[rows], want[rows]) and torch.equal(lse2[:, rows], lse[:, rows])
+    assert bool(out[int(cq[1]):int(cq[2])].isnan().all())
     assert ext.device_error() == 0
 
 
