@@ -291,19 +291,22 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
           }
           tc_fence_after();
           const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + 128 * part;
+          if (row0 < a.n) {  // else none of this warp's rows is one
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) {
-            uint32_t r[16];
-            tc_ld16(d + c, r);
-            tc_wait_ld();
+            for (int c = 0; c < 128; c += 16) {
+              uint32_t r[16];
+              tc_ld16(d + c, r);
+              tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) z[c + j] = kb0 == 0 ? __uint_as_float(r[j]) : z[c + j] + __uint_as_float(r[j]);
+              for (int j = 0; j < 16; ++j) z[c + j] = kb0 == 0 ? __uint_as_float(r[j]) : z[c + j] + __uint_as_float(r[j]);
+            }
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(drained + 8 * buf);
         }
         if (failed) break;
+        if (row0 >= a.n) continue;
         if (c0 + 128 > a.width) {  // columns behind the vocabulary count as -inf
 #pragma unroll
           for (int j = 0; j < 128; ++j)
@@ -344,8 +347,9 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
       const bool wide = kKind == kGrads && x.dh;  // fp32 rows of 32 columns, else 16-bit rows of 64
       const bool direct = kKind == kGrads && !x.dh && a.accumulate;
       const float f = kKind == kGrads && !x.dh ? *a.gmax / a.dz_scale : 1.f;
+      const int rows = kKind == kDz || wide ? a.n : a.width;
 #pragma unroll 1
-      for (int c = 0; c < kCols; c += 32) {
+      for (int c = 0; c < (row0 < rows ? kCols : 0); c += 32) {
         uint32_t r[32];
         tc_load32(d + c, r);
         tc_wait_ld();
@@ -409,8 +413,7 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
           __syncwarp();
           // rows and columns behind the end of a partly covered box are not written
           const int at = wide ? col : col - 32;
-          const int rows = kKind == kDz || wide ? a.n : a.width, cols = kKind == kDz ? a.width : a.hidden;
-          if (lane == 0 && row0 < rows && at < cols) {
+          if (lane == 0 && at < (kKind == kDz ? a.width : a.hidden)) {
             if (!wide)
               tma_store_2d(&tmOut, out, at, row0);
             else if (a.first_piece)
