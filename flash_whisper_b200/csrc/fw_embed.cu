@@ -304,8 +304,10 @@ __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const T* __restr
   __shared__ uint32_t s_key[kMaxChunk + 2], s_row[kMaxChunk];  // keys with one neighbour on each side
   __shared__ __align__(8) uint64_t s_bar[kMaxChunk / kBulkRows];
   const int tid = threadIdx.x;
-  if (VEC > 1 && tid < kMaxChunk / kBulkRows) mbar_init(&s_bar[tid], 1);
-  if (VEC > 1 && tid == 0) mbar_fence_init();
+  if (VEC > 1 && tid < kMaxChunk / kBulkRows) {
+    mbar_init(&s_bar[tid], 1);
+    mbar_fence_init();
+  }
   pdl_wait();
   pdl_trigger();
   const int c0 = blockIdx.x * p.chunk, len = min(p.chunk, p.n - c0);
@@ -377,21 +379,20 @@ __global__ void __launch_bounds__(32 * kMergeWarps) embed_merge_kernel(T* __rest
   constexpr int kCols = 32 * VEC * (kMergeWarps / kMergeParts);
   const unsigned slices = (p.hidden + kCols - 1) / kCols;
   for (unsigned item = blockIdx.x; item < listed * slices; item += gridDim.x) {
-  const int c = p.crossing[1 + item / slices];
-  const int col0 = item % slices * kCols;
-  const uint32_t key = p.keys[(c + 1) * p.chunk - 1];
-  int more = 0;  // chunks behind this one that begin inside the run
-  while (true) {
-    const int64_t at = static_cast<int64_t>(c + 1 + more + threadIdx.x) * p.chunk;
-    const int hit = __syncthreads_count(at < p.n && p.keys[at] == key);
-    more += hit;
-    if (hit < static_cast<int>(blockDim.x)) break;
-  }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slice = warp / kMergeParts, part = warp % kMergeParts;
-  const int m0 = static_cast<int>(static_cast<int64_t>(more) * part / kMergeParts);
-  const int m1 = static_cast<int>(static_cast<int64_t>(more) * (part + 1) / kMergeParts);
-  {
+    const int c = p.crossing[1 + item / slices];
+    const int col0 = item % slices * kCols;
+    const uint32_t key = p.keys[(c + 1) * p.chunk - 1];
+    int more = 0;  // chunks behind this one that begin inside the run
+    while (true) {
+      const int64_t at = static_cast<int64_t>(c + 1 + more + threadIdx.x) * p.chunk;
+      const int hit = __syncthreads_count(at < p.n && p.keys[at] == key);
+      more += hit;
+      if (hit < static_cast<int>(blockDim.x)) break;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slice = warp / kMergeParts, part = warp % kMergeParts;
+    const int m0 = static_cast<int>(static_cast<int64_t>(more) * part / kMergeParts);
+    const int m1 = static_cast<int>(static_cast<int64_t>(more) * (part + 1) / kMergeParts);
     const int col = col0 + (slice * 32 + lane) * VEC;
     float acc[VEC];
 #pragma unroll
@@ -427,7 +428,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps) embed_merge_kernel(T* __rest
       write_row<T, VEC>(p, dembed, key, col, acc);
     }
     __syncthreads();
-  }
   }
 }
 

@@ -383,7 +383,8 @@ int fw_encoder_forward(const fw_encoder_t* e, fw_stream_t stream);
  * (and FW_F32 for the embedding); sums are held in fp32 and rounded once.
  * A *_workspace call writes the bytes of 16-byte aligned device scratch that the operator needs for
  * these sizes (it depends on nothing else). The scratch needs no initial value, keeps nothing between
- * calls, and must not be shared by calls that overlap on the GPU.
+ * calls, and must not be shared by calls that overlap on the GPU (nor by two graphs that may run at the
+ * same time). Outputs and scratch must not overlap inputs or one another.
  * ---------------------------------------------------------------------------------------- */
 
 /* out[i] = T(scale * embed[ids[i]] + pos_embed[positions[i]]), i < n; rows of `hidden` elements of type
