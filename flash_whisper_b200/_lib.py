@@ -165,8 +165,7 @@ def lib():
 
 def call(name, *args):
     """Calls fw_<name> and raises RuntimeError with the library's message on a non-zero status."""
-    fn = getattr(lib(), name)
-    rc = fn(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != FW_OK:
         msg = lib().fw_last_error_string().decode(errors='replace')
         raise RuntimeError(msg or f'{name} failed with status {rc}')

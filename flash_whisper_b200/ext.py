@@ -95,12 +95,10 @@ def _size(ws):
 
 def _call_on(dev, name, *args):
     """Calls fw_<name> on device `dev`, whichever is current, and its current stream."""
-    stream = torch._C._cuda_getCurrentRawStream(dev)
-    if torch.cuda.current_device() == dev:
-        _lib.call(name, *args, stream)
-    else:
+    if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, stream)
+            return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 class Ext:
@@ -331,17 +329,19 @@ class Ext:
         _check_ints(ids, n, dev, 'ids')
         _check(embed.dim() == 2 and embed.numel() > 0, 'embed must be [vocab, hidden]')
         vocab, hidden = embed.shape
-        _check((pos_embed is None) == (positions is None), 'pos_embed and positions must be given together')
-        max_pos = 0
-        if pos_embed is not None:
+        max_pos = pos_at = positions_at = 0
+        if pos_embed is not None and positions is not None:
             _check_typed(pos_embed, dtype, dev, 'pos_embed')
             _check_ints(positions, n, dev, 'positions')
-            _check(pos_embed.dim() == 2 and pos_embed.size(1) == hidden and pos_embed.numel() > 0,
-                   'pos_embed must be [max_pos, hidden]')
             max_pos = pos_embed.size(0)
+            _check(pos_embed.dim() == 2 and max_pos > 0 and pos_embed.size(1) == hidden,
+                   'pos_embed must be [max_pos, hidden]')
+            pos_at, positions_at = pos_embed.data_ptr(), positions.data_ptr()
+        else:
+            _check(pos_embed is positions, 'pos_embed and positions must be given together')
         _check(out.numel() == n * hidden, 'embed_scaled: out must be [n, hidden]')
-        _call_on(dev, 'fw_embed_scaled', embed.data_ptr(), _address(pos_embed), ids.data_ptr(), _address(positions),
-                 out.data_ptr(), n, vocab, max_pos, hidden, scale, _DTYPES[dtype])
+        _call_on(dev, 'fw_embed_scaled', embed.data_ptr(), pos_at, ids.data_ptr(), positions_at, out.data_ptr(), n,
+                 vocab, max_pos, hidden, scale, _DTYPES[dtype])
 
     def embed_grad_workspace(self, n, hidden):
         return _workspace_bytes('fw_embed_grad_workspace', int(n), int(hidden))
