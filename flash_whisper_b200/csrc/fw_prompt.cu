@@ -1,17 +1,18 @@
 // Attention over whole prompts: packed sequences of different lengths, causal or not, grouped heads, any number of
-// queries per sequence (a whole prompt, a chunk behind a kept prefix, a single token), and its gradient.
+// queries per sequence (a whole prompt, a chunk behind a kept prefix, a single token).
 //
 //   s_ij = scale q_i . k_j for the keys j that query i sees: j < lk, and with `causal` j <= i + lk - lq (the last query
 //   sees the last key)        lse_i = log sum_j exp s_ij        o_i = sum_j exp(s_ij - lse_i) v_j
 // A query that sees no key has o = 0 and lse = -inf.
 //
-// Forward (prompt_attn_kernel): a CTA takes 128 query rows of one sequence and one key head. The rows of a tile are (token, head of the group) pairs, tokens major, so that one read of K and V serves the whole group and a
-// single token of a grouped model still fills several rows. S = Q K^T and O += P V run on tcgen05 with S, P and O in
-// tensor memory (P, 16 bits, is the A operand from there: it never passes through shared memory); one thread owns a
-// row, so maximum and sum need no exchange. S has a buffer of its own besides P: the next block's Q K^T runs while the
-// current block's exponentials are computed, and the two tiles alternate on the tensor core. The running maximum moves
-// only when a row exceeds it by 2^8, so O is seldom rescaled. What bounds it: 128 x 128 exponentials take twice as
-// long as the tile's two products of depth 64.
+// prompt_attn_kernel: a CTA takes 128 query rows of one sequence and one key head. The rows of a tile are (token, head of
+// the group) pairs, tokens major, so that one read of K and V serves the whole group and a single token of a grouped model
+// still fills several rows. S = Q K^T and O += P V run on tcgen05 with S, P and O in tensor memory (P, 16 bits, is the A
+// operand from there: it never passes through shared memory); one thread owns a row, so maximum and sum need no exchange.
+// S has a buffer of its own besides P: the next block's Q K^T runs while the current block's exponentials are computed,
+// and two CTAs share an SM, so that the softmax of one fills the waits of the other. The running maximum moves only when
+// a row exceeds it by 2^8, so O is seldom rescaled. What bounds it: 128 x 128 exponentials take twice as long as the
+// tile's two products of depth 64; an eighth of them run on the FMA pipe instead.
 // Few rows (serving): the keys are split over several CTAs, whose partial results prompt_join_kernel joins; where there
 // are so few that tiles would be empty, prompt_few_kernel takes the place of the tensor core.
 #include "fw_prompt.cuh"
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
     tmem_relinquish();
   }
   if (warp == 5) {
-    const Item it = find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens,
+    const Item it = find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, a.few,
                               blockIdx.x / a.splits / a.kv_heads, lane);
     if (lane == 0) {
       s_item = it;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
           for (int i = 0; i < 16; ++i) {
             float2 e = fma2(make_float2(__uint_as_float(x[h][2 * i]), __uint_as_float(x[h][2 * i + 1])),
                             make_float2(c, c), make_float2(off, off));
-            // every eighth pair on the FMA pipe (267 us with every fourth, 263 with none, 248); a masked score gives 2^-126 there
+            // every eighth pair on the FMA pipe (267 us with every fourth, 263 with none, 248)
             e = i % 8 == 7 ? ex2_fma(e) : make_float2(ex2(e.x), ex2(e.y));
             acc[i & 1] = add2(acc[i & 1], e);
             p[i] = Type16<T>::pack(e.x, e.y);
@@ -301,51 +302,50 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   if (warp == 4) tmem_dealloc(tmem, 256);
+  pdl_wait();  // what follows this kernel follows prompt_few_kernel, beside which it may run
 }
 
 // Few query rows per sequence and key head (single tokens while decoding): a tile of 128 rows would be nearly empty, and
 // the work is to read K and V once. One CTA per (sequence, key head, split of the keys), every warp on its own: lane =
 // key for the scores (32 keys at a time, fp32 dot products with q broadcast from shared memory), lane = two of the 64
 // columns for P V, with the running maxima and sums of kR rows in registers; the warps' results are joined in shared
-// memory. Sequences with more rows than kR take several turns. V's loads are issued before the scores are computed.
+// memory. Sequences with more rows than kR take several turns, those with more than a.few are left to the tiles. V's loads
+// are issued before the scores are computed.
+// kR goes by the sequence's own rows: 1, 2, 4 or 8.
 constexpr int kFewWarps = 4;
+struct FewRows {
+  const void *q, *k, *v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+};
+template <int kR>
+struct FewShared {
+  alignas(16) float q[kR][64];
+  float top[kFewWarps][kR], sum[kFewWarps][kR];
+  float2 o[kFewWarps][kR][32];
+};
 template <typename T, int kR>
-__global__ void __launch_bounds__(32 * kFewWarps) prompt_few_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                                    const T* __restrict__ v, int64_t q_token,
-                                                                    int64_t q_head, int64_t k_token, int64_t k_head,
-                                                                    int64_t v_token, int64_t v_head, PromptArgs a) {
-  __shared__ __align__(16) float s_q[kR][64];
-  __shared__ float s_top[kFewWarps][kR], s_sum[kFewWarps][kR];
-  __shared__ float2 s_o[kFewWarps][kR][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % a.splits;
-  const int kvh = blockIdx.x / a.splits % a.kv_heads;
-  const int seq = blockIdx.x / a.splits / a.kv_heads;
-  const int64_t q0 = a.cu_q[seq], q1 = a.cu_q[seq + 1], k0 = a.cu_k[seq], k1 = a.cu_k[seq + 1];
-  if (q0 < 0 || q1 < q0 || q1 > a.rows_q || k0 < 0 || k1 < k0 || k1 > a.rows_k) {
-    if (threadIdx.x == 0) prompt_flag(FW_DEVERR_BAD_INDEX);
-    return;
-  }
-  const int lq = static_cast<int>(q1 - q0), lk = static_cast<int>(k1 - k0), shift = lk - lq;
+__device__ __forceinline__ void few_rows(const FewRows& x, const PromptArgs& a, FewShared<kR>& sh, int64_t q0, int lq, int64_t k0,
+                                         int lk, int kvh, int split) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, shift = lk - lq;
   const int rows = lq * a.group;  // (token, head of the group), tokens major
   // this warp's keys
   const int parts = a.splits * kFewWarps, part = split * kFewWarps + warp;
   const int tiles = (lk + 31) / 32;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts);
-  const T* kb = k + k0 * k_token + kvh * k_head;
-  const T* vb = v + k0 * v_token + kvh * v_head + 2 * lane;
+  const T* kb = static_cast<const T*>(x.k) + k0 * x.k_token + kvh * x.k_head;
+  const T* vb = static_cast<const T*>(x.v) + k0 * x.v_token + kvh * x.v_head + 2 * lane;
 
   for (int r0 = 0; r0 < rows; r0 += kR) {
     __syncthreads();
     for (int i = threadIdx.x; i < kR * 32; i += 32 * kFewWarps) {
       const int r = r0 + i / 32, d = i % 32 * 2;
-      float2 x = make_float2(0.f, 0.f);
+      float2 f = make_float2(0.f, 0.f);
       if (r < rows)
-        x = Type16<T>::unpack(*reinterpret_cast<const uint32_t*>(q + (q0 + r / a.group) * q_token +
-                                                                 (kvh * a.group + r % a.group) * q_head + d));
-      s_q[i / 32][d] = x.x;
-      s_q[i / 32][d + 1] = x.y;
+        f = Type16<T>::unpack(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(x.q) + (q0 + r / a.group) * x.q_token +
+                                                                 (kvh * a.group + r % a.group) * x.q_head + d));
+      sh.q[i / 32][d] = f.x;
+      sh.q[i / 32][d + 1] = f.y;
     }
     __syncthreads();
     float top[kR], sum[kR];
@@ -368,11 +368,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) prompt_few_kernel(const T* __r
       for (int i = 0; i < 8; ++i) kw[i] = make_uint4(0u, 0u, 0u, 0u);
       if (key < lk) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) kw[i] = reinterpret_cast<const uint4*>(kb + key * k_token)[i];
+        for (int i = 0; i < 8; ++i) kw[i] = reinterpret_cast<const uint4*>(kb + key * x.k_token)[i];
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        vw[j] = j < n ? *reinterpret_cast<const uint32_t*>(vb + static_cast<int64_t>(32 * t + j) * v_token) : 0u;
+        vw[j] = j < n ? *reinterpret_cast<const uint32_t*>(vb + static_cast<int64_t>(32 * t + j) * x.v_token) : 0u;
       float s[kR];
 #pragma unroll
       for (int r = 0; r < kR; ++r) s[r] = 0.f;
@@ -381,11 +381,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) prompt_few_kernel(const T* __r
         const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float2 x = Type16<T>::unpack(w[2 * h]), y = Type16<T>::unpack(w[2 * h + 1]);
+          const float2 e = Type16<T>::unpack(w[2 * h]), g = Type16<T>::unpack(w[2 * h + 1]);
 #pragma unroll
           for (int r = 0; r < kR; ++r) {
-            const float4 f = *reinterpret_cast<const float4*>(&s_q[r][8 * i + 4 * h]);
-            s[r] = fmaf(x.x, f.x, fmaf(x.y, f.y, fmaf(y.x, f.z, fmaf(y.y, f.w, s[r]))));
+            const float4 f = *reinterpret_cast<const float4*>(&sh.q[r][8 * i + 4 * h]);
+            s[r] = fmaf(e.x, f.x, fmaf(e.y, f.y, fmaf(g.x, f.z, fmaf(g.y, f.w, s[r]))));
           }
         }
       }
@@ -403,55 +403,79 @@ __global__ void __launch_bounds__(32 * kFewWarps) prompt_few_kernel(const T* __r
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float2 x = Type16<T>::unpack(vw[j]);
+        const float2 e = Type16<T>::unpack(vw[j]);
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
           const float p = __shfl_sync(0xffffffffu, s[r], j);
-          o[r].x = fmaf(p, x.x, o[r].x);
-          o[r].y = fmaf(p, x.y, o[r].y);
+          o[r].x = fmaf(p, e.x, o[r].x);
+          o[r].y = fmaf(p, e.y, o[r].y);
         }
       }
     }
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       const float l = warp_sum(sum[r]);
-      s_o[warp][r][lane] = o[r];
+      sh.o[warp][r][lane] = o[r];
       if (lane == 0) {
-        s_top[warp][r] = top[r];
-        s_sum[warp][r] = l;
+        sh.top[warp][r] = top[r];
+        sh.sum[warp][r] = l;
       }
     }
     __syncthreads();
     for (int r = warp; r < kR && r0 + r < rows; r += kFewWarps) {
       float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, s_top[w][r]);
+      for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, sh.top[w][r]);
       const float off = m == -INFINITY ? 0.f : -m;
       float l = 0.f;
-      float2 x = make_float2(0.f, 0.f);
+      float2 e = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) {
-        const float f = ex2(s_top[w][r] + off);
-        const float2 y = s_o[w][r][lane];
-        l = fmaf(s_sum[w][r], f, l);
-        x = make_float2(fmaf(y.x, f, x.x), fmaf(y.y, f, x.y));
+        const float f = ex2(sh.top[w][r] + off);
+        const float2 y = sh.o[w][r][lane];
+        l = fmaf(sh.sum[w][r], f, l);
+        e = make_float2(fmaf(y.x, f, e.x), fmaf(y.y, f, e.y));
       }
       const bool none = l == 0.f;
       const float inv = none ? 0.f : 1.f / l;
-      x = none ? make_float2(0.f, 0.f) : make_float2(x.x * inv, x.y * inv);
+      e = none ? make_float2(0.f, 0.f) : make_float2(e.x * inv, e.y * inv);
       const float lse = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       const int64_t row = q0 + (r0 + r) / a.group;
       const int head = kvh * a.group + (r0 + r) % a.group;
       if (a.splits > 1) {
-        reinterpret_cast<float2*>(a.part_o + ((split * a.rows_q + row) * a.heads + head) * 64)[lane] = x;
+        reinterpret_cast<float2*>(a.part_o + ((split * a.rows_q + row) * a.heads + head) * 64)[lane] = e;
         if (lane == 0) a.part_lse[(static_cast<int64_t>(split) * a.heads + head) * a.rows_q + row] = lse;
       } else {
         reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + row * a.out_token + head * a.out_head)[lane] =
-            Type16<T>::pack(x.x, x.y);
+            Type16<T>::pack(e.x, e.y);
         if (lane == 0 && a.lse != nullptr) a.lse[head * a.rows_q + row] = lse;
       }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kFewWarps, 3) prompt_few_kernel(const FewRows x, const PromptArgs a) {
+  __shared__ FewShared<8> sh;
+  const int split = blockIdx.x % a.splits;
+  const int kvh = blockIdx.x / a.splits % a.kv_heads;
+  const int seq = blockIdx.x / a.splits / a.kv_heads;
+  pdl_trigger();
+  const int64_t q0 = a.cu_q[seq], q1 = a.cu_q[seq + 1], k0 = a.cu_k[seq], k1 = a.cu_k[seq + 1];
+  if (q0 < 0 || q1 < q0 || q1 > a.rows_q || k0 < 0 || k1 < k0 || k1 > a.rows_k) {
+    if (threadIdx.x == 0) prompt_flag(FW_DEVERR_BAD_INDEX);
+    return;
+  }
+  if (q1 - q0 > a.few) return;
+  const int lq = static_cast<int>(q1 - q0), lk = static_cast<int>(k1 - k0), rows = lq * a.group;
+  if (rows <= 1)
+    few_rows<T>(x, a, reinterpret_cast<FewShared<1>&>(sh), q0, lq, k0, lk, kvh, split);
+  else if (rows <= 2)
+    few_rows<T>(x, a, reinterpret_cast<FewShared<2>&>(sh), q0, lq, k0, lk, kvh, split);
+  else if (rows <= 4)
+    few_rows<T>(x, a, reinterpret_cast<FewShared<4>&>(sh), q0, lq, k0, lk, kvh, split);
+  else
+    few_rows<T>(x, a, sh, q0, lq, k0, lk, kvh, split);
 }
 
 // Joins the key splits of a (row, head), one warp each: o = sum_s exp(lse_s - lse) o_s.
@@ -500,7 +524,10 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 // Host side
 // From sizes only (the offsets are on the device): rows of an average sequence and key head, and whether they are few
 // enough for prompt_few_kernel. One token for 8 clips over caches up to 1500, 20 heads: 22 us in tiles of 128 rows, 8 us.
-constexpr int kFewRows = 8;
+// The average says nothing of the longest: a sequence of more than kFewMost rows, a prompt that came in among single
+// tokens, goes to the tiles all the same, in a launch beside the other (none where rows_q leaves no room for one). 127
+// single tokens and a prompt of 600, keys up to 1500, 20 heads: 4580 us with all of it in prompt_few_kernel, 131 us.
+constexpr int kFewRows = 8, kFewMost = 64;
 static int64_t average_rows(int64_t rows_q, int seqs, int group) {
   return seqs > 0 ? (rows_q + seqs - 1) / seqs * group : 0;
 }
@@ -520,12 +547,23 @@ static int prompt_splits(int64_t rows_q, int64_t rows_k, int seqs, int kv_heads,
   return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
-template <typename T, int kR>
-static cudaError_t launch_few(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v, const PromptArgs& a,
-                              cudaStream_t s) {
-  return launch(prompt_few_kernel<T, kR>, dim3(static_cast<unsigned>(a.seqs) * a.kv_heads * a.splits),
-                dim3(32 * kFewWarps), 0, s, false, static_cast<const T*>(q.ptr), static_cast<const T*>(k.ptr),
-                static_cast<const T*>(v.ptr), q.token, q.head, k.token, k.head, v.token, v.head, a);
+template <typename T>
+static int run_tiles(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v, const PromptArgs& a, int64_t items,
+                     cudaStream_t s) {
+  FW_REQUIRE(items < (int64_t(1) << 31), FW_ERR_SHAPE, "prompt_attention: too many query tiles");
+  CUtensorMap tq, tk, tv;
+  // no keys at all: any valid address serves, nothing is read through it
+  const bool keys = a.rows_k > 0;
+  int rc = make_rows_map(&tq, Type16<T>::kMap, q.ptr, a.rows_q, a.heads, q.token, q.head, a.group, a.tokens);
+  if (!rc) rc = keys ? make_rows_map(&tk, Type16<T>::kMap, k.ptr, a.rows_k, a.kv_heads, k.token, k.head, 1, kRows) : FW_OK;
+  if (!rc) rc = keys ? make_rows_map(&tv, Type16<T>::kMap, v.ptr, a.rows_k, a.kv_heads, v.token, v.head, 1, kRows) : FW_OK;
+  if (rc) return rc;
+  auto kern = prompt_attn_kernel<T>;
+  cudaError_t e = ensure_smem(kern, kFwdSmem);
+  if (e == cudaSuccess)
+    e = launch(kern, dim3(static_cast<unsigned>(items)), dim3(kFwdThreads), kFwdSmem, s, a.few > 0, tq, keys ? tk : tq,
+               keys ? tv : tq, a);
+  return launch_status(e, "prompt_attention");
 }
 
 template <typename T>
@@ -535,34 +573,16 @@ static int run_prompt(const fw_rows_t& q, const fw_rows_t& k, const fw_rows_t& v
   const int64_t rows = average_rows(a.rows_q, a.seqs, a.group);
   const int64_t few = static_cast<int64_t>(a.seqs) * a.kv_heads * a.splits;
   if (rows <= kFewRows && few < (int64_t(1) << 31)) {
-    if (rows <= 1)
-      e = launch_few<T, 1>(q, k, v, a, s);
-    else if (rows <= 2)
-      e = launch_few<T, 2>(q, k, v, a, s);
-    else if (rows <= 4)
-      e = launch_few<T, 4>(q, k, v, a, s);
-    else
-      e = launch_few<T, 8>(q, k, v, a, s);
+    a.few = kFewMost / a.group;
+    const FewRows x{q.ptr, k.ptr, v.ptr, q.token, q.head, k.token, k.head, v.token, v.head};
+    e = launch(prompt_few_kernel<T>, dim3(static_cast<unsigned>(few)), dim3(32 * kFewWarps), 0, s, false, x, a);
     rc = launch_status(e, "prompt_attention few rows");
-    if (rc || a.splits == 1) return rc;
-    e = launch(prompt_join_kernel<T>, dim3(static_cast<unsigned>((a.rows_q * a.heads + 3) / 4)), dim3(128), 0, s, true, a);
-    return launch_status(e, "prompt_attention join");
+    if (rc) return rc;
   }
-  CUtensorMap tq, tk, tv;
-  const int64_t items = (a.rows_q / a.tokens + a.seqs) * a.kv_heads * a.splits;
-  FW_REQUIRE(items < (int64_t(1) << 31), FW_ERR_SHAPE, "prompt_attention: too many query tiles");
-  // no keys at all: any valid address serves, nothing is read through it
-  const bool keys = a.rows_k > 0;
-  rc = make_rows_map(&tq, Type16<T>::kMap, q.ptr, a.rows_q, a.heads, q.token, q.head, a.group, a.tokens);
-  if (!rc) rc = keys ? make_rows_map(&tk, Type16<T>::kMap, k.ptr, a.rows_k, a.kv_heads, k.token, k.head, 1, kRows) : FW_OK;
-  if (!rc) rc = keys ? make_rows_map(&tv, Type16<T>::kMap, v.ptr, a.rows_k, a.kv_heads, v.token, v.head, 1, kRows) : FW_OK;
-  if (rc) return rc;
-  auto kern = prompt_attn_kernel<T>;
-  e = ensure_smem(kern, kFwdSmem);
-  if (e == cudaSuccess)
-    e = launch(kern, dim3(static_cast<unsigned>(items)), dim3(kFwdThreads), kFwdSmem, s, false, tq, keys ? tk : tq,
-               keys ? tv : tq, a);
-  rc = launch_status(e, "prompt_attention");
+  // sequences of more than a.few queries: rows_q / (few + 1) at most
+  const int64_t longer = a.rows_q / (a.few + 1) < a.seqs ? a.rows_q / (a.few + 1) : a.seqs;
+  const int64_t items = longer == 0 ? 0 : (a.rows_q / a.tokens + longer) * a.kv_heads * a.splits;
+  if (items > 0) rc = run_tiles<T>(q, k, v, a, items, s);
   if (rc || a.splits == 1) return rc;
   e = launch(prompt_join_kernel<T>, dim3(static_cast<unsigned>((a.rows_q * a.heads + 3) / 4)), dim3(128), 0, s, true, a);
   return launch_status(e, "prompt_attention join");

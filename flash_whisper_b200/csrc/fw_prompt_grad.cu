@@ -331,10 +331,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         x.end = index >= g.all_items;
         if (x.end) break;
         x.keys = index < g.key_items;
-        const int64_t in = x.keys ? index : index - g.key_items;
-        x.kvh = static_cast<int>(in % a.kv_heads);
-        const Item it = x.keys ? find_item(a.cu_k, a.cu_q, a.rows_k, a.rows_q, a.seqs, kRows, in / a.kv_heads, lane)
-                               : find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, in / a.kv_heads, lane);
+        const int in = static_cast<int>(x.keys ? index : index - g.key_items);
+        x.kvh = in % a.kv_heads;
+        const Item it = x.keys ? find_item(a.cu_k, a.cu_q, a.rows_k, a.rows_q, a.seqs, kRows, 0, in / a.kv_heads, lane)
+                               : find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, 0, in / a.kv_heads, lane);
         if (it.tile < 0) continue;
         x.seq = it.seq;
         x.q0 = x.keys ? it.k0 : it.q0, x.lq = x.keys ? it.lk : it.lq;  // find_item was asked with q and k swapped

@@ -85,10 +85,10 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 
 // 2^x of two numbers on the FMA pipe, for kernels that the special-function unit (16 results a cycle and SM) bounds.
 // x = n + f with n the nearest integer, 2^f by a polynomial of degree 5 fitted for the least relative error on
-// [-1/2, 1/2] (7.5e-8), times 2^n. x at most 127; below -126 the result is 2^-126; NaN stays.
+// [-1/2, 1/2] (7.5e-8), times 2^n. x at most 127; below -126.5 the result is 0; NaN stays.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
   const float magic = 12582912.f;  // 1.5 * 2^23: the sum's last bits are the nearest integer
   const float2 t = add2(x, make_float2(magic, magic));
   const float2 f = fma2(add2(t, make_float2(-magic, -magic)), make_float2(-1.f, -1.f), x);
@@ -98,6 +98,7 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
   p = fma2(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
   p = fma2(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
   p = fma2(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  // n = -127 gives the bits of 0
   const float2 s = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
                                __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
   return mul2(p, s);

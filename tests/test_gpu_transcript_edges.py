@@ -207,3 +207,36 @@ def test_loss_forward_with_every_target_and_width(ext):
         want_loss, want_lse, _, _ = _want(h, w, targets)
         err = _logit_error(h, w)
         assert bool(((lse.double() - want_lse).abs() <= err).all() and ((loss.double() - want_loss).abs() <= 2 * err).all())
+
+
+@pytest.mark.parametrize('singles,longer,group', [(127, [600], 1), (70, [65, 64, 300], 1), (300, [17, 16, 900], 4),
+                                                  (8, [64], 1)])
+@pytest.mark.parametrize('kv_heads', [2, 20])
+def test_prompt_attention_prompts_among_single_tokens(ext, singles, longer, group, kv_heads):
+    """Few rows on average, some sequences with many: on both sides of the length that tiles take over."""
+    lq = [1] * singles
+    for i, n in enumerate(longer):
+        lq.insert((37 * i + 5) % singles, n)
+    lk = [n + (53 * i) % 400 for i, n in enumerate(lq)]
+    q, k, v = _make(lq, lk, kv_heads * group, kv_heads, 'fp16', fused=False)
+    out, lse = torch.full_like(q, float('nan')), torch.full((q.size(1), q.size(0)), float('nan'), device='cuda')
+    ext.prompt_attention(q, k, v, out, _cu(lq), _cu(lk), 0.15, lse=lse)
+    assert ext.device_error() == 0
+    if kv_heads == 20:  # every head is alike: check four of them
+        heads = [0, 7 * group, 13 * group + group - 1, 20 * group - 1]
+        keep = [h // group for h in heads]
+        q, k, v, out, lse = q[:, heads], k[:, keep], v[:, keep], out[:, heads], lse[heads]
+    _check(q, k, v, out, lse, lq, lk, 0.15, True)
+
+
+def test_prompt_attention_masked_keys_of_any_finite_size(ext):
+    """What a later key holds reaches no earlier query, however large it is."""
+    q, k, v = _make([200], [200], 2, 2, 'bf16', fused=False)
+    outs = []
+    for fill in (1.0, torch.finfo(torch.bfloat16).max):
+        v[100:] = fill
+        k[100:] = fill if fill == 1.0 else 1e30
+        out = torch.empty_like(q)
+        ext.prompt_attention(q, k, v, out, _cu([200]), _cu([200]), 0.125)
+        outs.append(out)
+    assert torch.equal(outs[0][:100], outs[1][:100])
