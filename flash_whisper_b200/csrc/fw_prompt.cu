@@ -306,12 +306,14 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
 }
 
 // Few query rows per sequence and key head (single tokens while decoding): a tile of 128 rows would be nearly empty, and
-// the work is to read K and V once. One CTA per (sequence, key head, split of the keys), every warp on its own: lane =
-// key for the scores (32 keys at a time, fp32 dot products with q broadcast from shared memory), lane = two of the 64
-// columns for P V, with the running maxima and sums of kR rows in registers; the warps' results are joined in shared
-// memory. Sequences with more rows than kR take several turns, those with more than a.few are left to the tiles. V's loads
-// are issued before the scores are computed.
-// kR goes by the sequence's own rows: 1, 2, 4 or 8.
+// the work is to read K and V once. One CTA per (sequence, key head, split of the keys), every warp on its own, 32 keys at
+// a time: eight lanes read a key's 128 bytes, four keys a load, so a lane has 8 of the 64 dimensions of every fourth key.
+// 128 tokens over caches up to 1500, 20 heads, 498 MB: 87 us, 5.7 TB/s (with a key a lane each load touched 32 lines and
+// the L1 bound it: 122 us; with 5 CTAs an SM 93). Scores are fp32 dot
+// products, reduced over the eight lanes so that each lane ends with one key's; in P V the four groups of lanes sum their
+// own keys until the end. V's loads are issued before the scores are computed. The warps' results are joined in shared
+// memory. kR is 2 if the sequence has more than one row; those of more than two take several turns, those of more than
+// a.few queries are left to the tiles.
 constexpr int kFewWarps = 4;
 struct FewRows {
   const void *q, *k, *v;
@@ -333,8 +335,9 @@ __device__ __forceinline__ void few_rows(const FewRows& x, const PromptArgs& a, 
   const int tiles = (lk + 31) / 32;
   const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts);
-  const T* kb = static_cast<const T*>(x.k) + k0 * x.k_token + kvh * x.k_head;
-  const T* vb = static_cast<const T*>(x.v) + k0 * x.v_token + kvh * x.v_head + 2 * lane;
+  const int group = lane >> 3, at = lane & 7;  // of lanes, place in it
+  const T* kb = static_cast<const T*>(x.k) + k0 * x.k_token + kvh * x.k_head + 8 * at;
+  const T* vb = static_cast<const T*>(x.v) + k0 * x.v_token + kvh * x.v_head + 8 * at;
 
   for (int r0 = 0; r0 < rows; r0 += kR) {
     __syncthreads();
@@ -348,74 +351,89 @@ __device__ __forceinline__ void few_rows(const FewRows& x, const PromptArgs& a, 
       sh.q[i / 32][d + 1] = f.y;
     }
     __syncthreads();
-    float top[kR], sum[kR];
-    float2 o[kR];
+    float top[kR], sum[kR], o[kR][8];
     int limit[kR];
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       top[r] = -INFINITY;
       sum[r] = 0.f;
-      o[r] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[r][i] = 0.f;
       const int token = (r0 + r) / a.group;
       limit[r] = r0 + r >= rows ? -1 : a.causal ? min(lk - 1, token + shift) : lk - 1;
     }
     for (int t = t0; t < t1; ++t) {
-      const int key = 32 * t + lane;
-      const int n = min(32, lk - 32 * t);
-      uint4 kw[8];
-      uint32_t vw[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) kw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (key < lk) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) kw[i] = reinterpret_cast<const uint4*>(kb + key * x.k_token)[i];
-      }
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        vw[j] = j < n ? *reinterpret_cast<const uint32_t*>(vb + static_cast<int64_t>(32 * t + j) * x.v_token) : 0u;
-      float s[kR];
-#pragma unroll
-      for (int r = 0; r < kR; ++r) s[r] = 0.f;
+      uint4 kw[8], vw[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 e = Type16<T>::unpack(w[2 * h]), g = Type16<T>::unpack(w[2 * h + 1]);
-#pragma unroll
-          for (int r = 0; r < kR; ++r) {
-            const float4 f = *reinterpret_cast<const float4*>(&sh.q[r][8 * i + 4 * h]);
-            s[r] = fmaf(e.x, f.x, fmaf(e.y, f.y, fmaf(g.x, f.z, fmaf(g.y, f.w, s[r]))));
-          }
-        }
+        const int key = 32 * t + 4 * i + group;
+        kw[i] = key < lk ? *reinterpret_cast<const uint4*>(kb + key * x.k_token) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = 32 * t + 4 * i + group;
+        vw[i] = key < lk ? *reinterpret_cast<const uint4*>(vb + key * x.v_token) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      const int key = 32 * t + 4 * at + group;  // whose score this lane ends with
+      float p[kR];
+#pragma unroll
       for (int r = 0; r < kR; ++r) {
-        const float z = key <= limit[r] ? s[r] * a.scale_log2 : -INFINITY;
+        const float4 qa = *reinterpret_cast<const float4*>(&sh.q[r][8 * at]);
+        const float4 qb = *reinterpret_cast<const float4*>(&sh.q[r][8 * at + 4]);
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 e = Type16<T>::unpack(kw[i].x), f = Type16<T>::unpack(kw[i].y);
+          const float2 g = Type16<T>::unpack(kw[i].z), h = Type16<T>::unpack(kw[i].w);
+          s[i] = fmaf(e.x, qa.x, fmaf(e.y, qa.y, fmaf(f.x, qa.z, f.y * qa.w))) +
+                 fmaf(g.x, qb.x, fmaf(g.y, qb.y, fmaf(h.x, qb.z, h.y * qb.w)));
+        }
+        // sums over the eight lanes; each step halves the keys that a lane keeps
+#pragma unroll
+        for (int d = 4; d > 0; d >>= 1) {
+          const bool upper = (at & d) != 0;
+#pragma unroll
+          for (int i = 0; i < d; ++i) {
+            const float give = upper ? s[i] : s[i + d], keep = upper ? s[i + d] : s[i];
+            s[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+          }
+        }
+        const float z = key <= limit[r] ? s[0] * a.scale_log2 : -INFINITY;
         const float m = fmaxf(top[r], warp_max(z));
         const float off = m == -INFINITY ? 0.f : -m;
         const float f = ex2(top[r] + off);
-        const float p = ex2(z + off);
-        sum[r] = fmaf(sum[r], f, p);  // this lane's keys
-        o[r] = make_float2(o[r].x * f, o[r].y * f);
+        p[r] = ex2(z + off);
+        sum[r] = fmaf(sum[r], f, p[r]);  // this lane's keys
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[r][i] *= f;
         top[r] = m;
-        s[r] = p;
       }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float2 e = Type16<T>::unpack(vw[j]);
+      for (int i = 0; i < 8; ++i) {
+        const float2 e = Type16<T>::unpack(vw[i].x), f = Type16<T>::unpack(vw[i].y);
+        const float2 g = Type16<T>::unpack(vw[i].z), h = Type16<T>::unpack(vw[i].w);
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
-          const float p = __shfl_sync(0xffffffffu, s[r], j);
-          o[r].x = fmaf(p, e.x, o[r].x);
-          o[r].y = fmaf(p, e.y, o[r].y);
+          const float w = __shfl_sync(0xffffffffu, p[r], 8 * group + i);
+          o[r][0] = fmaf(w, e.x, o[r][0]), o[r][1] = fmaf(w, e.y, o[r][1]);
+          o[r][2] = fmaf(w, f.x, o[r][2]), o[r][3] = fmaf(w, f.y, o[r][3]);
+          o[r][4] = fmaf(w, g.x, o[r][4]), o[r][5] = fmaf(w, g.y, o[r][5]);
+          o[r][6] = fmaf(w, h.x, o[r][6]), o[r][7] = fmaf(w, h.y, o[r][7]);
         }
       }
     }
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
       const float l = warp_sum(sum[r]);
-      sh.o[warp][r][lane] = o[r];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // over the four groups
+        o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], 8);
+        o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], 16);
+      }
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sh.o[warp][r][4 * at + i] = make_float2(o[r][2 * i], o[r][2 * i + 1]);
+      }
       if (lane == 0) {
         sh.top[warp][r] = top[r];
         sh.sum[warp][r] = l;
@@ -455,8 +473,8 @@ __device__ __forceinline__ void few_rows(const FewRows& x, const PromptArgs& a, 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kFewWarps, 3) prompt_few_kernel(const FewRows x, const PromptArgs a) {
-  __shared__ FewShared<8> sh;
+__global__ void __launch_bounds__(32 * kFewWarps, 4) prompt_few_kernel(const FewRows x, const PromptArgs a) {
+  __shared__ FewShared<2> sh;
   const int split = blockIdx.x % a.splits;
   const int kvh = blockIdx.x / a.splits % a.kv_heads;
   const int seq = blockIdx.x / a.splits / a.kv_heads;
@@ -470,10 +488,6 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3) prompt_few_kernel(const Few
   const int lq = static_cast<int>(q1 - q0), lk = static_cast<int>(k1 - k0), rows = lq * a.group;
   if (rows <= 1)
     few_rows<T>(x, a, reinterpret_cast<FewShared<1>&>(sh), q0, lq, k0, lk, kvh, split);
-  else if (rows <= 2)
-    few_rows<T>(x, a, reinterpret_cast<FewShared<2>&>(sh), q0, lq, k0, lk, kvh, split);
-  else if (rows <= 4)
-    few_rows<T>(x, a, reinterpret_cast<FewShared<4>&>(sh), q0, lq, k0, lk, kvh, split);
   else
     few_rows<T>(x, a, sh, q0, lq, k0, lk, kvh, split);
 }
@@ -523,11 +537,12 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
 // ------------------------------------------------------------------------------------------------
 // Host side
 // From sizes only (the offsets are on the device): rows of an average sequence and key head, and whether they are few
-// enough for prompt_few_kernel. One token for 8 clips over caches up to 1500, 20 heads: 22 us in tiles of 128 rows, 8 us.
+// enough for prompt_few_kernel. 64 sequences over caches up to 1500, 20 heads: one row 53 us, two 63, four 95; tiles of
+// 128 rows 62 for any of them.
 // The average says nothing of the longest: a sequence of more than kFewMost rows, a prompt that came in among single
-// tokens, goes to the tiles all the same, in a launch beside the other (none where rows_q leaves no room for one). 127
-// single tokens and a prompt of 600, keys up to 1500, 20 heads: 4580 us with all of it in prompt_few_kernel, 131 us.
-constexpr int kFewRows = 8, kFewMost = 64;
+// tokens, goes to the tiles all the same, in a launch beside the other (none where rows_q leaves no room for one). 600
+// single tokens and a prompt of 600, keys up to 1500, 20 heads, 2.3 GB: 365 us, with all of it in tiles 541.
+constexpr int kFewRows = 2, kFewMost = 32;
 static int64_t average_rows(int64_t rows_q, int seqs, int group) {
   return seqs > 0 ? (rows_q + seqs - 1) / seqs * group : 0;
 }

@@ -210,7 +210,7 @@ def test_loss_forward_with_every_target_and_width(ext):
 
 
 @pytest.mark.parametrize('singles,longer,group', [(127, [600], 1), (70, [65, 64, 300], 1), (300, [17, 16, 900], 4),
-                                                  (8, [64], 1)])
+                                                  (8, [64], 1), (400, [300, 33, 32], 1), (90, [3, 2, 16, 17], 2)])
 @pytest.mark.parametrize('kv_heads', [2, 20])
 def test_prompt_attention_prompts_among_single_tokens(ext, singles, longer, group, kv_heads):
     """Few rows on average, some sequences with many: on both sides of the length that tiles take over."""
@@ -240,3 +240,17 @@ def test_prompt_attention_masked_keys_of_any_finite_size(ext):
         ext.prompt_attention(q, k, v, out, _cu([200]), _cu([200]), 0.125)
         outs.append(out)
     assert torch.equal(outs[0][:100], outs[1][:100])
+
+
+@pytest.mark.parametrize('lq,group', [([2] * 5 + [0], 1), ([3] * 5, 1), ([1] * 6, 2), ([1] * 6, 3), ([1, 0, 5, 0, 1, 1], 1),
+                                      ([2, 2, 3, 2, 1], 1), ([1], 1), ([1, 1], 1)])
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_prompt_attention_of_one_to_three_rows(ext, lq, group, dtype):
+    """On both sides of two rows; keys from none to several tiles of 32, cut anywhere by the warps and splits."""
+    for base in (0, 1, 31, 33, 260, 1500):
+        lk = [base + 13 * i if base else max(n - 1, 0) for i, n in enumerate(lq)]
+        q, k, v = _make(lq, lk, 3 * group, 3, dtype, fused=False)
+        out, lse = torch.full_like(q, float('nan')), torch.full((q.size(1), q.size(0)), float('nan'), device='cuda')
+        ext.prompt_attention(q, k, v, out, _cu(lq), _cu(lk), 0.2, lse=lse)
+        assert ext.device_error() == 0
+        _check(q, k, v, out, lse, lq, lk, 0.2, True)
