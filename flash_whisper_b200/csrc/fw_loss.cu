@@ -4,9 +4,9 @@
 //   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_i,t(i)        (0 where the target is ignored)
 //   dz_iv = g_i (exp(z_iv - lse_i) - [v = t(i)])        dh = dz W        dW = dz^T h
 //
-// All products run in one persistent tcgen05 kernel on CTA pairs (cta_group::2, 256 x 256 tiles: each CTA stages
+// All products but those of at most 64 rows (loss_few_kernel) run in one persistent tcgen05 kernel on CTA pairs (cta_group::2, 256 x 256 tiles: each CTA stages
 // 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a third less L2 traffic than two 128 x 256
-// tiles), fed by TMA through a 6-stage ring, with the accumulators of two tiles in tensor memory so that the
+// tiles), fed by TMA through a ring of 4 to 6 stages, with the accumulators of two tiles in tensor memory so that the
 // epilogue of one runs under the MMAs of the next.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
@@ -440,7 +440,178 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// Joins the (max, sum) of all half tiles of a row, both in powers of two, so that the differences of maxima are exact:
+// Forward of at most 64 rows (one transcript, the drafts of a few tokens): bound by reading W once, where a tile of 256 rows
+// would keep the tensor core busy for as long with rows that do not exist. The operands change places: 128 rows of W are
+// the M of a product, the kN >= n rows of h its N. One CTA an SM takes an equal, contiguous share of the vocabulary in
+// equal tiles of `box` <= 128 rows, each k block of which is one copy. 27 rows of 1280, vocabulary of 51866: 31 us with the
+// join, W at 4.9 TB/s (copies of 32 rows 37; in tiles of 256 rows 42; 64 rows 35, and 35 to 37 there). A thread owns a vocabulary row of each tile: it keeps maximum and sum of every row of h over its tiles by
+// itself, and the CTA joins its 128 threads once, at the end.
+constexpr int kFewRows = 64, kFewStages = 6, kFewThreads = 32 * 6;
+constexpr uint32_t few_stage(int rows) { return kHalfBytes + rows * 128; }
+constexpr int few_smem(int rows) { return kFewStages * few_stage(rows) + 1024; }
+
+template <typename T, int kN>
+__global__ void __launch_bounds__(kFewThreads, 1)
+    loss_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmH, LossArgs a, int share,
+                    int box) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kFewStages], empty_bar[kFewStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int s_target[kN];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  constexpr uint32_t kColumns = 2 * kN;
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmH);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_base_sh, kColumns);
+    tmem_relinquish();
+  }
+  for (int i = threadIdx.x; i < kN; i += kFewThreads) {
+    const int64_t t = i < a.n ? a.targets[i] : -1;
+    s_target[i] = t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem = tmem_base_sh;
+  const int v0 = blockIdx.x * share, v1 = min(a.vocab, v0 + share);
+  const int kbs = (a.hidden + kBK - 1) / kBK, segment = segment_of<T>(kbs);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int v = v0; v < v1 && ok; v += box) {
+        for (int kb = 0; kb < kbs; ++kb, ++it) {
+          const int s = it % kFewStages;
+          if (it >= kFewStages && !mbar_wait(&empty_bar[s], ((it / kFewStages) & 1u) ^ 1u)) {
+            loss_flag(FW_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + s * few_stage(kN);
+          mbar_arrive_expect_tx(&full_bar[s], (box + kN) * 128);  // of the tile's 128 rows the others are not used
+          tma_load_2d(dst, &tmW, &full_bar[s], kb * kBK, v);
+          tma_load_2d(dst + kHalfBytes, &tmH, &full_bar[s], kb * kBK, 0);
+        }
+      }
+    }
+  } else if (warp == 1) {  // the whole warp runs the loop, one lane issues
+    constexpr uint32_t idesc = make_idesc(128, kN, Type16<T>::kBf16, false, false);
+    int it = 0, local = 0;
+    bool ok = true;
+    for (int v = v0; v < v1 && ok; v += box) {
+      for (int kb0 = 0; kb0 < kbs && ok; kb0 += segment, ++local) {
+        const int buf = local & 1;
+        if (local >= 2) ok = mbar_wait_warp(&acc_empty[buf], ((local >> 1) & 1u) ^ 1u);
+        tc_fence_after();
+        for (int kb = kb0; kb < min(kbs, kb0 + segment) && ok; ++kb, ++it) {
+          const int s = it % kFewStages;
+          ok = mbar_wait_warp(&full_bar[s], (it / kFewStages) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = sw128_desc(base + s * few_stage(kN)), bd = sw128_desc(base + s * few_stage(kN) + kHalfBytes);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kBK / 16; ++kk)
+              tc_mma_f16(tmem + buf * kN, ad + 2 * kk, bd + 2 * kk, idesc, kb != kb0 || kk != 0 ? 1u : 0u);
+            tc_commit(&empty_bar[s]);
+          }
+          __syncwarp();
+        }
+        if (elect_one()) tc_commit(&acc_full[buf]);
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
+  } else {
+    const int q = warp & 3, mine = q * 32 + lane;  // this thread's vocabulary row of a tile
+    float top[kN], sum[kN];
+#pragma unroll
+    for (int c = 0; c < kN; ++c) top[c] = -INFINITY, sum[c] = 0.f;
+    int local = 0;
+    bool ok = true;
+    for (int v = v0; v < v1 && ok; v += box) {
+      float z[kN];
+      for (int kb0 = 0; kb0 < kbs; kb0 += segment, ++local) {
+        const int buf = local & 1;
+        ok = mbar_wait_warp(&acc_full[buf], (local >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kN; c += 16) {
+          uint32_t r[16];
+          tc_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kN + c, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) z[c + j] = kb0 == 0 ? __uint_as_float(r[j]) : z[c + j] + __uint_as_float(r[j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      }
+      if (!ok) break;
+      if (mine < box && v + mine < v1) {
+#pragma unroll
+        for (int c = 0; c < kN; ++c) {
+          if (s_target[c] == v + mine) a.target_logit[c] = z[c];
+          // maxima in powers of two, rounded once: the sum is relative to exactly this number
+          const float m = fmaxf(top[c], z[c] * kLog2e), off = m == -INFINITY ? 0.f : -m;
+          sum[c] = sum[c] * ex2(top[c] + off) + ex2(fmaf(z[c], kLog2e, off));
+          top[c] = m;
+        }
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
+    // All products are done, so the stages are free: [kN][128] maxima, then sums.
+    float* s_top = reinterpret_cast<float*>(smem);
+    float* s_sum = s_top + kN * 128;
+    if (ok) {
+#pragma unroll
+      for (int c = 0; c < kN; ++c) {
+        s_top[c * 128 + mine] = top[c];
+        s_sum[c * 128 + mine] = sum[c];
+      }
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int c = q; c < a.n && ok; c += 4) {
+      float t[4], m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        t[i] = s_top[c * 128 + 32 * i + lane];
+        m = fmaxf(m, t[i]);
+      }
+      m = warp_max(m);
+      const float off = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l = fmaf(s_sum[c * 128 + 32 * i + lane], ex2(t[i] + off), l);
+      l = warp_sum(l);
+      if (lane == 0) a.stats[static_cast<int64_t>(blockIdx.x) * a.n + c] = make_float2(m, l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kColumns);
+}
+
+// Joins the (max, sum) of all half tiles (shares) of a row, both in powers of two, so that the differences of maxima are exact:
 // 32 rows per CTA (lanes), the half tiles over its warps.
 constexpr int kCombineThreads = 1024;
 __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const float2* __restrict__ stats, int halves,
@@ -565,12 +736,18 @@ constexpr int64_t kDzBytes = int64_t(96) << 20;  // a piece's dz at most: it and
 
 struct LossLayout {
   int n_tiles;
+  int box, share;  // loss_few_kernel: vocabulary rows of a tile, of a CTA; 0 where it is not used
+  int parts;  // (max, sum) of a row
   int64_t total;
 };
 static LossLayout loss_layout(int n, int vocab) {
   LossLayout l;
   l.n_tiles = (vocab + kBN - 1) / kBN;
-  l.total = 2 * static_cast<int64_t>(l.n_tiles) * n * static_cast<int64_t>(sizeof(float2));
+  const int rows = up(vocab, 2 * kPairs) / (2 * kPairs), tiles = (rows + 127) / 128;  // of a CTA an SM
+  l.box = n > kFewRows ? 0 : rows < 32 ? 32 : (rows + tiles - 1) / tiles;
+  l.share = l.box * tiles;
+  l.parts = l.share > 0 ? (vocab + l.share - 1) / l.share : 2 * l.n_tiles;
+  l.total = static_cast<int64_t>(l.parts) * n * static_cast<int64_t>(sizeof(float2));
   return l;
 }
 
@@ -647,14 +824,24 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   return launch_status(e, "lm_head_loss");
 }
 
+template <typename T, int kN>
+static int launch_few(const CUtensorMap& tw, const void* h, const LossArgs& a, int share, int box,
+                      cudaStream_t s) {
+  CUtensorMap th;
+  int rc = make_map(&th, Type16<T>::kMap, h, a.hidden, a.n, a.hidden, kN);
+  if (rc) return rc;
+  auto kern = loss_few_kernel<T, kN>;
+  cudaError_t e = ensure_smem(kern, few_smem(kN));
+  if (e == cudaSuccess)
+    e = launch(kern, dim3((a.vocab + share - 1) / share), dim3(kFewThreads), few_smem(kN), s, false, tw, th, a, share, box);
+  return launch_status(e, "lm_head_loss");
+}
+
 template <typename T>
 static int run_loss(const void* h, const void* w, const int64_t* targets, float* loss, float* lse, int n, int vocab,
                     int hidden, int64_t ignore, void* ws, cudaStream_t s) {
   const LossLayout l = loss_layout(n, vocab);
   CUtensorMap ta, tb;
-  int rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
-  if (!rc) rc = make_map(&tb, Type16<T>::kMap, w, hidden, vocab, hidden, 128);
-  if (rc) return rc;
   LossArgs a{};
   a.n = n;
   a.hidden = hidden;
@@ -665,10 +852,17 @@ static int run_loss(const void* h, const void* w, const int64_t* targets, float*
   a.targets = targets;
   a.stats = static_cast<float2*>(ws);
   a.target_logit = loss;  // replaced by the loss when the halves are joined
-  rc = launch_gemm<kStats, T>(ta, tb, ta, tb, ta, ta, a, a.m_tiles * a.n_tiles, s, false);
+  int rc = make_map(&tb, Type16<T>::kMap, w, hidden, vocab, hidden, l.share > 0 ? l.box : 128);
+  if (rc) return rc;
+  if (l.share > 0) {
+    rc = n <= 32 ? launch_few<T, 32>(tb, h, a, l.share, l.box, s) : launch_few<T, kFewRows>(tb, h, a, l.share, l.box, s);
+  } else {
+    rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
+    if (!rc) rc = launch_gemm<kStats, T>(ta, tb, ta, tb, ta, ta, a, a.m_tiles * a.n_tiles, s, false);
+  }
   if (rc) return rc;
   cudaError_t e = launch(loss_combine_kernel, dim3((n + 31) / 32), dim3(kCombineThreads), 0, s, true,
-                         static_cast<const float2*>(a.stats), 2 * l.n_tiles, n, targets, ignore, vocab, loss, lse);
+                         static_cast<const float2*>(a.stats), l.parts, n, targets, ignore, vocab, loss, lse);
   return launch_status(e, "lm_head_loss combine");
 }
 

@@ -256,3 +256,38 @@ def test_loss_captured_and_on_another_stream(ext):
         ext.lm_head_loss_grad(h, w, targets, lse, g, dh2, dw2)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
+
+
+@pytest.mark.parametrize('n', [1, 16, 31, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize('vocab,hidden', [(1, 8), (33, 72), (129, 64), (4737, 136), (9600, 1280), (20001, 456)])
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_loss_of_few_rows(ext, n, vocab, hidden, dtype):
+    """Both sides of 32 and 64 rows; shares of the vocabulary from one row to several cut tiles."""
+    h, w, targets = _inputs(n, vocab, hidden, dtype)
+    targets[-1] = vocab - 1
+    need = ext.lm_head_loss_workspace(n, vocab)
+    room = torch.full((need + 512,), 77, dtype=torch.uint8, device='cuda')
+    loss, lse = (torch.full((n + 4,), 5.0, device='cuda') for _ in range(2))
+    ext.lm_head_loss(h, w, targets, loss[:n], lse[:n], ws=room[:need])
+    assert ext.device_error() == 0
+    want_loss, want_lse, _, _ = _want(h, w, targets)
+    err = _logit_error(h, w)
+    assert bool(((lse[:n].double() - want_lse).abs() <= err).all())
+    assert bool(((loss[:n].double() - want_loss).abs() <= 2 * err).all())
+    assert bool((room[need:] == 77).all()) and bool((loss[n:] == 5).all()) and bool((lse[n:] == 5).all())
+
+
+def test_loss_of_few_rows_with_rows_that_are_not_numbers(ext):
+    """A row of NaN reaches its own loss only; rows of W that are NaN or infinite reach every row's."""
+    h, w, targets = _inputs(20, 5000, 128, 'bf16')
+    targets.clamp_(min=0)
+    loss, lse = (torch.empty(20, device='cuda') for _ in range(2))
+    ext.lm_head_loss(h, w, targets, loss, lse)
+    h[3] = float('nan')
+    bad, bad_lse = (torch.empty(20, device='cuda') for _ in range(2))
+    ext.lm_head_loss(h, w, targets, bad, bad_lse)
+    rest = torch.arange(20, device='cuda') != 3
+    assert bool(bad[3].isnan()) and torch.equal(bad[rest], loss[rest]) and torch.equal(bad_lse[rest], lse[rest])
+    w[4999] = float('nan')
+    ext.lm_head_loss(h, w, targets, bad, bad_lse)
+    assert bool(bad_lse.isnan().all())
