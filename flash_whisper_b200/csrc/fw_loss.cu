@@ -4,10 +4,10 @@
 //   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_i,t(i)        (0 where the target is ignored)
 //   dz_iv = g_i (exp(z_iv - lse_i) - [v = t(i)])        dh = dz W        dW = dz^T h
 //
-// All products but those of at most 64 rows (loss_few_kernel) run in one persistent tcgen05 kernel on CTA pairs (cta_group::2, 256 x 256 tiles: each CTA stages
-// 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a third less L2 traffic than two 128 x 256
-// tiles), fed by TMA through a ring of 4 to 6 stages, with the accumulators of two tiles in tensor memory so that the
-// epilogue of one runs under the MMAs of the next.
+// All products but those of at most 64 rows (loss_few_kernel) run in one persistent tcgen05 kernel on CTA pairs
+// (cta_group::2, 256 x 256 tiles: each CTA stages 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a
+// third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 4 to 6 stages, with the accumulators of
+// two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
 //     row and half tile.
