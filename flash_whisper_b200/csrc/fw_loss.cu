@@ -6,7 +6,7 @@
 //
 // All products but those of at most 64 rows (loss_few_kernel) run in one persistent tcgen05 kernel on CTA pairs
 // (cta_group::2, 256 x 256 tiles: each CTA stages 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a
-// third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 4 to 6 stages, with the accumulators of
+// third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 5 or 6 stages, with the accumulators of
 // two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
@@ -36,7 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Kind { kStats, kDz, kGrads };  // what a launch computes
-constexpr int stages_of(int kind) { return kind == kStats ? 6 : kind == kDz ? 5 : 4; }
+constexpr int stages_of(int kind) { return kind == kGrads ? 5 : 6; }
 // Epilogue warps: twice as many where the products are short (dW of few rows) and the epilogue has little to compute.
 constexpr int epi_warps(int kind) { return kind == kGrads ? 16 : 8; }
 constexpr int threads_of(int kind) { return 32 * (2 + epi_warps(kind)); }
@@ -70,6 +70,7 @@ struct LossArgs {
   void* dw;                  // [vocab][hidden]
   const float* gmax;
   int first_piece, accumulate;
+  bool chunks;               // MN-major maps over [hidden / 64][rows][64]; hidden is a multiple of 64
 };
 
 struct Tile {
@@ -119,11 +120,14 @@ __device__ __forceinline__ Tile tile_at(const LossArgs& a, int t) {
   return x;
 }
 
-// A CTA's 128 rows of an operand for one k block. K-major: one box of 64 k x 128 rows. MN-major: two boxes of 64
-// rows (contiguous) x 64 k.
+// A CTA's 128 rows of an operand for one k block. K-major: one box of 64 k x 128 rows. MN-major: boxes of 64 rows
+// (contiguous) x 64 k, both as one copy where the map has chunks of 64 for its third dimension (dW of 211 rows, 8 copies a
+// k block and CTA pair: FIG).
 template <bool kMn>
-__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint32_t rbar, int row, int k) {
-  if (kMn) {
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint32_t rbar, int row, int k, bool chunks) {
+  if (kMn && chunks) {
+    tma_load_3d_pair(dst, map, rbar, 0, k, row >> 6);
+  } else if (kMn) {
     tma_load_2d_pair(dst, map, rbar, row, k);
     tma_load_2d_pair(dst + kHalfBytes / 2, map, rbar, row + 64, k);
   } else {
@@ -208,14 +212,14 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
           const int row_a = x.m0 + 128 * static_cast<int>(rank), row_b = x.n0 + 128 * static_cast<int>(rank);
           const int k = (x.kb0 + kb) * kBK;
           if (kKind != kGrads) {
-            load_half<false>(dst, &tmA, rbar, row_a, k);
-            load_half<false>(dst + kHalfBytes, &tmB, rbar, row_b, k);
+            load_half<false>(dst, &tmA, rbar, row_a, k, false);
+            load_half<false>(dst + kHalfBytes, &tmB, rbar, row_b, k, false);
           } else if (x.dh) {
-            load_half<false>(dst, &tmA, rbar, row_a, k);
-            load_half<true>(dst + kHalfBytes, &tmB, rbar, row_b, k);
+            load_half<false>(dst, &tmA, rbar, row_a, k, false);
+            load_half<true>(dst + kHalfBytes, &tmB, rbar, row_b, k, a.chunks);
           } else {
-            load_half<true>(dst, &tmA2, rbar, row_a, k);
-            load_half<true>(dst + kHalfBytes, &tmB2, rbar, row_b, k);
+            load_half<true>(dst, &tmA2, rbar, row_a, k, true);
+            load_half<true>(dst + kHalfBytes, &tmB2, rbar, row_b, k, a.chunks);
           }
         }
       }
@@ -794,6 +798,21 @@ static int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* ptr, i
   return FW_OK;
 }
 
+// The same rows as {64, outer, chunks of 64}: boxes of 64 x 64 x 2 chunks.
+static int make_chunk_map(CUtensorMap* m, CUtensorMapDataType type, const void* ptr, int64_t chunks, int64_t outer,
+                          int64_t ld) {
+  EncodeTiledFn enc = tensor_map_encode_fn();
+  if (!enc) return set_error(FW_ERR_LAUNCH, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(chunks)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, 128};
+  cuuint32_t box[3] = {64, 64, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FW_ERR_ARG, "lm_head_loss: tensor map encode failed (%d)", static_cast<int>(r));
+  return FW_OK;
+}
+
 // 3-D map over fp32 sums [splits][n][hidden]; boxes of 32 x 32.
 static int make_part_map(CUtensorMap* m, const void* ptr, int hidden, int n, int splits) {
   EncodeTiledFn enc = tensor_map_encode_fn();
@@ -885,15 +904,21 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
   int rc = launch_status(e, "lm_head_loss_grad scale");
   CUtensorMap ta, tb, ga, gb, ga2, gb2, tz, tw, tp;
   if (!rc) rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
-  if (!rc) rc = make_map(&gb2, Type16<T>::kMap, scaled, hidden, n, hidden, 64);
+  const bool chunks = hidden % 64 == 0;
+  if (!rc)
+    rc = chunks ? make_chunk_map(&gb2, Type16<T>::kMap, scaled, hidden / 64, n, hidden)
+                : make_map(&gb2, Type16<T>::kMap, scaled, hidden, n, hidden, 64);
   if (!rc) rc = make_part_map(&tp, part, hidden, n, l.splits);
   for (int p = 0; p < l.pieces && !rc; ++p) {
     const int v0 = p * l.width, width = vocab - v0 < l.width ? vocab - v0 : l.width;
     const T* wp = static_cast<const T*>(w) + static_cast<int64_t>(v0) * hidden;
     rc = make_map(&tb, Type16<T>::kMap, wp, hidden, width, hidden, 128);
     if (!rc) rc = make_map(&ga, Type16<T>::kMap, dz, width, n, l.width, 128);
-    if (!rc) rc = make_map(&gb, Type16<T>::kMap, wp, hidden, width, hidden, 64);
-    if (!rc) rc = make_map(&ga2, Type16<T>::kMap, dz, width, n, l.width, 64);
+    if (!rc)
+      rc = chunks ? make_chunk_map(&gb, Type16<T>::kMap, wp, hidden / 64, width, hidden)
+                  : make_map(&gb, Type16<T>::kMap, wp, hidden, width, hidden, 64);
+    // whole chunks: what dz holds behind `width` gives rows of dW that are not stored
+    if (!rc) rc = make_chunk_map(&ga2, Type16<T>::kMap, dz, (width + 63) / 64, n, l.width);
     if (!rc) rc = make_map(&tz, Type16<T>::kMap, dz, width, n, l.width, 32);
     if (!rc && dw != nullptr)
       rc = make_map(&tw, Type16<T>::kMap, static_cast<T*>(dw) + static_cast<int64_t>(v0) * hidden, hidden, width, hidden, 32);
@@ -924,6 +949,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     a.gmax = gmax;
     a.first_piece = p == 0;
     a.accumulate = accumulate;
+    a.chunks = chunks;
     rc = launch_gemm<kGrads, T>(ga, gb, ga2, gb2, tw, tp, a, (a.dh_m_tiles * a.splits + a.m_tiles) * a.n_tiles, s, true);
   }
   if (rc || dh == nullptr) return rc;
