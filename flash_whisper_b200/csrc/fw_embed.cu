@@ -1,7 +1,7 @@
 // Token embedding of whole (packed) transcripts and its gradient.
 //
 // Forward: out_i = T(scale E[id_i] + P[pos_i]), fp32 arithmetic, one rounding. One warp per row with 16-byte
-// accesses; bound by HBM.
+// accesses; bound by HBM (32749 rows of 1280 bf16, 168 MB: 33 us a call, 5.1 TB/s).
 //
 // Gradient: dE[v] = scale sum_{i: id_i = v} dout_i, the sum in fp32 in the order of i. Tokens repeat a lot (text
 // is close to a Zipf law), so the rows of one token are brought together by a stable sort instead of adding them
@@ -14,7 +14,9 @@
 //   3. embed_sum_kernel: equal chunks of the sorted list, so a frequent token costs no CTA more than a rare one; a
 //      run of equal ids inside a chunk is written at once, a run that crosses a chunk's end leaves fp32 partials.
 //   4. embed_merge_kernel: adds the partials of each crossing run in chunk order.
-// Bound by HBM (the gradient is written once, dout read once) and, for few tokens, by the launches' latency.
+// Bound by HBM (the gradient is written once, dout read once) and, for few tokens, by the sort's latency: 32749 tokens over
+// 51866 rows of 1280 (bf16, 217 MB) 67 us, 3.2 TB/s (sort 22 and zero rows 23 side by side, sums 29, crossing runs 12);
+// 3584 tokens (fp16, 142 MB) 37 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -294,8 +296,8 @@ constexpr int kBulkRows = 8;        // rows that share an mbarrier
 constexpr int kSumThreads = 128;
 
 // One CTA: a chunk of the sorted list, a slice of the columns. Whole 16-byte rows (VEC > 1) come by bulk copies, all of
-// the chunk's at once, which needs no registers for what is in flight (loads into registers, 4 a thread: 74 us for 32749
-// rows of 1280 and the rest of the call; this: see fw_embed_grad).
+// the chunk's at once, which needs no registers for what is in flight (loads into registers, 4 a thread: 74 us for the
+// call of 32749 rows of 1280, 67 so).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads) embed_sum_kernel(const T* __restrict__ dout, T* __restrict__ dembed,
                                                                 SumParams p, int slice) {

@@ -8,6 +8,9 @@
 // (cta_group::2, 256 x 256 tiles: each CTA stages 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a
 // third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 5 or 6 stages, with the accumulators of
 // two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
+// Measured (vocabulary 51866, hidden 1280, bf16; below the power cap): forward of 16381 rows 1340 us, 1.62 PFLOP/s, the
+// tensor pipe 95% active; gradient of 8189 rows 2684 us, 1.62 PFLOP/s with the logits formed again; of 211 rows (fp16)
+// 125 us, of which dW's 133 MB of stores and dh's 133 MB of loads take 40 at the memory's rate and overlap little.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
 //     row and half tile.
@@ -121,10 +124,11 @@ __device__ __forceinline__ Tile tile_at(const LossArgs& a, int t) {
 }
 
 // A CTA's 128 rows of an operand for one k block. K-major: one box of 64 k x 128 rows. MN-major: boxes of 64 rows
-// (contiguous) x 64 k, both as one copy where the map has chunks of 64 for its third dimension (dW of 211 rows, 8 copies a
-// k block and CTA pair: FIG).
+// (contiguous) x 64 k, both as one copy where the map has chunks of 64 for its third dimension (gradient of 8189 rows,
+// a copy a box: 2780 us, 2684).
 template <bool kMn>
-__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint32_t rbar, int row, int k, bool chunks) {
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint32_t rbar, int row, int k,
+                                          bool chunks) {
   if (kMn && chunks) {
     tma_load_3d_pair(dst, map, rbar, 0, k, row >> 6);
   } else if (kMn) {
@@ -262,8 +266,9 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
     }
   } else {
     // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns
-    // kCols ((w - 2) / 4) .. + kCols - 1. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128 bytes, 128-byte
-    // swizzle) to tensor stores: 16 bytes a thread straight to rows 2560 bytes apart took three times as long.
+    // kCols ((w - 2) / 4) .. + kCols - 1. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128
+    // bytes, 128-byte swizzle) to tensor stores: 16 bytes a thread straight to rows 2560 bytes apart took three times
+    // as long.
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t drained = cluster_map(&acc_empty[0], 0);
     constexpr int kCols = 2 * 4 * 128 / epi_warps(kKind);  // columns of a warp
@@ -448,8 +453,9 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
 // would keep the tensor core busy for as long with rows that do not exist. The operands change places: 128 rows of W are
 // the M of a product, the kN >= n rows of h its N. One CTA an SM takes an equal, contiguous share of the vocabulary in
 // equal tiles of `box` <= 128 rows, each k block of which is one copy. 27 rows of 1280, vocabulary of 51866: 31 us with the
-// join, W at 4.9 TB/s (copies of 32 rows 37; in tiles of 256 rows 42; 64 rows 35, and 35 to 37 there). A thread owns a vocabulary row of each tile: it keeps maximum and sum of every row of h over its tiles by
-// itself, and the CTA joins its 128 threads once, at the end.
+// join, W at 4.9 TB/s (copies of 32 rows 37; in tiles of 256 rows 42; 64 rows 35, and 35 to 37 there). A thread owns a
+// vocabulary row of each tile: it keeps maximum and sum of every row of h over its tiles by itself, and the CTA joins its
+// 128 threads once, at the end.
 constexpr int kFewRows = 64, kFewStages = 6, kFewThreads = 32 * 6;
 constexpr uint32_t few_stage(int rows) { return kHalfBytes + rows * 128; }
 constexpr int few_smem(int rows) { return kFewStages * few_stage(rows) + 1024; }
