@@ -9,8 +9,8 @@
 // third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 5 or 6 stages, with the accumulators of
 // two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
 // Measured (vocabulary 51866, hidden 1280, bf16; below the power cap): forward of 16381 rows 1340 us, 1.62 PFLOP/s, the
-// tensor pipe 95% active; gradient of 8189 rows 2684 us, 1.62 PFLOP/s with the logits formed again; of 211 rows (fp16)
-// 125 us, of which dW's 133 MB of stores and dh's 133 MB of loads take 40 at the memory's rate and overlap little.
+// tensor pipe 95% active; gradient of 8189 rows 2575 to 2713 us as the clocks allow, 1.2 PFLOP/s with the logits formed
+// again; of 211 rows (fp16) 125 us, of which dW's 133 MB of stores and dh's 133 MB of loads take 40 at the memory's rate and overlap little.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
 //     row and half tile.
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(const float* __restrict__ 
 static int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 constexpr int kPairs = 74;                        // CTA pairs of a B200
-constexpr int64_t kDzBytes = int64_t(96) << 20;  // a piece's dz at most: it and what it meets stay mostly in L2
+constexpr int64_t kDzBytes = int64_t(112) << 20;  // a piece's dz at most: it and what it meets stay mostly in L2
 
 struct LossLayout {
   int n_tiles;
@@ -765,23 +765,50 @@ struct GradLayout {
   int pieces, width, splits;  // width: columns of a piece, a multiple of the tile
   int64_t gmax, dz, part, total;
 };
+
+// Time of a piece of `c` vocabulary tiles, in k blocks of the CTA pair that has the most to do (tiles are dealt out in turn,
+// dh's before dW's). A tile costs one k block more than its contraction, and 12 at least (its epilogue), a launch 15.
+// dh's fp32 sums, read and written for each piece and split, cost as much as a k block (0.27 us) for every 100000.
+static int64_t piece_time(int64_t m, int64_t nh, int64_t kb_n, int64_t kb_h, int64_t c, int64_t splits) {
+  const int64_t dh = m * nh * splits, all = dh + c * nh;
+  const int64_t t_dh = (c * (kBN / kBK) + splits - 1) / splits + 1, t_dw = kb_n + 1 > 12 ? kb_n + 1 : 12;
+  int64_t most = 0;
+  const int64_t turns[3] = {0, dh % kPairs, all % kPairs};  // where the number of dh's, or of all tiles, changes
+  for (int64_t p : turns) {
+    const int64_t here_dh = (dh - p + kPairs - 1) / kPairs, here = (all - p + kPairs - 1) / kPairs;
+    const int64_t t = here_dh * t_dh + (here - here_dh) * t_dw;
+    if (t > most) most = t;
+  }
+  return most + (m * c + kPairs - 1) / kPairs * (kb_h + 1) + 30;
+}
+
 static GradLayout grad_layout(int n, int vocab, int hidden) {
-  GradLayout l;
-  const int64_t tiles = (vocab + kBN - 1) / kBN;
+  GradLayout l{};
+  const int64_t tiles = (vocab + kBN - 1) / kBN, m = up(n > 0 ? n : 1, kBM) / kBM, nh = up(hidden, kBN) / kBN;
+  const int64_t kb_n = up(n, kBK) / kBK, kb_h = up(hidden, kBK) / kBK;
   int64_t most = kDzBytes / (2 * static_cast<int64_t>(n > 0 ? n : 1)) / kBN;
   if (most < 1) most = 1;
-  l.pieces = static_cast<int>((tiles + most - 1) / most);
-  const int64_t per = (tiles + l.pieces - 1) / l.pieces;
-  l.width = static_cast<int>(per * kBN);
-  // Few rows: dh has few tiles with a contraction as long as the piece; split it until every pair has one.
-  const int64_t dh_tiles = up(n, kBM) / kBM * (up(hidden, kBN) / kBN);
-  int64_t s = dh_tiles > 0 ? kPairs / dh_tiles : 1;
-  const int64_t kb = up(vocab < l.width ? vocab : l.width, kBK) / kBK / 4;  // at least 4 k blocks a part
-  if (s > kb) s = kb;
-  l.splits = static_cast<int>(s < 1 ? 1 : s);
-  // every piece, the last one too, has at least one k block for each split
-  const int64_t last = (vocab - static_cast<int64_t>(l.pieces - 1) * l.width + kBK - 1) / kBK;
-  if (l.splits > last) l.splits = static_cast<int>(last < 1 ? 1 : last);
+  // Pieces from as few as dz allows, and parts of dh's contraction (few rows: dh has few tiles, whose contraction is as long
+  // as the piece), so that the pairs end together. With as few pieces as possible, and parts until every pair has a tile of
+  // dh: 1024 rows of 1280 339 us, 2048 rows 824, 8189 rows 2756; so 325, 729, 2713.
+  const int64_t least = (tiles + most - 1) / most;
+  int64_t best = -1;
+  for (int64_t pieces = least; pieces <= least + 4 && pieces <= tiles; ++pieces) {
+    const int64_t per = (tiles + pieces - 1) / pieces, whole = (tiles - 1) / per, last = tiles - whole * per;
+    // at least 4 k blocks a part, and one in the last piece, whose last tile may be cut
+    const int64_t kb = (vocab < per * kBN ? up(vocab, kBK) : per * kBN) / kBK / 4;
+    const int64_t kb_last = (vocab - whole * per * kBN + kBK - 1) / kBK;
+    for (int64_t splits = 1; splits <= 16; ++splits) {
+      if (splits > 1 && (splits > kb || splits > kb_last)) break;
+      const int64_t t = whole * piece_time(m, nh, kb_n, kb_h, per, splits) +
+                        piece_time(m, nh, kb_n, kb_h, last, splits) + (whole + 1) * splits * n * hidden / 100000;
+      if (best >= 0 && t >= best) continue;
+      best = t;
+      l.pieces = static_cast<int>(whole + 1);
+      l.width = static_cast<int>(per * kBN);
+      l.splits = static_cast<int>(splits);
+    }
+  }
   l.gmax = up(static_cast<int64_t>(n) * hidden * 2, 256);
   l.dz = l.gmax + 256;
   l.part = l.dz + up(static_cast<int64_t>(n) * l.width * 2, 256);
