@@ -254,3 +254,50 @@ def test_prompt_attention_of_one_to_three_rows(ext, lq, group, dtype):
         ext.prompt_attention(q, k, v, out, _cu(lq), _cu(lk), 0.2, lse=lse)
         assert ext.device_error() == 0
         _check(q, k, v, out, lse, lq, lk, 0.2, True)
+
+
+@pytest.mark.parametrize('n,vocab,hidden', [(300, 5000, 136), (300, 5000, 128), (2000, 40001, 64), (2000, 40001, 72),
+                                            (1, 33, 64), (65, 200, 192)])
+def test_loss_grad_with_scratch_of_nan(ext, n, vocab, hidden):
+    """Whole and cut chunks of 64, several pieces and splits; the scratch holds NaN before the call."""
+    h, w, targets = _inputs(n, vocab, hidden, 'bf16', seed=3)
+    loss, lse = torch.empty(n, device='cuda'), torch.empty(n, device='cuda')
+    ext.lm_head_loss(h, w, targets, loss, lse,
+                     ws=torch.full((ext.lm_head_loss_workspace(n, vocab),), 255, dtype=torch.uint8, device='cuda'))
+    assert bool(((lse.double() - _want(h, w, targets)[1]).abs() <= _logit_error(h, w)).all())
+    g = torch.rand(n, device='cuda')
+    dh, dw = torch.full_like(h, float('nan')), torch.full_like(w, float('nan'))
+    ws = torch.full((ext.lm_head_loss_grad_workspace(n, vocab, hidden),), 255, dtype=torch.uint8, device='cuda')
+    ext.lm_head_loss_grad(h, w, targets, lse, g, dh, dw, ws=ws)
+    assert ext.device_error() == 0
+    _check_loss_grad(h, w, targets, g, lse, dh, dw)
+
+
+@pytest.mark.parametrize('lq,lk', [([1, 1], [3000, 700]), ([5, 130, 0], [900, 131, 40]), ([300, 1], [300, 1])])
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_prompt_attention_with_scratch_of_nan(ext, lq, lk, dtype):
+    q, k, v = _make(lq, lk, 4, 2, dtype, fused=False)
+    out, lse = torch.full_like(q, float('nan')), torch.empty(4, sum(lq), device='cuda')
+    sizes = (sum(lq), sum(lk), len(lq), 4, 2)
+    ws = torch.full((ext.prompt_attention_workspace(*sizes) + 16,), 255, dtype=torch.uint8, device='cuda')
+    ext.prompt_attention(q, k, v, out, _cu(lq), _cu(lk), 0.125, lse=lse, ws=ws)
+    _check(q, k, v, out, lse, lq, lk, 0.125, True)
+    dout = torch.randn(q.shape, device='cuda').to(q.dtype)
+    grads = [torch.full_like(x, float('nan')) for x in (q, k, v)]
+    ws = torch.full((ext.prompt_attention_grad_workspace(*sizes),), 255, dtype=torch.uint8, device='cuda')
+    ext.prompt_attention_grad(q, k, v, out, dout, lse, _cu(lq), _cu(lk), 0.125, *grads, ws=ws)
+    assert ext.device_error() == 0
+    _check_grad(q, k, v, dout, grads, lq, lk, 0.125, True)
+
+
+def test_embed_grad_with_scratch_of_nan(ext):
+    for n in (1, 40, 9000):
+        ids, dout = torch.randint(300, (n,), device='cuda'), torch.randn(n, 72, device='cuda')
+        ws = torch.full((ext.embed_grad_workspace(n, 72),), 255, dtype=torch.uint8, device='cuda')
+        got, again = (torch.full((300, 72), float('nan'), device='cuda') for _ in range(2))
+        ext.embed_grad(dout, ids, got, ws=ws)
+        ext.embed_grad(dout, ids, again)
+        want = torch.zeros(300, 72, dtype=torch.float64, device='cuda').index_add_(0, ids, dout.double())
+        # n additions in fp32 at most, each off by half a step of the sum of magnitudes
+        size = torch.zeros(300, 72, dtype=torch.float64, device='cuda').index_add_(0, ids, dout.double().abs())
+        assert torch.equal(got, again) and bool(((got.double() - want).abs() <= n * 2.0 ** -24 * size).all())
