@@ -13,7 +13,7 @@
 // and two CTAs share an SM, so that the softmax of one fills the waits of the other. The running maximum moves only when
 // a row exceeds it by 2^8, so O is seldom rescaled. What bounds it: 128 x 128 exponentials take twice as long as the
 // tile's two products of depth 64; an eighth of them run on the FMA pipe instead. Six sequences up to 4096, 32 heads on 8 (bf16):
-// 236 us, 0.65 PFLOP/s, the special-function unit 45% and the tensor pipe 25% active: the softmax warps' own chain.
+// 235 us, 0.66 PFLOP/s, the special-function unit 45% and the tensor pipe 25% active: the softmax warps' own chain.
 // Few rows (serving): the keys are split over several CTAs, whose partial results prompt_join_kernel joins; where there
 // are so few that tiles would be empty, prompt_few_kernel takes the place of the tensor core.
 #include "fw_prompt.cuh"
@@ -23,6 +23,22 @@ namespace fw {
 constexpr int kKStages = 3, kVStages = 2;  // 97 KB with Q: two CTAs an SM
 constexpr int kFwdSmem = (1 + kKStages + kVStages) * kTileBytes + 1024;
 constexpr int kFwdThreads = 32 * 6;  // 4 softmax warps, products, loads
+
+// What a CTA has of its item: first token of the tile, first key block and number of them (this split's).
+struct Span {
+  int tok, j0, cnt;
+};
+__device__ __forceinline__ Span span_of(const PromptArgs& a, const Item& it, int split) {
+  // Causal: the tiles of a sequence from its end, so that the longest start first.
+  const int items = (it.lq + a.tokens - 1) / a.tokens;
+  Span x;
+  x.tok = (a.causal ? items - 1 - it.tile : it.tile) * a.tokens;
+  const int last = min(it.lq, x.tok + a.tokens) - 1;
+  const int all = ((a.causal ? max(0, last + it.lk - it.lq + 1) : it.lk) + kRows - 1) / kRows;  // key blocks that it sees
+  x.j0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
+  x.cnt = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - x.j0;
+  return x;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -34,6 +50,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
       empty_v[kVStages], landed_v, s_full, s_free, p_full, o_done;
   __shared__ uint32_t tmem_base_sh;
   __shared__ Item s_item;
+  __shared__ Span s_span;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
@@ -68,9 +85,15 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
       mbar_init(&p_full, 4);  // P is in tensor memory
       mbar_init(&o_done, 1);  // P V has been added to O
       mbar_fence_init();
-      tma_prefetch_desc(&tmQ);
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
+      const Span x = span_of(a, it, split);
+      s_span = x;
+      if (it.tile >= 0 && x.cnt > 0) {  // the first loads need nobody else
+        mbar_arrive_expect_tx(&bar_q, static_cast<uint32_t>(a.tokens * a.group) * 128);
+        tma_load_3d(smem, &tmQ, &bar_q, 0, kvh * a.group, static_cast<int>(it.q0) + x.tok);
+        mbar_arrive_expect_tx(&full_k[0], kTileBytes);
+        tma_load_3d(ks, &tmK, &full_k[0], 0, kvh, static_cast<int>(it.k0) + x.j0 * kRows);
+        tma_prefetch_desc(&tmV);
+      }
     }
   }
   tc_fence_before();
@@ -79,21 +102,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
   const uint32_t tmem = tmem_base_sh;  // columns: S 0, P 128, O 192
   const Item it = s_item;
   if (it.tile >= 0) {
-    // Causal: the tiles of a sequence from its end, so that the longest start first.
-    const int items = (it.lq + a.tokens - 1) / a.tokens;
-    const int tok = (a.causal ? items - 1 - it.tile : it.tile) * a.tokens;  // the tile's first token
-    const int shift = it.lk - it.lq;
-    const int last = min(it.lq, tok + a.tokens) - 1;
-    const int all = ((a.causal ? max(0, last + shift + 1) : it.lk) + kRows - 1) / kRows;  // key blocks that it sees
-    const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
-    const int cnt = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits) - j0;
+    const int tok = s_span.tok, j0 = s_span.j0, cnt = s_span.cnt, shift = it.lk - it.lq;
 
     if (warp == 5) {
       // ---- loads
-      if (lane == 0 && cnt > 0) {
-        mbar_arrive_expect_tx(&bar_q, static_cast<uint32_t>(a.tokens * a.group) * 128);
-        tma_load_3d(smem, &tmQ, &bar_q, 0, kvh * a.group, static_cast<int>(it.q0 + tok));
-      }
       bool ok = true;
       for (int jj = 0; jj < cnt && ok; ++jj) {
         const int s = jj % kKStages, sv = jj % kVStages;
@@ -102,8 +114,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) prompt_attn_kernel(const __gri
         if (lane == 0) {
           if (jj >= kKStages) ok = mbar_wait(&empty_k[s], ((jj / kKStages) & 1u) ^ 1u);
           if (ok) {
-            mbar_arrive_expect_tx(&full_k[s], kTileBytes);
-            tma_load_3d(ks + s * kTileBytes, &tmK, &full_k[s], 0, kvh, row);
+            if (jj > 0) {  // the first one is on its way
+              mbar_arrive_expect_tx(&full_k[s], kTileBytes);
+              tma_load_3d(ks + s * kTileBytes, &tmK, &full_k[s], 0, kvh, row);
+            }
             if (jj >= kVStages) ok = mbar_wait(&empty_v[sv], ((jj / kVStages) & 1u) ^ 1u);
           }
           if (ok) {
