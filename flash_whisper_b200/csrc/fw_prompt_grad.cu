@@ -17,7 +17,7 @@
 // the step after the next once P and dS are there: a step's hand-overs hide behind the exponentials. Steps run on across
 // items: the loads and the first products of the next item start while the results of the last one are read out (with one
 // CTA per item 24 CTAs an SM spent 8 us each outside of their steps).
-// Six sequences up to 4096, 32 heads on 8 (bf16): 616 us, 0.63 PFLOP/s of what the formulas need, the special-function
+// Six sequences up to 4096, 32 heads on 8 (bf16): 611 us, 0.63 PFLOP/s of what the formulas need, the special-function
 // unit 46% and the tensor pipe 40% active. Tried and slower: steps of 64 with two sets of X and Y and 8 warps on each
 // (693), all products from one warp (674: its waits add to the products' time), A in tensor memory with P and dS over Y
 // (715), the two halves of the warps taking turns at the exponentials (667), a quarter of the exponentials as polynomials
@@ -304,16 +304,23 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     }
     mbar_fence_init();
   }
-  pdl_wait();
-  if (warp == 16 && !Type16<T>::kBf16) {
-    float m = 0.f;
-    for (int i = lane; i < kDeltaBlocks; i += 32) m = fmaxf(m, g.largest[i]);
-    m = warp_max(m);
-    if (lane == 0) s_norm = normalizer(m);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // prompt_delta_kernel runs beside all this and the first loads, up to here for those who read what it writes
+  if (warp < 17) {
+    pdl_wait();
+    if (!Type16<T>::kBf16) {
+      if (warp == 16) {
+        float m = 0.f;
+        for (int i = lane; i < kDeltaBlocks; i += 32) m = fmaxf(m, g.largest[i]);
+        m = warp_max(m);
+        if (lane == 0) s_norm = normalizer(m);
+        __syncwarp();
+      }
+      asm volatile("bar.sync 1, 544;" ::: "memory");
+    }
+  }
   const uint32_t tmem = tmem_base_sh;  // columns: X 0 and 128, Y 256, dV 384, dK or dQ 448
 
   if (warp == 17) {
@@ -321,14 +328,20 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     bool ok = true, end = false;
     uint32_t cut = 0;  // tiles that end inside a step so far
     int step = 0;
+    // The first item is this CTA's by its number; the next ones are drawn while the one before is being loaded.
+    unsigned ahead = blockIdx.x;
+    bool waited = false;
+    auto draw = [&] {
+      if (!waited) pdl_wait();  // the counter, and the statistics, are prompt_delta_kernel's
+      waited = true;
+      if (lane == 0) ahead = gridDim.x + atomicAdd(g.next, 1u);
+    };
     for (int n = 0; ok && !end; ++n) {
       // The next item with something to do. Rows without a step (keys that no query sees, queries that see no key) have
       // zero gradients, written here.
       GradItem x;
       while (true) {
-        unsigned drawn = 0;
-        if (lane == 0) drawn = atomicAdd(g.next, 1u);
-        const int64_t index = __shfl_sync(0xffffffffu, drawn, 0);
+        const int64_t index = __shfl_sync(0xffffffffu, ahead, 0);
         x.end = index >= g.all_items;
         if (x.end) break;
         x.keys = index < g.key_items;
@@ -336,7 +349,10 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         x.kvh = in % a.kv_heads;
         const Item it = x.keys ? find_item(a.cu_k, a.cu_q, a.rows_k, a.rows_q, a.seqs, kRows, 0, in / a.kv_heads, lane)
                                : find_item(a.cu_q, a.cu_k, a.rows_q, a.rows_k, a.seqs, a.tokens, 0, in / a.kv_heads, lane);
-        if (it.tile < 0) continue;
+        if (it.tile < 0) {
+          draw();
+          continue;
+        }
         x.seq = it.seq;
         x.q0 = x.keys ? it.k0 : it.q0, x.lq = x.keys ? it.lk : it.lq;  // find_item was asked with q and k swapped
         x.k0 = x.keys ? it.q0 : it.k0, x.lk = x.keys ? it.lq : it.lk;
@@ -369,6 +385,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                                       (x.kvh * a.group + r % a.group) * g.dq_head + c) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
+        draw();
       }
       end = x.end != 0;
       if (n >= kRing) ok = mbar_wait_warp(&item_free[n % kRing], ((n / kRing) & 1u) ^ 1u);
@@ -400,13 +417,15 @@ __global__ void __launch_bounds__(kGradThreads, 1)
         uint8_t* dst = smem + 4 * kTileBytes + s * kGradStage;
         if (step >= kGradStages) ok = mbar_wait_warp(&empty[s], ((step / kGradStages) & 1u) ^ 1u);
         if (!ok) break;
+        uint64_t* bar = valid >= kStep ? &full[s] : &landed;
         if (lane == 0) {
-          uint64_t* bar = valid >= kStep ? &full[s] : &landed;
           mbar_arrive_expect_tx(bar, kGradStage + (x.keys ? kStep * 8 : 0));
           tma_load_3d(dst, x.keys ? &tmQ : &tmK, bar, 0, head, row);
           tma_load_3d(dst + kTileBytes, x.keys ? &tmD : &tmV, bar, 0, head, row);
-          if (x.keys) bulk_g2s(s_stat[s], stat_at(g, head, stat_start(x.q0, x.seq) + at), kStep * 8, bar);
         }
+        __syncwarp();
+        if (j == 0) draw();
+        if (x.keys && lane == 0) bulk_g2s(s_stat[s], stat_at(g, head, stat_start(x.q0, x.seq) + at), kStep * 8, bar);
         __syncwarp();
         if (valid < kStep) {
           // Rows behind the sequence's end may hold anything, and 0 x NaN must not reach a sum over them.
