@@ -128,7 +128,7 @@ static int check_rows(const char* what, const char* name, const fw_rows_t& x, in
   FW_REQUIRE(aligned16(x.ptr) && x.token % 8 == 0 && x.head % 8 == 0, FW_ERR_ALIGN,
              "%s: %s must start on 16 bytes and have strides of a multiple of 8 elements", what, name);
   FW_REQUIRE(x.head >= 64 && x.token >= 64 && x.token < (int64_t(1) << 36) && x.head < (int64_t(1) << 36) &&
-                 (heads == 1 || rows <= 1 || x.token >= x.head * (heads - 1) + 64 || x.head >= x.token * (rows - 1) + 64),
+                 (heads == 1 || rows <= 1 || x.token >= x.head * (heads - 1) + 64 || (x.head - 64) / x.token >= rows - 1),
              FW_ERR_SHAPE, "%s: %s has overlapping or negative strides", what, name);
   return FW_OK;
 }

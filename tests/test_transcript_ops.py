@@ -173,3 +173,22 @@ def test_prompt_wrappers_refuse():
 
 def test_rows_struct_matches_header():
     assert ctypes.sizeof(_lib.Rows) == 24 and _lib.Rows.token.offset == 8 and _lib.Rows.head.offset == 16
+
+
+def test_prompt_attention_refuses_what_overflows():
+    for scale in (2.5e38, 3.4e38):  # times log2 e no longer finite
+        _refused('fw_prompt_attention', _attn(scale=scale), 4, 'positive and finite')
+        _refused('fw_prompt_attention_grad', _attn_grad(scale=scale), 4, 'positive and finite')
+    wide = _rows(token=1 << 35, head=(1 << 35) - 64)  # neither rows behind heads nor heads behind rows
+    _refused('fw_prompt_attention', _attn(k=wide, rows_k=(1 << 29) + 1), 2, 'overlapping')
+
+
+@pytest.mark.parametrize('vocab,hidden', [(1, 8), (33, 64), (5003, 384), (51866, 1280), (1 << 22, 1280)])
+def test_loss_scratch_grows_with_rows_and_stays_bounded(vocab, hidden):
+    """Over the rows' whole range, kernels and pieces changing on the way: never more than dz's 112 MB (or one tile of 256
+    columns), 16 parts of dh's sums and the copy of h; and the forward's 8 bytes a row and half tile, or a CTA."""
+    ext = Ext()
+    for n in (1, 2, 31, 32, 33, 64, 65, 211, 1024, 2047, 4096, 8189, 16381, 100001):
+        most = max(112 << 20, n * 256 * 2) + n * hidden * (16 * 4 + 2) + 4096
+        assert n * hidden * 6 < ext.lm_head_loss_grad_workspace(n, vocab, hidden) <= most
+        assert 8 * n <= ext.lm_head_loss_workspace(n, vocab) <= 8 * n * max(148, 2 * -(-vocab // 256))
