@@ -301,3 +301,29 @@ def test_embed_grad_with_scratch_of_nan(ext):
         # n additions in fp32 at most, each off by half a step of the sum of magnitudes
         size = torch.zeros(300, 72, dtype=torch.float64, device='cuda').index_add_(0, ids, dout.double().abs())
         assert torch.equal(got, again) and bool(((got.double() - want).abs() <= n * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize('lq,lk', [([1] * 60 + [200], [300] * 61), ([1] * 9 + [70], [5000] * 10)])
+def test_prompt_among_single_tokens_captured_and_replayed(ext, lq, lk):
+    """Both launches (and the join of the key splits) in a graph, replayed over new contents."""
+    q, k, v = _make(lq, lk, 1, 1, 'fp16', fused=False)
+    cu_q, cu_k, out = _cu(lq), _cu(lk), torch.empty_like(q)
+    lse = torch.empty(1, sum(lq), device='cuda')
+    ws = torch.empty(ext.prompt_attention_workspace(sum(lq), sum(lk), len(lq), 1, 1) + 16, dtype=torch.uint8,
+                     device='cuda')
+
+    def step():
+        ext.prompt_attention(q, k, v, out, cu_q, cu_k, 0.125, lse=lse, ws=ws)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+        step()
+    for seed in (1, 2):
+        for x, y in zip((q, k, v), _make(lq, lk, 1, 1, 'fp16', seed=seed, fused=False)):
+            x.copy_(y)
+        out.fill_(float('nan'))
+        graph.replay()
+        _check(q, k, v, out, lse, lq, lk, 0.125, True)
+    assert ext.device_error() == 0
