@@ -219,7 +219,7 @@ __device__ __forceinline__ bool grad_steps(const GradRow& g, int first, int h, c
     tc_wait_store();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(g.p_full);
+    if (lane == 0) mbar_arrive(g.p_full + (j & 1));
   }
   return true;
 }
@@ -268,8 +268,8 @@ __global__ void __launch_bounds__(kGradThreads, 1)
                        const __grid_constant__ CUtensorMap tmQa, const __grid_constant__ CUtensorMap tmDa, GradArgs g) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) float s_stat[kGradStages][2 * kStep];
-  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], y_full, y_free, p_full, a_full[2],
-      a_free[2], done, item_full[kRing], item_free[kRing];
+  __shared__ __align__(8) uint64_t full[kGradStages], empty[kGradStages], landed, x_full[2], y_full, y_free, p_full[2],
+      a_full[2], a_free[2], done, item_full[kRing], item_free[kRing];
   __shared__ uint32_t tmem_base_sh;
   __shared__ GradItem s_item[kRing];
   __shared__ float s_norm;
@@ -291,12 +291,15 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     mbar_init(&landed, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x_full[i], 1);  // X of an even or odd step is in tensor memory
+      // P and dS of an even or odd step are there. One barrier for both would not do: a warp has given Y back before it
+      // stores dS, so another could run ahead to the next step and arrive in its place. Its next arrival on the barrier of
+      // the same parity follows x_full of two steps on, which is issued only after this step's sixteen have been waited for.
+      mbar_init(&p_full[i], 16);
       mbar_init(&a_full[i], 1);  // A1 and A2 of an even or odd item have landed
       mbar_init(&a_free[i], 2);  // its X and its Y are done
     }
     mbar_init(&y_full, 1);   // Y is in tensor memory
     mbar_init(&y_free, 16);  // it has been read
-    mbar_init(&p_full, 16);  // P and dS are in tensor memory
     mbar_init(&done, 1);     // an item's results are
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&item_full[i], 1);
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       if (j >= 0) {
         ok = cs.next(s_item, item_full);
         if (!ok || cs.end) break;
-        ok = mbar_wait_warp(&p_full, j & 1u);
+        ok = mbar_wait_warp(&p_full[j & 1], (j >> 1) & 1u);
         if (!ok) break;
         tc_fence_after();
         const uint64_t b1 = sw128_mn_desc(b_base + j % kGradStages * kGradStage, kTileBytes),
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       }
       gr.tx = tmem + lanes + 32 * grp;
       gr.ty = tmem + lanes + 256 + 32 * grp;
-      gr.x_full = x_full, gr.y_full = &y_full, gr.y_free = &y_free, gr.p_full = &p_full;
+      gr.x_full = x_full, gr.y_full = &y_full, gr.y_free = &y_free, gr.p_full = p_full;
       gr.full = full;
       if (keys) {
         gr.hi0 = it.lq;
