@@ -507,6 +507,17 @@ __global__ void __launch_bounds__(32 * kFewWarps, 4) prompt_few_kernel(const Few
     few_rows<T>(x, a, sh, q0, lq, k0, lk, kvh, split);
 }
 
+// Whether `row` lies in a sequence that has been computed, by one warp. Every sequence is looked at, each by its own offsets: a
+// search by bisection would stop at a sequence with bad offsets and miss the good one behind it. (Where keys are split there
+// are at most 592 sequences.)
+__device__ __forceinline__ bool row_is_computed(const PromptArgs& a, int64_t row, int lane) {
+  for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+    const int b = b0 + lane;
+    if (__any_sync(0xffffffffu, b < a.seqs && good_sequence(a, b) && a.cu_q[b] <= row && row < a.cu_q[b + 1])) return true;
+  }
+  return false;
+}
+
 // Joins the key splits of a (row, head), one warp each: o = sum_s exp(lse_s - lse) o_s.
 template <typename T>
 __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
@@ -516,19 +527,8 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(PromptArgs a) {
   if (i >= a.rows_q * a.heads) return;
   const int64_t row = i / a.heads;
   const int head = static_cast<int>(i % a.heads);
-  // rows that belong to no sequence keep what they hold; sequences with bad offsets were left out above
-  int64_t lo = 0, hi = a.seqs;  // the sequence with cu_q[lo] <= row < cu_q[lo + 1]
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.cu_q[mid] <= row)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  const int64_t k0 = a.cu_k[lo], k1 = a.cu_k[lo + 1];
-  if (row < a.cu_q[lo] || row >= a.cu_q[lo + 1] || a.cu_q[lo] < 0 || a.cu_q[lo + 1] > a.rows_q || k0 < 0 || k1 < k0 ||
-      k1 > a.rows_k)
-    return;
+  // rows that belong to no sequence keep what they hold, and so do those of sequences that were left out above
+  if (!row_is_computed(a, row, lane)) return;
   float top = -INFINITY;
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_lse[(static_cast<int64_t>(s) * a.heads + head) * a.rows_q + row]);
   const float off = top == -INFINITY ? 0.f : -top * kLog2;

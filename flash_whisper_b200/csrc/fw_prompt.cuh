@@ -29,6 +29,12 @@ struct PromptArgs {
   float *part_o, *part_lse;     // splits > 1: [splits][rows_q][heads][64], [splits][heads][rows_q]
 };
 
+// Offsets in order and in range: what does not hold of them leaves a sequence out.
+__device__ __forceinline__ bool good_sequence(const PromptArgs& a, int b) {
+  const int64_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
+  return q0 >= 0 && q1 >= q0 && q1 <= a.rows_q && k0 >= 0 && k1 >= k0 && k1 <= a.rows_k;
+}
+
 // Where a work item lies: a tile of one sequence.
 struct Item {
   int64_t q0, k0;  // first rows of the sequence
