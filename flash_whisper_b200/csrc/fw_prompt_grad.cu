@@ -66,6 +66,10 @@ __device__ __forceinline__ float normalizer(float x) {
   return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
 }
 
+__device__ __forceinline__ bool holds_row(const PromptArgs& a, int seq, int64_t row) {
+  return good_sequence(a, seq) && a.cu_q[seq] <= row && row < a.cu_q[seq + 1];
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
   __shared__ float s_max[8];
@@ -76,13 +80,14 @@ __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
   const int64_t units = a.rows_q * a.heads;
   constexpr float kP = Type16<T>::kBf16 ? 0.f : 8.f;  // log2 of the factor that P carries
   float big = 0.f;
+  int ordered = -1;  // whether cu_q is in order, once it is asked for
   for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; u0 < units; u0 += static_cast<int64_t>(gridDim.x) * 32) {
     const int64_t u = u0 + (lane >> 3);
     float dot = 0.f, row_big = 0.f;
-    bool mine = u < units;
+    bool mine = false, lost = false;
     int64_t row = 0, q0 = 0;
     int head = 0, seq = 0;
-    if (mine) {
+    if (u < units) {
       row = u / a.heads;
       head = static_cast<int>(u % a.heads);
       int lo = 0, hi = a.seqs;
@@ -94,9 +99,25 @@ __global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
           hi = mid;
       }
       seq = lo;
-      q0 = a.cu_q[lo];
-      mine = q0 >= 0 && q0 <= row && row < a.cu_q[lo + 1];  // rows of no sequence may hold anything
+      mine = holds_row(a, seq, row);  // rows of no sequence may hold anything
+      lost = !mine;
     }
+    // Offsets out of order mislead the bisection: a good sequence behind them is found by looking at each.
+    if (__any_sync(0xffffffffu, lost)) {
+      if (ordered < 0) {
+        bool back = false;
+        for (int b = lane; b < a.seqs; b += 32) back = back || a.cu_q[b] > a.cu_q[b + 1];
+        ordered = !__any_sync(0xffffffffu, back);
+      }
+      if (lost && !ordered) {
+        for (int b = 0; b < a.seqs && !mine; ++b) {
+          mine = holds_row(a, b, row);
+          seq = b;
+        }
+      }
+      __syncwarp();
+    }
+    if (mine) q0 = a.cu_q[seq];
     if (mine) {
       const uint4 d = reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + row * g.d_token + head * g.d_head)[lane & 7];
       const uint4 o = reinterpret_cast<const uint4*>(static_cast<const T*>(g.o) + row * g.o_token + head * g.o_head)[lane & 7];

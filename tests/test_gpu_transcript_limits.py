@@ -62,3 +62,67 @@ def test_prompt_attention_good_sequences_behind_bad_offsets(ext, cu_q, cu_k, goo
         _check(q[rq], k[rk], v[rk], out[rq], lse[:, rq], [rq.stop - rq.start], [rk.stop - rk.start], 0.125, True)
         left[rq] = False
     assert bool((out[left] == 3).all()) and bool((lse[:, left] == 3).all())
+
+
+@pytest.mark.parametrize('cu_q,cu_k,good', MIDDLE)
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_prompt_attention_grad_good_sequences_behind_bad_offsets(ext, cu_q, cu_k, good, dtype):
+    """As above, with scratch of NaN and with NaN in what belongs to no good sequence."""
+    rows_q, rows_k, heads, kv_heads = 192, 256, 4, 2
+    q, k, v = _make([rows_q], [rows_k], heads, kv_heads, dtype, fused=False)
+    dout = torch.randn(q.shape, device='cuda').to(q.dtype)
+    out, lse = torch.full_like(q, float('nan')), torch.full((heads, rows_q), float('nan'), device='cuda')
+    spans = [(slice(cu_q[b], cu_q[b + 1]), slice(cu_k[b], cu_k[b + 1])) for b in good]
+    no_q, no_k = (torch.ones(n, dtype=torch.bool, device='cuda') for n in (rows_q, rows_k))
+    for rq, rk in spans:
+        o, l = torch.empty_like(q[rq]), torch.empty(heads, rq.stop - rq.start, device='cuda')
+        ext.prompt_attention(q[rq], k[rk], v[rk], o, _cu([o.size(0)]), _cu([rk.stop - rk.start]), 0.125, lse=l)
+        out[rq], lse[:, rq] = o, l
+        no_q[rq] = no_k[rk] = False
+    q[no_q], dout[no_q], k[no_k], v[no_k] = (float('nan'),) * 4
+    need = ext.prompt_attention_grad_workspace(rows_q, rows_k, len(cu_q) - 1, heads, kv_heads)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device='cuda')
+    grads = [torch.full_like(x, 3.0) for x in (q, k, v)]
+    ext.device_error()
+    ext.prompt_attention_grad(q, k, v, out, dout, lse, _offsets(*cu_q), _offsets(*cu_k), 0.125, *grads, ws=ws)
+    assert ext.device_error() == 2
+    for rq, rk in spans:
+        _check_grad(q[rq], k[rk], v[rk], dout[rq], [grads[0][rq], grads[1][rk], grads[2][rk]], [rq.stop - rq.start],
+                    [rk.stop - rk.start], 0.125, True)
+    assert bool((grads[0][no_q] == 3).all() and (grads[1][no_k] == 3).all() and (grads[2][no_k] == 3).all())
+
+
+def test_prompt_attention_grad_first_sequence_in_front_of_bad_offsets(ext):
+    """The sequence in front keeps its gradients, not finite ones only."""
+    q, k, v = _make([64, 64], [64, 64], 2, 2, 'fp16', fused=False)
+    dout = torch.randn(q.shape, device='cuda').half()
+    out, lse, _ = _run(ext, q, k, v, dout, _cu([64, 64]), _cu([64, 64]), 0.1, True)
+    for cu_q, cu_k in (([0, 64, 200], [0, 64, 128]), ([0, 64, 128], [0, 64, 300]), ([0, 64, 10], [0, 64, 128]),
+                       ([0, 64, 128], [0, 64, -5])):
+        grads = [torch.full_like(x, 3.0) for x in (q, k, v)]
+        ext.prompt_attention_grad(q, k, v, out, dout, lse, _offsets(*cu_q), _offsets(*cu_k), 0.1, *grads)
+        assert ext.device_error() == 2
+        # the largest |do| may lie in the other sequence: the bound for this one goes by the call's
+        _check_grad(q, k, v, dout, [torch.cat([x[:64], y[64:]]) for x, y in zip(grads, _run(
+            ext, q, k, v, dout, _cu([64, 64]), _cu([64, 64]), 0.1, True)[2])], [64, 64], [64, 64], 0.1, True)
+
+
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_prompt_attention_grad_padded_batch_of_many_sequences(ext, dtype):
+    """Rows in front of, and behind, 70 sequences: which belong to no sequence, with offsets in order."""
+    lens = [(i * 37) % 23 for i in range(70)]
+    n = sum(lens)
+    q, k, v = _make([n + 50], [n + 50], 4, 2, dtype, fused=False)
+    dout = torch.randn(q.shape, device='cuda').to(q.dtype)
+    cu = _cu(lens) + 20
+    for x in (q, k, v, dout):
+        x[:20], x[n + 20:] = float('nan'), float('nan')
+    out, lse = torch.zeros_like(q), torch.zeros(4, n + 50, device='cuda')
+    ext.prompt_attention(q, k, v, out, cu, cu, 0.125, lse=lse)
+    grads = [torch.full_like(x, 3.0) for x in (q, k, v)]
+    ws = torch.full((ext.prompt_attention_grad_workspace(n + 50, n + 50, 70, 4, 2),), 255, dtype=torch.uint8, device='cuda')
+    ext.prompt_attention_grad(q, k, v, out, dout, lse, cu, cu, 0.125, *grads, ws=ws)
+    assert ext.device_error() == 0
+    mid = slice(20, n + 20)
+    _check_grad(q[mid], k[mid], v[mid], dout[mid], [x[mid] for x in grads], lens, lens, 0.125, True)
+    assert all(bool((x[:20] == 3).all() and (x[n + 20:] == 3).all()) for x in grads)
