@@ -509,11 +509,20 @@ __global__ void __launch_bounds__(32 * kFewWarps, 4) prompt_few_kernel(const Few
 
 // Whether `row` lies in a sequence that has been computed, by one warp. Every sequence is looked at, each by its own offsets: a
 // search by bisection would stop at a sequence with bad offsets and miss the good one behind it. (Where keys are split there
-// are at most 592 sequences.)
+// are at most 592 sequences.) As for the tiles, one that begins before the end of a good one in front does not count.
 __device__ __forceinline__ bool row_is_computed(const PromptArgs& a, int64_t row, int lane) {
+  int reach = 0;  // furthest end of a good sequence so far
   for (int b0 = 0; b0 < a.seqs; b0 += 32) {
     const int b = b0 + lane;
-    if (__any_sync(0xffffffffu, b < a.seqs && good_sequence(a, b) && a.cu_q[b] <= row && row < a.cu_q[b + 1])) return true;
+    int first = 0, end = 0;
+    if (b < a.seqs && good_sequence(a, b)) first = static_cast<int>(a.cu_q[b]), end = static_cast<int>(a.cu_q[b + 1]);
+    const unsigned holds = __ballot_sync(0xffffffffu, first <= row && row < end);
+    if (first == end) end = 0;
+    if (holds != 0) {
+      const int at = __ffs(holds) - 1;
+      return max(reach, __reduce_max_sync(0xffffffffu, lane < at ? end : 0)) <= __shfl_sync(0xffffffffu, first, at);
+    }
+    reach = max(reach, __reduce_max_sync(0xffffffffu, end));
   }
   return false;
 }

@@ -44,12 +44,16 @@ struct Item {
 };
 
 // Finds item `index` (counting ceil(lq / per) items per sequence of more than `skip` rows), by one warp, 32 U sequences at
-// a time. Sequences whose offsets are out of order or out of range have none and set the error bit.
+// a time. Sequences whose offsets are out of order or out of range have none and set the error bit. Launches have room for
+// sequences that share no rows. Only behind bad offsets can one begin before the end of a good one in front of it; it has no
+// items either, lest those behind it find no room.
 template <int U>
 __device__ __forceinline__ Item find_among(const int64_t* cu_a, const int64_t* cu_b, int64_t rows_a, int64_t rows_b,
                                            int seqs, int per, int skip, int index, int lane) {
   Item it{};
   it.tile = -1;
+  bool disorder = false;  // bad offsets so far
+  int reach = 0;          // if so, the furthest end of a good sequence so far
   for (int b0 = 0; b0 < seqs; b0 += 32 * U) {
     const int b = b0 + U * lane;
     int64_t a[U + 1], c[U + 1];
@@ -59,17 +63,45 @@ __device__ __forceinline__ Item find_among(const int64_t* cu_a, const int64_t* c
       c[u] = b + u <= seqs ? cu_b[b + u] : 0;
     }
     int n[U], sum = 0;
+    unsigned bad = 0;  // bit u
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       n[u] = 0;
       if (b + u >= seqs) continue;
       if (a[u] < 0 || a[u + 1] < a[u] || a[u + 1] > rows_a || c[u] < 0 || c[u + 1] < c[u] || c[u + 1] > rows_b) {
         prompt_flag(FW_DEVERR_BAD_INDEX);
+        bad |= 1u << u;
         continue;
       }
       const unsigned rows = static_cast<unsigned>(a[u + 1] - a[u]);
       if (rows > static_cast<unsigned>(skip)) n[u] = (rows + per - 1) / static_cast<unsigned>(per);
       sum += n[u];
+    }
+    if (disorder || __any_sync(0xffffffffu, bad != 0)) {
+      if (!disorder) reach = max(0, static_cast<int>(__shfl_sync(0xffffffffu, b0 > 0 ? a[0] : 0, 0)));  // in order up to here
+      disorder = true;
+      int end[U], front = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        end[u] = b + u < seqs && !(bad & (1u << u)) && a[u + 1] > a[u] ? static_cast<int>(a[u + 1]) : 0;
+        front = max(front, end[u]);
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, front, o);
+        if (lane >= o) front = max(front, x);
+      }
+      const int all = __shfl_sync(0xffffffffu, front, 31);
+      front = __shfl_up_sync(0xffffffffu, front, 1);
+      front = lane == 0 ? reach : max(reach, front);
+      reach = max(reach, all);
+      sum = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (a[u] < front) n[u] = 0;
+        front = max(front, end[u]);
+        sum += n[u];
+      }
     }
     int incl = sum;
 #pragma unroll

@@ -422,7 +422,9 @@ typedef struct {
  * Queries that see no key have out = 0 and lse = -inf. Rows that belong to no sequence are left as they
  * are, and what they hold reaches no result; nor does one sequence's content reach another's. (Within a
  * sequence a NaN or infinity in v reaches the 127 queries before it as well: the products run on tiles.)
- * Offsets out of order or out of range set FW_DEVERR_BAD_INDEX and leave that sequence out. Scores, sums and
+ * Offsets out of order or out of range set FW_DEVERR_BAD_INDEX and leave that sequence out; each sequence is
+ * judged by its own offsets. If they go back behind it, a sequence that begins before the end of a good one in front
+ * of it may be left out too, and rows that two sequences name are undefined. Scores, sums and
  * outputs are fp32 until the one rounding of out; the probabilities are rounded to 16 bits (at most 2^8,
  * relative to a running maximum) for their product with v. Replaces no reference kernel: the reference
  * feeds its prompt token by token (custom/model.py:196-207). */

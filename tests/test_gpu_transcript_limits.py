@@ -126,3 +126,43 @@ def test_prompt_attention_grad_padded_batch_of_many_sequences(ext, dtype):
     mid = slice(20, n + 20)
     _check_grad(q[mid], k[mid], v[mid], dout[mid], [x[mid] for x in grads], lens, lens, 0.125, True)
     assert all(bool((x[:20] == 3).all() and (x[n + 20:] == 3).all()) for x in grads)
+
+
+@pytest.mark.parametrize('rows,lens_k', [(1000, 1000), (1000, 60000), (12, 4000)])
+@pytest.mark.parametrize('heads,kv_heads', [(2, 2), (8, 1)])
+def test_prompt_attention_sequence_behind_sequences_that_share_rows(ext, rows, lens_k, heads, kv_heads):
+    """Offsets that go back over and over: the sequence behind them still has its tiles, with and without split keys.
+    Its gradient too."""
+    last, cut_k = rows // 10, lens_k - lens_k // 10
+    cu_q = _offsets(*[0, rows - last] * 20, rows)
+    cu_k = _offsets(*[0, cut_k] * 20, lens_k)
+    q, k, v = _make([rows], [lens_k], heads, kv_heads, 'bf16', fused=False)
+    out, lse = torch.full_like(q, 3.0), torch.full((heads, rows), 3.0, device='cuda')
+    sizes = (rows, lens_k, 40, heads, kv_heads)
+    ws = torch.full((ext.prompt_attention_workspace(*sizes) + 16,), 255, dtype=torch.uint8, device='cuda')
+    ext.device_error()
+    ext.prompt_attention(q, k, v, out, cu_q, cu_k, 0.125, lse=lse, ws=ws)
+    assert ext.device_error() == 2
+    rq, rk = slice(rows - last, rows), slice(cut_k, lens_k)
+    size = [last], [lens_k - cut_k]
+    _check(q[rq], k[rk], v[rk], out[rq], lse[:, rq], *size, 0.125, True)
+    dout = torch.randn(q.shape, device='cuda').bfloat16()
+    grads = [torch.full_like(x, 3.0) for x in (q, k, v)]
+    ws = torch.full((ext.prompt_attention_grad_workspace(*sizes),), 255, dtype=torch.uint8, device='cuda')
+    ext.prompt_attention_grad(q, k, v, out, dout, lse, cu_q, cu_k, 0.125, *grads, ws=ws)
+    assert ext.device_error() == 2
+    _check_grad(q[rq], k[rk], v[rk], dout[rq], [grads[0][rq], grads[1][rk], grads[2][rk]], *size, 0.125, True)
+
+
+def test_prompt_attention_sequences_out_of_their_order(ext):
+    """Good sequences that do not share rows, the later rows first: computed, or left as they were."""
+    q, k, v = _make([192], [192], 4, 2, 'fp16', fused=False)
+    cu = _offsets(128, 192, 0, 70, 128)
+    out, lse = torch.full_like(q, 3.0), torch.full((4, 192), 3.0, device='cuda')
+    ext.device_error()
+    ext.prompt_attention(q, k, v, out, cu, cu, 0.125, lse=lse)
+    assert ext.device_error() == 2
+    for first, end, must in ((128, 192, True), (0, 70, False), (70, 128, False)):
+        s = slice(first, end)
+        if must or not bool((out[s] == 3).all()):
+            _check(q[s], k[s], v[s], out[s], lse[:, s], [end - first], [end - first], 0.125, True)
