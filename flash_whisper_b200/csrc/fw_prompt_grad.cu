@@ -22,8 +22,9 @@
 // (693), all products from one warp (674: its waits add to the products' time), A in tensor memory with P and dS over Y
 // (715), the two halves of the warps taking turns at the exponentials (667), a quarter of the exponentials as polynomials
 // on the FMA pipe (no change).
-// fp16 range: P is kept times 2^8, and dS times 2^4 over the power of two of the largest |do| (of the row in a query
-// item, of the call in a key item), so that gradients of any size keep their bits; bf16 needs neither.
+// fp16 range: P is kept times 2^8, and dS times 2^6 over the powers of two of the largest |v| (of the call) and the largest
+// |do| (of the row in a query item, of the call in a key item), so that gradients of any size keep their bits and none
+// overflows: |do . v - delta| is at most 2 x 64 times the two, so what is kept stays below 2^15. bf16 needs neither.
 #include "fw_prompt.cuh"
 
 namespace fw {
@@ -38,8 +39,8 @@ constexpr int kRing = 4;  // items known ahead; the first products look two step
 
 struct GradArgs {
   PromptArgs p;
-  const void *o, *dout;
-  int64_t o_token, o_head, d_token, d_head;
+  const void *o, *dout, *v;
+  int64_t o_token, o_head, d_token, d_head, v_token, v_head;
   void *dq, *dk, *dv;
   int64_t dq_token, dq_head, dk_token, dk_head, dv_token, dv_head;
   // [heads][stat_rows]: log2 of P's factor - lse log2 e, and -delta, four rows of the first and then of the second at a
@@ -47,7 +48,7 @@ struct GradArgs {
   float* stat;
   int64_t stat_rows;
   float* norm;                   // fp16: [heads][stat_rows], the power of two that takes a row's largest |do| to [1, 2)
-  float* largest;                // fp16: [kDeltaBlocks], largest finite |do| each block met
+  float* largest;                // fp16: [2][kDeltaBlocks], largest finite |do| and |v| each block met
   unsigned* next;                // the next work item to be drawn
   int64_t key_items, all_items;  // key items come first: they are the longer ones
   float scale;
@@ -66,84 +67,113 @@ __device__ __forceinline__ float normalizer(float x) {
   return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
 }
 
-__device__ __forceinline__ bool holds_row(const PromptArgs& a, int seq, int64_t row) {
-  return good_sequence(a, seq) && a.cu_q[seq] <= row && row < a.cu_q[seq + 1];
+// The good sequence that holds `row` of those that `cu` (cu_q or cu_k) divides, -1 for none. A warp's lanes may ask for
+// different rows, negative ones for nothing. Bisection; offsets out of order mislead it, and a good sequence behind them is
+// found by looking at each. `ordered`: whether they are in order, -1 until it is needed.
+__device__ __forceinline__ int sequence_at(const PromptArgs& a, const int64_t* cu, int64_t row, int* ordered, int lane) {
+  const auto holds = [&](int b) { return good_sequence(a, b) && cu[b] <= row && row < cu[b + 1]; };
+  int found = -1;
+  if (row >= 0) {
+    int lo = 0, hi = a.seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (cu[mid] <= row)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    if (holds(lo)) found = lo;
+  }
+  const bool lost = row >= 0 && found < 0;
+  if (__any_sync(0xffffffffu, lost)) {
+    if (*ordered < 0) {
+      bool back = false;
+      for (int b = lane; b < a.seqs; b += 32) back = back || cu[b] > cu[b + 1];
+      *ordered = !__any_sync(0xffffffffu, back);
+    }
+    if (lost && !*ordered) {
+      for (int b = 0; b < a.seqs && found < 0; ++b)
+        if (holds(b)) found = b;
+    }
+    __syncwarp();
+  }
+  return found;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) prompt_delta_kernel(GradArgs g) {
+__device__ __forceinline__ float largest_finite(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = Type16<T>::unpack(w[i]);
+    if (fabsf(x.x) < INFINITY) big = fmaxf(big, fabsf(x.x));
+    if (fabsf(x.y) < INFINITY) big = fmaxf(big, fabsf(x.y));
+  }
+  return big;
+}
+
+// fp16: a second half of the grid looks for the largest |v| (as a second loop of the same CTAs: 51 us for eight transcripts
+// up to 448, 20 heads; so 49, and 46 without |v|).
+template <typename T>
+__global__ void __launch_bounds__(256, 8) prompt_delta_kernel(GradArgs g) {
   __shared__ float s_max[8];
   pdl_trigger();
   if (blockIdx.x == 0 && threadIdx.x == 0) *g.next = 0u;
   const PromptArgs& a = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t units = a.rows_q * a.heads;
+  const bool values = !Type16<T>::kBf16 && blockIdx.x >= kDeltaBlocks;
+  const int64_t first = ((blockIdx.x - (values ? kDeltaBlocks : 0)) * 8 + warp) * 4;
+  constexpr int kUnits = kDeltaBlocks * 32;  // (row, head) pairs of a turn
   constexpr float kP = Type16<T>::kBf16 ? 0.f : 8.f;  // log2 of the factor that P carries
   float big = 0.f;
-  int ordered = -1;  // whether cu_q is in order, once it is asked for
-  for (int64_t u0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; u0 < units; u0 += static_cast<int64_t>(gridDim.x) * 32) {
-    const int64_t u = u0 + (lane >> 3);
-    float dot = 0.f, row_big = 0.f;
-    bool mine = false, lost = false;
-    int64_t row = 0, q0 = 0;
-    int head = 0, seq = 0;
-    if (u < units) {
-      row = u / a.heads;
-      head = static_cast<int>(u % a.heads);
-      int lo = 0, hi = a.seqs;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.cu_q[mid] <= row)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      seq = lo;
-      mine = holds_row(a, seq, row);  // rows of no sequence may hold anything
-      lost = !mine;
+  int ordered = -1;
+  if (values) {
+    const int64_t units = a.rows_k * a.kv_heads;
+    for (int64_t u0 = first; u0 < units; u0 += kUnits) {
+      const int64_t u = u0 + (lane >> 3);
+      const int64_t row = u < units ? u / a.kv_heads : -1;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= 0)
+        v = reinterpret_cast<const uint4*>(static_cast<const T*>(g.v) + row * g.v_token + u % a.kv_heads * g.v_head)[lane & 7];
+      if (sequence_at(a, a.cu_k, row, &ordered, lane) >= 0) big = fmaxf(big, largest_finite<T>(v));
     }
-    // Offsets out of order mislead the bisection: a good sequence behind them is found by looking at each.
-    if (__any_sync(0xffffffffu, lost)) {
-      if (ordered < 0) {
-        bool back = false;
-        for (int b = lane; b < a.seqs; b += 32) back = back || a.cu_q[b] > a.cu_q[b + 1];
-        ordered = !__any_sync(0xffffffffu, back);
-      }
-      if (lost && !ordered) {
-        for (int b = 0; b < a.seqs && !mine; ++b) {
-          mine = holds_row(a, b, row);
-          seq = b;
-        }
-      }
-      __syncwarp();
-    }
-    if (mine) q0 = a.cu_q[seq];
-    if (mine) {
-      const uint4 d = reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + row * g.d_token + head * g.d_head)[lane & 7];
-      const uint4 o = reinterpret_cast<const uint4*>(static_cast<const T*>(g.o) + row * g.o_token + head * g.o_head)[lane & 7];
-      const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, ow[4] = {o.x, o.y, o.z, o.w};
+  } else {
+    const int64_t units = a.rows_q * a.heads;
+    for (int64_t u0 = first; u0 < units; u0 += kUnits) {
+      const int64_t u = u0 + (lane >> 3);
+      const int64_t row = u < units ? u / a.heads : -1;
+      const int head = static_cast<int>(u % a.heads);
+      const int seq = sequence_at(a, a.cu_q, row, &ordered, lane);  // rows of no sequence may hold anything
+      float dot = 0.f, row_big = 0.f;
+      if (seq >= 0) {
+        const uint4 d =
+            reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + row * g.d_token + head * g.d_head)[lane & 7];
+        const uint4 o = reinterpret_cast<const uint4*>(static_cast<const T*>(g.o) + row * g.o_token + head * g.o_head)[lane & 7];
+        const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, ow[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = Type16<T>::unpack(dw[i]), y = Type16<T>::unpack(ow[i]);
-        dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
-        if (fabsf(x.x) < INFINITY) row_big = fmaxf(row_big, fabsf(x.x));
-        if (fabsf(x.y) < INFINITY) row_big = fmaxf(row_big, fabsf(x.y));
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = Type16<T>::unpack(dw[i]), y = Type16<T>::unpack(ow[i]);
+          dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
+        }
+        if (!Type16<T>::kBf16) row_big = largest_finite<T>(d);
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        row_big = fmaxf(row_big, __shfl_xor_sync(0xffffffffu, row_big, o));
       }
       big = fmaxf(big, row_big);
-    }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      row_big = fmaxf(row_big, __shfl_xor_sync(0xffffffffu, row_big, o));
-    }
-    if (mine && (lane & 7) == 0) {
-      const int64_t at = stat_start(q0, seq) + row - q0;
-      float* st = stat_at(g, head, at);
-      st[0] = kP - a.lse[head * a.rows_q + row] * kLog2;
-      st[4] = -dot;
-      if (!Type16<T>::kBf16) g.norm[head * g.stat_rows + at] = normalizer(row_big);
+      if (seq >= 0 && (lane & 7) == 0) {
+        const int64_t q0 = a.cu_q[seq], at = stat_start(q0, seq) + row - q0;
+        float* st = stat_at(g, head, at);
+        st[0] = kP - a.lse[head * a.rows_q + row] * kLog2;
+        st[4] = -dot;
+        if (!Type16<T>::kBf16) g.norm[head * g.stat_rows + at] = normalizer(row_big);
+      }
     }
   }
+  if (Type16<T>::kBf16) return;
   big = warp_max(big);
   if (lane == 0) s_max[warp] = big;
   __syncthreads();
@@ -293,7 +323,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       a_full[2], a_free[2], done, item_full[kRing], item_free[kRing];
   __shared__ uint32_t tmem_base_sh;
   __shared__ GradItem s_item[kRing];
-  __shared__ float s_norm;
+  __shared__ float s_norm, s_norm_v;  // powers of two for the call's largest |do| and |v|, the second for the latter alone
   const PromptArgs& a = g.p;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -336,10 +366,14 @@ __global__ void __launch_bounds__(kGradThreads, 1)
     pdl_wait();
     if (!Type16<T>::kBf16) {
       if (warp == 16) {
-        float m = 0.f;
-        for (int i = lane; i < kDeltaBlocks; i += 32) m = fmaxf(m, g.largest[i]);
+        float m = 0.f, v = 0.f;
+        for (int i = lane; i < kDeltaBlocks; i += 32) {
+          m = fmaxf(m, g.largest[i]);
+          v = fmaxf(v, g.largest[kDeltaBlocks + i]);
+        }
         m = warp_max(m);
-        if (lane == 0) s_norm = normalizer(m);
+        v = warp_max(v);
+        if (lane == 0) s_norm_v = normalizer(v), s_norm = normalizer(m) * s_norm_v;
         __syncwarp();
       }
       asm volatile("bar.sync 1, 544;" ::: "memory");
@@ -567,13 +601,13 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       gr.c = a.scale_log2;
       gr.off = gr.del = 0.f;
       gr.norm = 1.f;  // the factor of dS besides P's
-      if (!Type16<T>::kBf16 && keys) gr.norm = 0.0625f * s_norm;
+      if (!Type16<T>::kBf16 && keys) gr.norm = 0.25f * s_norm;
       if (!keys && live) {
         const int64_t at = stat_start(it.q0, it.seq) + token;
         const float* st = stat_at(g, head, at);
         gr.off = st[0];
         gr.del = st[4];
-        if (!Type16<T>::kBf16) gr.norm = 0.0625f * g.norm[head * g.stat_rows + at];
+        if (!Type16<T>::kBf16) gr.norm = 0.25f * s_norm_v * g.norm[head * g.stat_rows + at];
       }
       gr.tx = tmem + lanes + 32 * grp;
       gr.ty = tmem + lanes + 256 + 32 * grp;
@@ -637,7 +671,8 @@ static int run_prompt_grad(const fw_rows_t& q, const fw_rows_t& k, const fw_rows
   g.all_items = g.key_items + query_items;
   FW_REQUIRE(g.all_items < (int64_t(1) << 31), FW_ERR_SHAPE, "prompt_attention_grad: too many tiles");
   if (g.all_items == 0) return FW_OK;
-  cudaError_t e = launch(prompt_delta_kernel<T>, dim3(kDeltaBlocks), dim3(256), 0, s, false, g);
+  cudaError_t e = launch(prompt_delta_kernel<T>, dim3(Type16<T>::kBf16 ? kDeltaBlocks : 2 * kDeltaBlocks), dim3(256), 0, s,
+                         false, g);
   int rc = launch_status(e, "prompt_attention_grad delta");
   if (rc) return rc;
   CUtensorMap tq{}, td{}, tk{}, tv{}, tqa{}, tda{};
@@ -686,7 +721,7 @@ int fw_prompt_attention_grad_workspace(int64_t rows_q, int64_t rows_k, int seqs,
   FW_REQUIRE(bytes != nullptr, FW_ERR_NULL, "prompt_attention_grad_workspace: bytes is NULL");
   int rc = check_prompt("prompt_attention_grad", bytes, bytes, seqs, rows_q, rows_k, heads, kv_heads, 1.f, FW_F16);
   if (rc) return rc;
-  *bytes = (kDeltaBlocks + 4) * 4 + heads * grad_stat_rows(rows_q, seqs) * 12;
+  *bytes = (2 * kDeltaBlocks + 4) * 4 + heads * grad_stat_rows(rows_q, seqs) * 12;
   return FW_OK;
 }
 
@@ -733,12 +768,13 @@ int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_ro
   a.lse = const_cast<float*>(lse);
   g.o = out->ptr, g.o_token = out->token, g.o_head = out->head;
   g.dout = dout->ptr, g.d_token = dout->token, g.d_head = dout->head;
+  g.v = v->ptr, g.v_token = v->token, g.v_head = v->head;
   g.dq = dq->ptr, g.dq_token = dq->token, g.dq_head = dq->head;
   g.dk = dk->ptr, g.dk_token = dk->token, g.dk_head = dk->head;
   g.dv = dv->ptr, g.dv_token = dv->token, g.dv_head = dv->head;
   g.largest = static_cast<float*>(workspace);
-  g.next = reinterpret_cast<unsigned*>(g.largest + kDeltaBlocks);
-  g.stat = g.largest + kDeltaBlocks + 4;
+  g.next = reinterpret_cast<unsigned*>(g.largest + 2 * kDeltaBlocks);
+  g.stat = g.largest + 2 * kDeltaBlocks + 4;
   g.stat_rows = grad_stat_rows(rows_q, seqs);
   g.norm = g.stat + 2 * heads * g.stat_rows;
   g.scale = scale;

@@ -438,9 +438,9 @@ int fw_prompt_attention_workspace(int64_t rows_q, int64_t rows_k, int seqs, int 
  * dk and dv are summed over the heads of a group in a fixed order (no atomics: results do not vary from run
  * to run). Every row of a sequence is written (0 where nothing is seen), rows of no sequence are left as
  * they are and what they hold reaches no result. Between the products, the probabilities and their
- * gradients are rounded to 16 bits (in fp16 scaled by powers of two, so that small gradients keep their
- * bits: p (do . v - do . o) may be up to 2047 times the largest |do| of its row for dq, of the call for dk,
- * before it overflows to an infinity); sums are fp32. */
+ * gradients are rounded to 16 bits (in fp16 scaled by powers of two, so that small gradients keep their bits and
+ * none overflows: what lies below 2^-31 of the largest |v| of the call times the largest |do|, of its row for dq,
+ * of the call for dk, may be lost); sums are fp32. */
 int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t* v, const fw_rows_t* out,
                              const fw_rows_t* dout, const float* lse, const int64_t* cu_q, const int64_t* cu_k,
                              int seqs, int64_t rows_q, int64_t rows_k, int heads, int kv_heads, float scale, int causal,

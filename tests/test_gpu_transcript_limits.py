@@ -166,3 +166,36 @@ def test_prompt_attention_sequences_out_of_their_order(ext):
         s = slice(first, end)
         if must or not bool((out[s] == 3).all()):
             _check(q[s], k[s], v[s], out[s], lse[:, s], [end - first], [end - first], 0.125, True)
+
+
+@pytest.mark.parametrize('v_size,do_size,scale', [(4000.0, 1.0, 0.03), (60000.0, 1e-3, 0.02), (300.0, 50.0, 0.03),
+                                                 (1e-3, 100.0, 0.1), (65504.0, 4e-4, 0.001)])
+@pytest.mark.parametrize('lens', [[3, 2, 1], [200, 5], [140, 300]])
+def test_prompt_attention_grad_of_large_values(ext, v_size, do_size, scale, lens):
+    """fp16: values of v in the thousands, where do . v is far beyond the largest |do|; nothing overflows that is in range.
+    Scores are small, so that no probability is below 2^-11: then the error that p brings (2^-17 p times the sum of |do| |v|, of
+    which there are 64) covers half a subnormal step of what is kept, 2^-31 of the largest |do| times the largest |v|."""
+    q, k, v = _make(lens, lens, 4, 2, 'fp16', fused=False)
+    g = torch.Generator(device='cuda').manual_seed(3)
+    v = ((torch.rand(v.shape, device='cuda', generator=g) * 2 - 1) * v_size).half()
+    dout = ((torch.rand(q.shape, device='cuda', generator=g) * 2 - 1) * do_size).half()
+    cu = _cu(lens)
+    _, _, grads = _run(ext, q, k, v, dout, cu, cu, scale, True)
+    assert ext.device_error() == 0
+    assert all(bool(x.isfinite().all()) for x in grads)
+    _check_grad(q, k, v, dout, grads, lens, lens, scale, True)
+
+
+def test_prompt_attention_grad_largest_value_counts_good_rows_only(ext):
+    """What rows of no sequence hold of v does not change a bit; infinities and NaN in a sequence stay there."""
+    lens = [60, 30]
+    q, k, v = _make([120], [120], 4, 2, 'fp16', fused=False)
+    dout = torch.randn(q.shape, device='cuda').half() * 1e-6
+    cu = _cu(lens) + 10
+    want = _run(ext, q, k, v, dout, cu, cu, 0.125, True)
+    for fill in (65504.0, float('inf'), float('nan')):
+        v2 = v.clone()
+        v2[:10], v2[100:] = fill, fill
+        got = _run(ext, q, k, v2, dout, cu, cu, 0.125, True)
+        for a, b in zip(got[2], want[2]):
+            assert torch.equal(a[10:100], b[10:100])
