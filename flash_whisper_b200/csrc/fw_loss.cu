@@ -20,7 +20,8 @@
 // 16-bit dz: exp(z - lse) - [v = t] lies in [-1, 1] whatever g is, so it is stored without g (times 2^12 in fp16,
 // which keeps probabilities down to 2^-36 above the smallest subnormal); g multiplies dh's rows in fp32 at the end, and
 // is folded into the 16-bit copy of h that dW's product reads, relative to the largest |g|, so that with equal
-// weights nothing is rounded a second time.
+// weights nothing is rounded a second time. fp16: the copy is taken up to 2^15 by a power of two, so that rows of small
+// weight keep their bits as far as 2^-29 of the largest |h g|.
 #include "fw_host.h"
 #include "fw_tc.cuh"
 
@@ -71,7 +72,7 @@ struct LossArgs {
   float dz_scale;            // the factor stored with dz
   float* part;               // [splits][n][hidden]
   void* dw;                  // [vocab][hidden]
-  const float* gmax;
+  const float* unscale;      // what loss_scale_kernel's copy of h has to be multiplied with
   int first_piece, accumulate;
   bool chunks;               // MN-major maps over [hidden / 64][rows][64]; hidden is a multiple of 64
 };
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
       const uint32_t d = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * kBN + kCols * part;
       const bool wide = kKind == kGrads && x.dh;  // fp32 rows of 32 columns, else 16-bit rows of 64
       const bool direct = kKind == kGrads && !x.dh && a.accumulate;
-      const float f = kKind == kGrads && !x.dh ? *a.gmax / a.dz_scale : 1.f;
+      const float f = kKind == kGrads && !x.dh ? *a.unscale / a.dz_scale : 1.f;
       const int rows = kKind == kDz || wide ? a.n : a.width;
 #pragma unroll 1
       for (int c = 0; c < (row0 < rows ? kCols : 0); c += 32) {
@@ -661,37 +662,93 @@ __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const flo
   loss[row] = t == ignore || bad ? 0.f : l - loss[row];  // held the target's logit
 }
 
-// Gradient, before the products: the largest finite |g| of the rows that count (each CTA finds it by itself from L2)
-// and h scaled by g relative to it, zero in rows that do not count.
-template <typename T>
-__global__ void __launch_bounds__(256) loss_scale_kernel(const T* __restrict__ h, const float* __restrict__ g,
-                                                         const int64_t* __restrict__ targets, int64_t ignore,
-                                                         int vocab, int n, int hidden, T* __restrict__ scaled,
-                                                         float* __restrict__ gmax) {
-  __shared__ float s_max[8];
-  pdl_trigger();
-  float m = 0.f;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int64_t t = targets[i];
-    const float v = fabsf(g[i]);
-    const bool bad = t != ignore && (t < 0 || t >= vocab);
-    if (bad && blockIdx.x == 0) loss_flag(FW_DEVERR_BAD_INDEX);
-    if (t != ignore && !bad && v < INFINITY) m = fmaxf(m, v);  // NaN fails the comparison
-  }
+constexpr int kScaleThreads = 256, kRangeBlocks = 592;
+__device__ __forceinline__ float block_max(float m, float* shared) {
   m = warp_max(m);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, s_max[w]);
+  for (int w = 0; w < kScaleThreads / 32; ++w) m = fmaxf(m, shared[w]);
+  return m;
+}
+
+// Gradient in fp16, before all else: each CTA's largest finite |g| and |h g| of the rows that count.
+__global__ void __launch_bounds__(kScaleThreads) loss_range_kernel(const half* __restrict__ h, const float* __restrict__ g,
+                                                                   const int64_t* __restrict__ targets, int64_t ignore,
+                                                                   int vocab, int n, int hidden, float2* __restrict__ range) {
+  __shared__ float s_max[2][kScaleThreads / 32];
+  pdl_trigger();
+  const int packs = hidden / 8;
+  float big = 0.f, product = 0.f;
+#pragma unroll 4
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kScaleThreads + threadIdx.x; i < static_cast<int64_t>(n) * packs;
+       i += static_cast<int64_t>(gridDim.x) * kScaleThreads) {
+    const int row = static_cast<int>(i / packs);
+    const int64_t t = targets[row];
+    const float w = fabsf(g[row]);
+    const uint4 v = reinterpret_cast<const uint4*>(h)[i];
+    if (t < 0 || t >= vocab || t == ignore || !(w < INFINITY)) continue;
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    big = fmaxf(big, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = Type16<half>::unpack(u[j]);
+      if (fabsf(x.x) < INFINITY) product = fmaxf(product, fabsf(x.x) * w);
+      if (fabsf(x.y) < INFINITY) product = fmaxf(product, fabsf(x.y) * w);
+    }
+  }
+  big = block_max(big, s_max[0]);
+  product = block_max(product, s_max[1]);
+  if (threadIdx.x == 0) range[blockIdx.x] = make_float2(big, product);
+}
+
+// Gradient, before the products: h scaled by g relative to the largest finite |g| of the rows that count, zero in rows that
+// do not. bf16: each CTA finds that |g| by itself from L2. fp16: loss_range_kernel has, and the power of two that takes the
+// largest |h g| to [2^14, 2^15) besides (1 at least, 2^24 at most). *unscale takes both back.
+template <typename T>
+__global__ void __launch_bounds__(kScaleThreads) loss_scale_kernel(const T* __restrict__ h, const float* __restrict__ g,
+                                                         const int64_t* __restrict__ targets, int64_t ignore,
+                                                         int vocab, int n, int hidden, T* __restrict__ scaled,
+                                                         float* __restrict__ unscale, const float2* __restrict__ range,
+                                                         int ranges) {
+  __shared__ float s_max[2][kScaleThreads / 32];
+  pdl_trigger();
+  float m = 0.f, up = 1.f;
+  if (Type16<T>::kBf16 || blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int64_t t = targets[i];
+      const float v = fabsf(g[i]);
+      const bool bad = t != ignore && (t < 0 || t >= vocab);
+      if (bad && blockIdx.x == 0) loss_flag(FW_DEVERR_BAD_INDEX);
+      if (t != ignore && !bad && v < INFINITY) m = fmaxf(m, v);  // NaN fails the comparison
+    }
+  }
+  if (!Type16<T>::kBf16) {
+    float product = 0.f;
+    pdl_wait();
+    for (int i = threadIdx.x; i < ranges; i += kScaleThreads) {
+      m = fmaxf(m, range[i].x);
+      product = fmaxf(product, range[i].y);
+    }
+    m = block_max(m, s_max[0]);
+    product = block_max(product, s_max[1]) / m;
+    // below 2^16, as |g| / m is at most 1; neither 0, nor infinite for want of fp32's range
+    if (product > 0.f && product < 131072.f) {
+      const int exponent = static_cast<int>(__float_as_uint(product) >> 23) - 127;
+      up = __uint_as_float(static_cast<uint32_t>(min(max(14 - exponent, 0), 24) + 127) << 23);
+    }
+  } else {
+    m = block_max(m, s_max[0]);
+  }
   if (m == 0.f) m = 1.f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *gmax = m;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = m / up;
   const int packs = hidden / 8;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < static_cast<int64_t>(n) * packs;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int row = static_cast<int>(i / packs);
     const int64_t t = targets[row];
     const bool counts = t >= 0 && t < vocab && t != ignore;
-    const float f = counts ? g[row] / m : 0.f;
+    const float f = counts ? g[row] / m * up : 0.f;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (counts) {
       v = reinterpret_cast<const uint4*>(h)[i];
@@ -763,7 +820,7 @@ static LossLayout loss_layout(int n, int vocab) {
 
 struct GradLayout {
   int pieces, width, splits;  // width: columns of a piece, a multiple of the tile
-  int64_t gmax, dz, part, total;
+  int64_t range, dz, part, total;  // offsets (range: loss_scale_kernel's factor, then loss_range_kernel's results); all bytes
 };
 
 // Time of a piece of `c` vocabulary tiles, in k blocks of the CTA pair that has the most to do (tiles are dealt out in turn,
@@ -809,8 +866,8 @@ static GradLayout grad_layout(int n, int vocab, int hidden) {
       l.splits = static_cast<int>(splits);
     }
   }
-  l.gmax = up(static_cast<int64_t>(n) * hidden * 2, 256);
-  l.dz = l.gmax + 256;
+  l.range = up(static_cast<int64_t>(n) * hidden * 2, 256);
+  l.dz = l.range + up((1 + kRangeBlocks) * static_cast<int64_t>(sizeof(float2)), 256);
   l.part = l.dz + up(static_cast<int64_t>(n) * l.width * 2, 256);
   l.total = l.part + static_cast<int64_t>(l.splits) * n * hidden * 4;
   return l;
@@ -925,16 +982,26 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
   const GradLayout l = grad_layout(n, vocab, hidden);
   uint8_t* b = static_cast<uint8_t*>(ws);
   T* scaled = reinterpret_cast<T*>(b);
-  float* gmax = reinterpret_cast<float*>(b + l.gmax);
+  float* unscale = reinterpret_cast<float*>(b + l.range);
+  float2* range = reinterpret_cast<float2*>(b + l.range) + 1;
   void* dz = b + l.dz;
   float* part = reinterpret_cast<float*>(b + l.part);
   const float dz_scale = Type16<T>::kBf16 ? 1.f : 4096.f;
   const int64_t packs = static_cast<int64_t>(n) * (hidden / 8);
   const int64_t blocks = (packs + 255) / 256;
-  cudaError_t e = launch(loss_scale_kernel<T>, dim3(static_cast<unsigned>(blocks < 4 * num_sms() ? blocks : 4 * num_sms())),
-                         dim3(256), 0, s, false, static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden, scaled,
-                         gmax);
-  int rc = launch_status(e, "lm_head_loss_grad scale");
+  const int ranges = static_cast<int>(blocks < kRangeBlocks ? blocks : kRangeBlocks);
+  cudaError_t e = cudaSuccess;
+  int rc = FW_OK;
+  if (!Type16<T>::kBf16) {
+    e = launch(loss_range_kernel, dim3(ranges), dim3(kScaleThreads), 0, s, false, static_cast<const half*>(h), g, targets,
+               ignore, vocab, n, hidden, range);
+    rc = launch_status(e, "lm_head_loss_grad range");
+    if (rc) return rc;
+  }
+  e = launch(loss_scale_kernel<T>, dim3(static_cast<unsigned>(blocks < 4 * num_sms() ? blocks : 4 * num_sms())),
+             dim3(kScaleThreads), 0, s, !Type16<T>::kBf16, static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden,
+             scaled, unscale, static_cast<const float2*>(range), ranges);
+  rc = launch_status(e, "lm_head_loss_grad scale");
   CUtensorMap ta, tb, ga, gb, ga2, gb2, tz, tw, tp;
   if (!rc) rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
   const bool chunks = hidden % 64 == 0;
@@ -979,7 +1046,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     a.splits = l.splits;
     a.part = part;
     a.dw = dw;
-    a.gmax = gmax;
+    a.unscale = unscale;
     a.first_piece = p == 0;
     a.accumulate = accumulate;
     a.chunks = chunks;

@@ -465,8 +465,9 @@ int fw_lm_head_loss_workspace(int n, int vocab, int64_t* bytes);
  * lse is fw_lm_head_loss's for the same h and w, g fp32 [n] (1 / count for a mean). dh or dw may be NULL.
  * Ignored rows have dh = 0 and leave dw alone, whatever h and g hold there. The logits are recomputed in
  * pieces of the vocabulary; exp(z - lse) - [..] is rounded to 16 bits between the products (scaled by 2^12
- * in fp16), which run in fp32; dh and dw have the type of h and w. No atomics: results do not vary from
- * run to run. */
+ * in fp16), which run in fp32, and so is h times g over the largest |g| for dw (in fp16 taken up to 2^15 by a power
+ * of two: what lies below 2^-39 of the largest |h g| is lost); dh and dw have the type of h and w. No atomics:
+ * results do not vary from run to run. */
 int fw_lm_head_loss_grad(const void* h, const void* w, const int64_t* targets, const float* lse, const float* g,
                          void* dh, void* dw, int n, int vocab, int hidden, int64_t ignore_index, int accumulate,
                          int dtype, void* workspace, int64_t workspace_bytes, fw_stream_t stream);

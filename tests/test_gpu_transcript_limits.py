@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.test_gpu_prompt import _check, _cu, _make
-from tests.test_gpu_prompt_grad import _check_grad, _run
+from tests.test_gpu_prompt_grad import _check_grad, _run, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -199,3 +199,38 @@ def test_prompt_attention_grad_largest_value_counts_good_rows_only(ext):
         got = _run(ext, q, k, v2, dout, cu, cu, 0.125, True)
         for a, b in zip(got[2], want[2]):
             assert torch.equal(a[10:100], b[10:100])
+
+
+@pytest.mark.parametrize('top', [0, 12, -8])
+@pytest.mark.parametrize('size', [1.0, 0.01, 200.0])
+def test_loss_grad_of_unequal_weights(ext, top, size):
+    """fp16: weights from 2^top down to 2^(top - 26), and rows so sure of a wrong token that each row of dw comes from one
+    row of h: w[i] is row i's token, row 500 + i its target, so dw[i] = g h and dw[500 + i] = -g h. Roundings: p - [t] (u of it
+    and 2^-37, half a subnormal step over 2^12), the scaled copy of h (u of it, or half a subnormal step 2^-25 where the
+    largest |h g| is kept as at least 2^14, or h as 2^24 times its own), the result (u, or 2^-25); and exp(z) for the others,
+    below 2^-40 in sum."""
+    n, vocab, hidden, u = 105, 1000, 256, 2.0 ** -11
+    gen = torch.Generator(device='cuda').manual_seed(4)
+    w = torch.randn(vocab, hidden, device='cuda', generator=gen)
+    w = (w / size if size < 1 else w * 0.25).half()
+    h = (w[:n].float() * (size * size if size < 1 else 4 * size)).half()
+    targets = 500 + torch.arange(n, device='cuda')
+    g = 2.0 ** (top - torch.arange(n, device='cuda') / 4.0)
+    loss, lse = torch.empty(n, device='cuda'), torch.empty(n, device='cuda')
+    ext.lm_head_loss(h, w, targets, loss, lse)
+    assert bool((loss > 40).all())
+    dh, dw = torch.empty_like(h), torch.full_like(w, float('nan'))
+    ext.lm_head_loss_grad(h, w, targets, lse, g, dh, dw)
+    assert ext.device_error() == 0
+    p = torch.softmax(h.double() @ w.double().T, 1)
+    p[torch.arange(n, device='cuda'), targets] -= 1.0
+    want = (p * g.double()[:, None]).T @ h.double()
+    z_err = 3 * (hidden * 2.0 ** -23 * (h.double().abs() @ w.double().abs().T).amax(1) + 2.0 ** -17)
+    gh = g.double()[:, None] * h.double().abs()
+    kept = max(2.0 ** -39 * float(gh.max()), 2.0 ** -49 * float(g.max()))
+    each = (3 * u + z_err[:, None]) * gh + kept  # of the two rows that row i of h goes to
+    bound = torch.full_like(want, 2.0 ** -25) + (2.0 ** -37 + 2.0 ** -40) * gh.sum(0)
+    bound[:n] += each
+    bound[targets] += each
+    # 200 times 2^12 is beyond fp16: such values round to infinity, which _within allows where the bound reaches that far
+    _within(dw, want, bound, 'dw')
