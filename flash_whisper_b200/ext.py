@@ -69,6 +69,16 @@ def _check_fp32(t, n, dev, name):
         raise RuntimeError(f'{name} must be contiguous CUDA fp32 [{n}] on cuda:{dev}')
 
 
+def _check_lse(t, heads, rows, dev):
+    """Rows before heads would be as many numbers in another order."""
+    _check_fp32(t, heads * rows, dev, 'lse')
+    if t.shape != (heads, rows):
+        more = [n for n in t.shape if n != 1]
+        if len(more) < 2 or more == [heads, rows]:
+            return  # flat, or with dimensions of 1 besides
+        raise RuntimeError(f'lse must be [heads, rows_q] = [{heads}, {rows}]')
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(name, *sizes):
     need = ctypes.c_int64(0)
@@ -399,7 +409,7 @@ class Ext:
         rk, rv = self._rows(k, dtype, dev, like_k, 'k'), self._rows(v, dtype, dev, like_k, 'v')
         rows_q, heads, rows_k, kv_heads = like_q[0], like_q[1], like_k[0], like_k[1]
         if lse is not None:
-            _check_fp32(lse, heads * rows_q, dev, 'lse')
+            _check_lse(lse, heads, rows_q, dev)
         ws = _workspace(ws, self.prompt_attention_workspace(rows_q, rows_k, seqs, heads, kv_heads), dev)
         _call_on(dev, 'fw_prompt_attention', ref(rq), ref(rk), ref(rv), ref(ro), _address(lse), cu_q.data_ptr(),
                  cu_k.data_ptr(), seqs, rows_q, rows_k, heads, kv_heads, scale, 1 if causal else 0, _DTYPES[dtype],
@@ -418,7 +428,7 @@ class Ext:
         rk, rv, rdk, rdv = (self._rows(t, dtype, dev, like_k, name)
                             for t, name in ((k, 'k'), (v, 'v'), (dk, 'dk'), (dv, 'dv')))
         rows_q, heads, rows_k, kv_heads = like_q[0], like_q[1], like_k[0], like_k[1]
-        _check_fp32(lse, heads * rows_q, dev, 'lse')
+        _check_lse(lse, heads, rows_q, dev)
         ws = _workspace(ws, self.prompt_attention_grad_workspace(rows_q, rows_k, seqs, heads, kv_heads), dev)
         _call_on(dev, 'fw_prompt_attention_grad', ref(rq), ref(rk), ref(rv), ref(ro), ref(rd), lse.data_ptr(),
                  cu_q.data_ptr(), cu_k.data_ptr(), seqs, rows_q, rows_k, heads, kv_heads, scale, 1 if causal else 0,

@@ -1,0 +1,72 @@
+"""CPU tests of what the whole-transcript wrappers refuse although sizes and pointers alone would do: stand-ins for CUDA
+tensors, and a library call that is not made."""
+
+import math
+
+import pytest
+import torch
+
+from flash_whisper_b200 import ext as ext_module
+from flash_whisper_b200.ext import Ext
+
+
+class Stub:
+    """What the wrappers ask of a contiguous tensor on cuda:0, of any size."""
+
+    def __init__(self, *shape, dtype=torch.float16):
+        self.shape, self.dtype = torch.Size(shape), dtype
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return len(self.shape)
+
+    def size(self, i):
+        return self.shape[i]
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def stride(self, i=None):
+        steps = tuple(math.prod(self.shape[j + 1:]) for j in range(len(self.shape)))
+        return steps if i is None else steps[i]
+
+    def data_ptr(self):
+        return 256
+
+
+def ints(*shape):
+    return Stub(*shape, dtype=torch.long)
+
+
+def floats(*shape):
+    return Stub(*shape, dtype=torch.float32)
+
+
+def scratch():
+    return Stub(1 << 45, dtype=torch.uint8)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+    monkeypatch.setattr(ext_module, '_call_on', lambda dev, name, *args: made.append(name))
+    return made
+
+
+@pytest.mark.parametrize('shape', [(30, 4), (1, 30, 4), (2, 60), (30, 2, 2)])
+def test_lse_with_rows_before_heads_is_refused(calls, shape):
+    ext, q, cu = Ext(), Stub(30, 4, 64), ints(3)
+    for good in ((4, 30), (120,), (1, 4, 30), (120, 1)):
+        ext.prompt_attention(q, q, q, q, cu, cu, 0.125, lse=floats(*good), ws=scratch())
+        ext.prompt_attention_grad(q, q, q, q, q, floats(*good), cu, cu, 0.125, q, q, q, ws=scratch())
+    assert len(calls) == 8
+    with pytest.raises(RuntimeError, match=r'lse must be \[heads, rows_q\] = \[4, 30\]'):
+        ext.prompt_attention(q, q, q, q, cu, cu, 0.125, lse=floats(*shape), ws=scratch())
+    with pytest.raises(RuntimeError, match=r'lse must be \[heads, rows_q\]'):
+        ext.prompt_attention_grad(q, q, q, q, q, floats(*shape), cu, cu, 0.125, q, q, q, ws=scratch())
+    assert len(calls) == 8
