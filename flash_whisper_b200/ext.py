@@ -79,8 +79,15 @@ def _check_lse(t, heads, rows, dev):
         raise RuntimeError(f'lse must be [heads, rows_q] = [{heads}, {rows}]')
 
 
+def _check_sizes(*sizes):
+    """The library takes these in 32 bits, to which they would be cut silently."""
+    if max(sizes) > 0x7fffffff:
+        raise RuntimeError(f'sizes must be below 2^31, not {max(sizes)}')
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(name, *sizes):
+    _check_sizes(*sizes)
     need = ctypes.c_int64(0)
     _lib.call(name, *sizes, ctypes.byref(need))
     return need.value
@@ -350,6 +357,7 @@ class Ext:
         else:
             _check(pos_embed is positions, 'pos_embed and positions must be given together')
         _check(out.numel() == n * hidden, 'embed_scaled: out must be [n, hidden]')
+        _check_sizes(n, vocab, max_pos, hidden)
         _call_on(dev, 'fw_embed_scaled', embed.data_ptr(), pos_at, ids.data_ptr(), positions_at, out.data_ptr(), n,
                  vocab, max_pos, hidden, scale, _DTYPES[dtype])
 
@@ -367,6 +375,7 @@ class Ext:
         _check(dembed.dim() == 2 and dembed.numel() > 0, 'dembed must be [vocab, hidden]')
         vocab, hidden = dembed.shape
         _check(dout.numel() == n * hidden, 'embed_grad: dout must be [n, hidden]')
+        _check_sizes(n, vocab, hidden)
         ws = _workspace(ws, self.embed_grad_workspace(n, hidden), dev)
         _call_on(dev, 'fw_embed_grad', dout.data_ptr(), ids.data_ptr(), dembed.data_ptr(), n, vocab, hidden, scale,
                  padding_idx, 1 if accumulate else 0, _DTYPES[dtype], _address(ws), _size(ws))
@@ -393,6 +402,7 @@ class Ext:
         dev, seqs = q.get_device(), max(cu_q.numel() - 1, 0)
         _check_ints(cu_q, seqs + 1, dev, 'cu_q')
         _check_ints(cu_k, seqs + 1, dev, 'cu_k')
+        _check_sizes(seqs, heads, kv_heads)
         return dev, (rows_q, heads, HEAD_DIM), (rows_k, kv_heads, HEAD_DIM), seqs
 
     def prompt_attention_workspace(self, rows_q, rows_k, seqs, heads, kv_heads):
@@ -442,6 +452,7 @@ class Ext:
         _check(h.dim() == 2 and w.dim() == 2 and w.size(1) == h.size(1) and w.size(0) > 0 and w.size(1) > 0,
                'h must be [n, hidden], w [vocab, hidden]')
         _check_ints(targets, h.size(0), dev, 'targets')
+        _check_sizes(*h.shape, *w.shape)
         return dev, h.size(0), w.size(0), h.size(1)
 
     def lm_head_loss_workspace(self, n, vocab):

@@ -70,3 +70,33 @@ def test_lse_with_rows_before_heads_is_refused(calls, shape):
     with pytest.raises(RuntimeError, match=r'lse must be \[heads, rows_q\]'):
         ext.prompt_attention_grad(q, q, q, q, q, floats(*shape), cu, cu, 0.125, q, q, q, ws=scratch())
     assert len(calls) == 8
+
+
+FAR = (1 << 32) + 4  # 4 in 32 bits
+
+
+def test_sizes_past_32_bits_are_refused(calls):
+    ext, f = Ext(), floats(4)
+    few, many = Stub(4, 8), Stub(FAR, 8)
+    cases = [
+        lambda: ext.embed_scaled(few, ints(FAR), many),
+        lambda: ext.embed_scaled(many, ints(4), few),
+        lambda: ext.embed_scaled(few, ints(4), few, pos_embed=many, positions=ints(4)),
+        lambda: ext.embed_scaled(Stub(4, FAR), ints(4), Stub(4, FAR)),
+        lambda: ext.embed_grad(many, ints(FAR), few, ws=scratch()),
+        lambda: ext.embed_grad(few, ints(4), many, ws=scratch()),
+        lambda: ext.lm_head_loss(few, many, ints(4), f, f, ws=scratch()),
+        lambda: ext.lm_head_loss(many, few, ints(FAR), floats(FAR), floats(FAR), ws=scratch()),
+        lambda: ext.lm_head_loss_grad(few, many, ints(4), f, f, few, many, ws=scratch()),
+        lambda: ext.prompt_attention(Stub(4, 2, 64), Stub(4, 2, 64), Stub(4, 2, 64), Stub(4, 2, 64), ints(FAR + 1),
+                                     ints(FAR + 1), 0.1, ws=scratch()),
+        lambda: ext.embed_grad_workspace(FAR, 8),
+        lambda: ext.lm_head_loss_workspace(4, FAR),
+        lambda: ext.lm_head_loss_grad_workspace(4, 4, FAR),
+        lambda: ext.prompt_attention_workspace(4, 4, FAR, 2, 2),
+    ]
+    for i, case in enumerate(cases):
+        with pytest.raises(RuntimeError, match='below 2'):
+            case()
+            pytest.fail(f'case {i} was not refused')
+    assert not calls
