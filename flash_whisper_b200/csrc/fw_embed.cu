@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(256) embed_scaled_kernel(const T* __restrict__
                                                            const int64_t* __restrict__ positions, T* __restrict__ out,
                                                            int n, int vocab, int max_pos, int hidden, float scale) {
   using P = Pack<T, VEC>;
-  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);  // may pass 2^31 at the end
+  const int lane = threadIdx.x & 31;
   if (row >= n) return;
   int64_t id = ids[row], at = pos != nullptr ? positions[row] : 0;
   if (id < 0 || id >= vocab || (pos != nullptr && (at < 0 || at >= max_pos))) {
@@ -458,6 +459,11 @@ static EmbedGradLayout embed_grad_layout(int n, int hidden) {
 template <typename T, int VEC>
 static int run_embed_grad(const void* dout, void* dembed, const EmbedGradLayout& l, SortParams sp, SumParams q,
                           cudaStream_t s) {
+  // equal slices of whole packs
+  const int packs = q.hidden / VEC, most = kSliceBytes / static_cast<int>(sizeof(T)) / VEC;
+  const int slices = (packs - 1) / most + 1;
+  FW_REQUIRE(slices <= 65535, FW_ERR_SHAPE, "embed_grad: hidden is too large");
+  const int slice = (packs + slices - 1) / slices * VEC;
   // Sorting CTAs: one up to 2048 tokens, where cluster barriers would cost more than they save.
   const int ctas = sp.n <= 2048 ? 1 : kSortCtas;
   cudaError_t e = cudaSuccess;
@@ -476,11 +482,6 @@ static int run_embed_grad(const void* dout, void* dembed, const EmbedGradLayout&
     rc = launch_status(e, "embed_grad fill");
   }
   if (rc || q.n == 0) return rc;
-  // equal slices of whole packs
-  const int packs = q.hidden / VEC, most = kSliceBytes / static_cast<int>(sizeof(T)) / VEC;
-  const int slices = (packs + most - 1) / most;
-  const int slice = (packs + slices - 1) / slices * VEC;
-  FW_REQUIRE(slices <= 65535, FW_ERR_SHAPE, "embed_grad: hidden is too large");
   const int smem = VEC > 1 ? l.chunk * slice * static_cast<int>(sizeof(T)) : 0;
   e = launch(embed_sum_kernel<T, VEC>, dim3(l.chunks, slices), dim3(kSumThreads), smem, s, true,
              static_cast<const T*>(dout), static_cast<T*>(dembed), q, slice);
@@ -495,7 +496,7 @@ template <typename T, int VEC>
 static int run_embed_scaled(const void* embed, const void* pos, const int64_t* ids, const int64_t* positions,
                             void* out, int n, int vocab, int max_pos, int hidden, float scale, cudaStream_t s) {
   const int warps = n >= 8 * num_sms() ? 8 : 1;  // few rows: spread over the SMs
-  cudaError_t e = launch(embed_scaled_kernel<T, VEC>, dim3((n + warps - 1) / warps), dim3(32 * warps), 0, s, false,
+  cudaError_t e = launch(embed_scaled_kernel<T, VEC>, dim3((static_cast<int64_t>(n) + warps - 1) / warps), dim3(32 * warps), 0, s, false,
                          static_cast<const T*>(embed), static_cast<const T*>(pos), ids, positions,
                          static_cast<T*>(out), n, vocab, max_pos, hidden, scale);
   return launch_status(e, "embed_scaled");
@@ -519,7 +520,7 @@ int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids
   FW_REQUIRE(embed && (n == 0 || (ids && out)), FW_ERR_NULL, "embed_scaled: embed, ids and out are required");
   FW_REQUIRE(n == 0 || (pos_embed == nullptr) == (positions == nullptr), FW_ERR_ARG,
              "embed_scaled: pos_embed and positions must be given together");
-  FW_REQUIRE(n >= 0 && vocab > 0 && hidden > 0 && (pos_embed == nullptr || max_pos > 0), FW_ERR_SHAPE,
+  FW_REQUIRE(n >= 0 && vocab > 0 && hidden > 0 && hidden <= (1 << 30) && (pos_embed == nullptr || max_pos > 0), FW_ERR_SHAPE,
              "embed_scaled: bad sizes");
   FW_REQUIRE(dtype >= FW_F16 && dtype <= FW_F32, FW_ERR_ARG, "embed_scaled: dtype must be fp16, bf16 or fp32");
   const int size = dtype == FW_F32 ? 4 : 2;
@@ -528,7 +529,7 @@ int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids
              FW_ERR_ALIGN, "embed_scaled: pointers must be aligned to their type");
   if (n == 0) return FW_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool wide = hidden * size % 16 == 0 && aligned16(embed) && aligned16(out) && aligned16(pos_embed);
+  const bool wide = hidden * static_cast<int64_t>(size) % 16 == 0 && aligned16(embed) && aligned16(out) && aligned16(pos_embed);
 #define FW_EMBED(T, V) \
   return run_embed_scaled<T, V>(embed, pos_embed, ids, positions, out, n, vocab, max_pos, hidden, scale, s)
   if (dtype == FW_F16) {
@@ -546,7 +547,7 @@ int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids
 
 int fw_embed_grad_workspace(int n, int hidden, int64_t* bytes) {
   FW_REQUIRE(bytes != nullptr, FW_ERR_NULL, "embed_grad_workspace: bytes is NULL");
-  FW_REQUIRE(n >= 0 && hidden > 0, FW_ERR_SHAPE, "embed_grad: bad sizes");
+  FW_REQUIRE(n >= 0 && n <= (1 << 30) && hidden > 0, FW_ERR_SHAPE, "embed_grad: bad sizes");
   *bytes = embed_grad_layout(n, hidden).total;
   return FW_OK;
 }

@@ -390,7 +390,7 @@ int fw_encoder_forward(const fw_encoder_t* e, fw_stream_t stream);
 /* out[i] = T(scale * embed[ids[i]] + pos_embed[positions[i]]), i < n; rows of `hidden` elements of type
  * dtype. pos_embed and positions are given together or both NULL. fw_embed_pos with a scale, with the
  * positions optional and in every type; ids and positions out of range are clamped and set
- * FW_DEVERR_BAD_INDEX as there. */
+ * FW_DEVERR_BAD_INDEX as there. hidden at most 2^30. */
 int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids, const int64_t* positions, void* out,
                     int n, int vocab, int max_pos, int hidden, float scale, int dtype, fw_stream_t stream);
 
@@ -399,7 +399,7 @@ int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids
  * runs in fp32 in the order of i (tokens are sorted, no atomics: the result is the same in every run).
  * accumulate 0 writes every row (zero where no token names it); 1 adds to dembed and touches only the
  * rows that tokens name. Tokens equal to padding_idx (-1: none) are left out; ids out of range are left
- * out and set FW_DEVERR_BAD_INDEX. */
+ * out and set FW_DEVERR_BAD_INDEX. n and vocab at most 2^30, rows of at most 65535 * 1280 bytes. */
 int fw_embed_grad(const void* dout, const int64_t* ids, void* dembed, int n, int vocab, int hidden, float scale,
                   int64_t padding_idx, int accumulate, int dtype, void* workspace, int64_t workspace_bytes,
                   fw_stream_t stream);

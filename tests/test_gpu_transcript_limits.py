@@ -234,3 +234,16 @@ def test_loss_grad_of_unequal_weights(ext, top, size):
     bound[targets] += each
     # 200 times 2^12 is beyond fp16: such values round to infinity, which _within allows where the bound reaches that far
     _within(dw, want, bound, 'dw')
+
+
+def test_embedding_of_nearly_2_31_tokens(ext):
+    """As many tokens as 32 bits count, rows of one element."""
+    n = (1 << 31) - 3
+    table = torch.arange(7, device='cuda').bfloat16()[:, None]
+    ids = torch.zeros(n, dtype=torch.long, device='cuda')
+    ids[-5:], ids[1 << 30] = torch.arange(2, 7, device='cuda'), 1
+    out = torch.full((n, 1), 9.0, dtype=torch.bfloat16, device='cuda')
+    ext.embed_scaled(table, ids, out, scale=2.0)
+    assert ext.device_error() == 0
+    assert out[-6:, 0].tolist() == [0, 4, 6, 8, 10, 12] and float(out[1 << 30]) == 2.0
+    assert float(out.float().sum()) == 42.0

@@ -1,11 +1,13 @@
 """CPU tests of what the whole-transcript wrappers refuse although sizes and pointers alone would do: stand-ins for CUDA
 tensors, and a library call that is not made."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
+from flash_whisper_b200 import _lib
 from flash_whisper_b200 import ext as ext_module
 from flash_whisper_b200.ext import Ext
 
@@ -100,3 +102,17 @@ def test_sizes_past_32_bits_are_refused(calls):
             case()
             pytest.fail(f'case {i} was not refused')
     assert not calls
+
+
+def test_embedding_sizes_at_the_end_of_32_bits():
+    """Scratch for more tokens than the operator takes would come out negative; rows of 2^30 elements and more would
+    overflow the kernels' column counts."""
+    ext, lib, p = Ext(), _lib.lib(), ctypes.c_void_p(256)
+    assert ext.embed_grad_workspace(1 << 30, 8) > 4 << 32
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        with pytest.raises(RuntimeError, match='bad sizes'):
+            ext.embed_grad_workspace(n, 8)
+    assert lib.fw_embed_scaled(p, None, p, None, p, 4, 1, 0, (1 << 30) + 1, 1.0, 1, None) == 2
+    # refused before anything is launched, so without a GPU too
+    assert lib.fw_embed_grad(p, p, p, 4, 1, 1 << 30, 1.0, -1, 0, 1, p, 1 << 62, None) == 2
+    assert b'hidden is too large' in lib.fw_last_error_string()
