@@ -3,7 +3,7 @@
 // Forward: out_i = T(scale E[id_i] + P[pos_i]), fp32 arithmetic, one rounding. One warp per row with 16-byte
 // accesses; bound by HBM (32749 rows of 1280 bf16, 168 MB: 33 us a call, 5.1 TB/s).
 //
-// Gradient: dE[v] = scale sum_{i: id_i = v} dout_i, the sum in fp32 in the order of i. Tokens repeat a lot (text
+// Gradient: dE[v] = scale sum_{i: id_i = v} dout_i, the sum in fp32 in a fixed order. Tokens repeat a lot (text
 // is close to a Zipf law), so the rows of one token are brought together by a stable sort instead of adding them
 // with atomics, whose order would change the result from run to run:
 //   1. embed_sort_kernel: one cluster sorts (id, row) by id, an LSD radix sort of 8 bits a pass whose digit counts are

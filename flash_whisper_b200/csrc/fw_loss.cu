@@ -8,9 +8,10 @@
 // (cta_group::2, 256 x 256 tiles: each CTA stages 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a
 // third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 5 or 6 stages, with the accumulators of
 // two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
-// Measured (vocabulary 51866, hidden 1280, bf16; below the power cap): forward of 16381 rows 1340 us, 1.62 PFLOP/s, the
-// tensor pipe 95% active; gradient of 8189 rows 2575 to 2713 us as the clocks allow, 1.2 PFLOP/s with the logits formed
-// again; of 211 rows (fp16) 125 us, of which dW's 133 MB of stores and dh's 133 MB of loads take 40 at the memory's rate and overlap little.
+// Measured (vocabulary 51866, hidden 1280, bf16), as the clocks allow: forward of 16381 rows 1340 to 1570 us, 1.4 to 1.6
+// PFLOP/s, the tensor pipe 95% active; gradient of 8189 rows 2575 to 2740 us, 1.2 PFLOP/s by the formulas, which do not count
+// the logits that are formed again; of 211 rows (fp16) 125 to 139 us, of which dW's 133 MB of stores and dh's 133 MB of loads
+// take 40 at the memory's rate and overlap little.
 //   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
 //     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
 //     row and half tile.
@@ -48,7 +49,8 @@ constexpr int smem_of(int kind) {
   return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : epi_warps(kind) * kOutBytes) + 1024;
 }
 // The tensor core's fp32 additions truncate: the 80 of a contraction of 1280 leave logits 1.3e-6 (bf16) or 2.4e-6 (fp16)
-// of their size short. For the loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
+// of their size short. The gradient, whose logits are rounded to 16 bits as probabilities next, leaves it at that. For the
+// loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
 // those segments rounding to nearest: below 8e-7 for any contraction. The tensor core is at the next segment meanwhile;
 // shorter ones leave it idle during a tile's exponentials (16381 rows: none 1265 us, 10 1355, 7 1466, 4 1850).
 template <typename T>
@@ -375,7 +377,9 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
         }
-        if (direct) {  // dW added to what is there
+        // dW added to what is there, 16 bytes a thread: 211 rows (fp16) 262 us against 125 that write, 8189 rows 2710 to 2750
+        // against 2620 to 2700.
+        if (direct) {
           if (row < a.width) {
             uint4* dst =
                 reinterpret_cast<uint4*>(static_cast<T*>(a.dw) + (static_cast<int64_t>(a.v0) + row) * a.hidden + col);

@@ -13,7 +13,9 @@
 // and two CTAs share an SM, so that the softmax of one fills the waits of the other. The running maximum moves only when
 // a row exceeds it by 2^8, so O is seldom rescaled. What bounds it: 128 x 128 exponentials take twice as long as the
 // tile's two products of depth 64; an eighth of them run on the FMA pipe instead. Six sequences up to 4096, 32 heads on 8 (bf16):
-// 235 us, 0.66 PFLOP/s, the special-function unit 45% and the tensor pipe 25% active: the softmax warps' own chain.
+// 235 to 248 us as the clocks allow, 0.62 to 0.66 PFLOP/s, the special-function unit 45% and the tensor pipe 25% active, 39%
+// of issue slots: the latency of the softmax warps' own chain. (Moving the maximum only past a threshold and exponentials on
+// the FMA pipe are published techniques.)
 // Few rows (serving): the keys are split over several CTAs, whose partial results prompt_join_kernel joins; where there
 // are so few that tiles would be empty, prompt_few_kernel takes the place of the tensor core.
 #include "fw_prompt.cuh"

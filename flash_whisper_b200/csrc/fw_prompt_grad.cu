@@ -17,11 +17,11 @@
 // the step after the next once P and dS are there: a step's hand-overs hide behind the exponentials. Steps run on across
 // items: the loads and the first products of the next item start while the results of the last one are read out (with one
 // CTA per item 24 CTAs an SM spent 8 us each outside of their steps).
-// Six sequences up to 4096, 32 heads on 8 (bf16): 611 us, 0.63 PFLOP/s of what the formulas need, the special-function
-// unit 46% and the tensor pipe 40% active. Tried and slower: steps of 64 with two sets of X and Y and 8 warps on each
-// (693), all products from one warp (674: its waits add to the products' time), A in tensor memory with P and dS over Y
-// (715), the two halves of the warps taking turns at the exponentials (667), a quarter of the exponentials as polynomials
-// on the FMA pipe (no change).
+// Six sequences up to 4096, 32 heads on 8 (bf16): 611 to 691 us as the clocks allow, 0.56 to 0.63 PFLOP/s of what the
+// formulas need, the special-function unit 46% and the tensor pipe 40% active. Tried and slower (611 on that box): steps of 64
+// with two sets of X and Y and 8 warps on each (693), all products from one warp (674: its waits add to the products' time), A
+// in tensor memory with P and dS over Y (715), the two halves of the warps taking turns at the exponentials (667), a quarter of
+// the exponentials as polynomials on the FMA pipe (no change).
 // fp16 range: P is kept times 2^8, and dS times 2^6 over the powers of two of the largest |v| (of the call) and the largest
 // |do| (of the row in a query item, of the call in a key item), so that gradients of any size keep their bits and none
 // overflows: |do . v - delta| is at most 2 x 64 times the two, so what is kept stays below 2^15. bf16 needs neither.

@@ -84,8 +84,9 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 }
 
 // 2^x of two numbers on the FMA pipe, for kernels that the special-function unit (16 results a cycle and SM) bounds.
-// x = n + f with n the nearest integer, 2^f by a polynomial of degree 5 fitted for the least relative error on
-// [-1/2, 1/2] (7.5e-8), times 2^n. x at most 127; below -126.5 the result is 0; NaN stays.
+// x = n + f with n the nearest integer, 2^f by a polynomial of degree 5 fitted for a small relative error on [-1/2, 1/2]
+// (1.5e-7 with these coefficients, 2.2e-7 with fp32's roundings), times 2^n. x at most 127; below -126.5 the result is 0; NaN
+// stays.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));

@@ -366,7 +366,7 @@ class Ext:
 
     def embed_grad(self, dout, ids, dembed, scale=1.0, padding_idx=-1, accumulate=False, ws=None):
         """dembed[v] = (dembed[v] if accumulate) + scale * sum of dout[i] over ids[i] == v != padding_idx, summed in
-        fp32 in the order of i. With ids = positions and scale 1 it is the position table's gradient."""
+        fp32 in an order that only the ids decide. With ids = positions and scale 1 it is the position table's gradient."""
         dtype, dev, n = dembed.dtype, dembed.get_device(), ids.numel()
         _check(dtype in _DTYPES, 'dembed must be fp16, bf16 or fp32')
         _check_typed(dembed, dtype, dev, 'dembed')

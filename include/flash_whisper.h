@@ -396,7 +396,8 @@ int fw_embed_scaled(const void* embed, const void* pos_embed, const int64_t* ids
 
 /* Gradient of fw_embed_scaled with respect to embed (or, with ids = positions and scale 1, to pos_embed):
  * dembed[v] = [dembed[v] +] scale * sum over i with ids[i] == v of dout[i], for every v < vocab. The sum
- * runs in fp32 in the order of i (tokens are sorted, no atomics: the result is the same in every run).
+ * runs in fp32, over parts of the tokens in the order of i, then over the parts in order (tokens are sorted, no
+ * atomics: the result is the same in every run).
  * accumulate 0 writes every row (zero where no token names it); 1 adds to dembed and touches only the
  * rows that tokens name. Tokens equal to padding_idx (-1: none) are left out; ids out of range are left
  * out and set FW_DEVERR_BAD_INDEX. n and vocab at most 2^30, rows of at most 65535 * 1280 bytes. */
@@ -437,7 +438,8 @@ int fw_prompt_attention_workspace(int64_t rows_q, int64_t rows_k, int seqs, int 
 /* Gradient of fw_prompt_attention: dq, dk and dv for dout (all as the forward's rows), from its out and lse.
  * dk and dv are summed over the heads of a group in a fixed order (no atomics: results do not vary from run
  * to run). Every row of a sequence is written (0 where nothing is seen), rows of no sequence are left as
- * they are and what they hold reaches no result. Between the products, the probabilities and their
+ * they are and what they hold reaches no result (a NaN or infinity within a sequence reaches rows of its own that
+ * share a tile, masked or not). Offsets as in the forward pass. Between the products, the probabilities and their
  * gradients are rounded to 16 bits (in fp16 scaled by powers of two, so that small gradients keep their bits and
  * none overflows: what lies below 2^-31 of the largest |v| of the call times the largest |do|, of its row for dq,
  * of the call for dk, may be lost); sums are fp32. */
@@ -464,7 +466,7 @@ int fw_lm_head_loss_workspace(int n, int vocab, int64_t* bytes);
  * dh = dz . w and dw = [dw +] dz^T . h (accumulate 1 adds to dw, as the tied embedding's gradient needs).
  * lse is fw_lm_head_loss's for the same h and w, g fp32 [n] (1 / count for a mean). dh or dw may be NULL.
  * Ignored rows have dh = 0 and leave dw alone, whatever h and g hold there. The logits are recomputed in
- * pieces of the vocabulary; exp(z - lse) - [..] is rounded to 16 bits between the products (scaled by 2^12
+ * pieces of the vocabulary, as plain fp32 tensor-core sums; exp(z - lse) - [..] is rounded to 16 bits between the products (scaled by 2^12
  * in fp16), which run in fp32, and so is h times g over the largest |g| for dw (in fp16 taken up to 2^15 by a power
  * of two: what lies below 2^-39 of the largest |h g| is lost); dh and dw have the type of h and w. No atomics:
  * results do not vary from run to run. */
