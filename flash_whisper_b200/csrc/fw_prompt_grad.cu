@@ -17,14 +17,15 @@
 // the step after the next once P and dS are there: a step's hand-overs hide behind the exponentials. Steps run on across
 // items: the loads and the first products of the next item start while the results of the last one are read out (with one
 // CTA per item 24 CTAs an SM spent 8 us each outside of their steps).
-// Six sequences up to 4096, 32 heads on 8 (bf16): 611 to 691 us as the clocks allow, 0.56 to 0.63 PFLOP/s of what the
+// Six sequences up to 4096, 32 heads on 8 (bf16): 611 to 704 us as the clocks allow, 0.55 to 0.63 PFLOP/s of what the
 // formulas need, the special-function unit 46% and the tensor pipe 40% active. Tried and slower (611 on that box): steps of 64
 // with two sets of X and Y and 8 warps on each (693), all products from one warp (674: its waits add to the products' time), A
 // in tensor memory with P and dS over Y (715), the two halves of the warps taking turns at the exponentials (667), a quarter of
 // the exponentials as polynomials on the FMA pipe (no change).
-// fp16 range: P is kept times 2^8, and dS times 2^6 over the powers of two of the largest |v| (of the call) and the largest
-// |do| (of the row in a query item, of the call in a key item), so that gradients of any size keep their bits and none
-// overflows: |do . v - delta| is at most 2 x 64 times the two, so what is kept stays below 2^15. bf16 needs neither.
+// fp16 range: P is kept times 2^8, and dS times 2^12 over the powers of two of the largest norm ||v|| (of the call) and of
+// ||do|| (of the row in a query item, the largest of the call in a key item), so that gradients of any size keep their bits and
+// none overflows: |do . v - delta| is at most twice the product of the norms, so what is kept stays below 2^15. (The largest
+// elements bound it too, but 64 times as far off where one element is large.) bf16 needs neither.
 #include "fw_prompt.cuh"
 
 namespace fw {
@@ -47,8 +48,8 @@ struct GradArgs {
   // time; a sequence's rows start at stat_start()
   float* stat;
   int64_t stat_rows;
-  float* norm;                   // fp16: [heads][stat_rows], the power of two that takes a row's largest |do| to [1, 2)
-  float* largest;                // fp16: [2][kDeltaBlocks], largest finite |do| and |v| each block met
+  float* norm;                   // fp16: [heads][stat_rows], the power of two that takes a row's ||do|| to [1, 2)
+  float* largest;                // fp16: [2][kDeltaBlocks], largest ||do||^2 and ||v||^2 each block met
   unsigned* next;                // the next work item to be drawn
   int64_t key_items, all_items;  // key items come first: they are the longer ones
   float scale;
@@ -61,10 +62,10 @@ __device__ __forceinline__ float* stat_at(const GradArgs& g, int head, int64_t r
   return g.stat + (head * g.stat_rows + row / 4 * 4) * 2 + row % 4;
 }
 
-// The power of two that takes x into [1, 2); 1 for 0, and within what fp32 holds.
+// The power of two that takes the root of x, a sum of squares of fp16 numbers, into [1, 2); 1 for 0.
 __device__ __forceinline__ float normalizer(float x) {
-  const int e = static_cast<int>(__float_as_uint(x) >> 23);  // x >= 0 and finite
-  return e == 0 ? 1.f : __uint_as_float(static_cast<uint32_t>(min(254 - e, 227)) << 23);
+  const int e = static_cast<int>(__float_as_uint(x) >> 23) - 127;
+  return x == 0.f ? 1.f : __uint_as_float(static_cast<uint32_t>(127 - (e >> 1)) << 23);
 }
 
 // The good sequence that holds `row` of those that `cu` (cu_q or cu_k) divides, -1 for none. A warp's lanes may ask for
@@ -100,21 +101,22 @@ __device__ __forceinline__ int sequence_at(const PromptArgs& a, const int64_t* c
   return found;
 }
 
+// Sum of squares, of finite elements.
 template <typename T>
-__device__ __forceinline__ float largest_finite(uint4 v) {
+__device__ __forceinline__ float square(uint4 v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float big = 0.f;
+  float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 x = Type16<T>::unpack(w[i]);
-    if (fabsf(x.x) < INFINITY) big = fmaxf(big, fabsf(x.x));
-    if (fabsf(x.y) < INFINITY) big = fmaxf(big, fabsf(x.y));
+    if (fabsf(x.x) < INFINITY) sum = fmaf(x.x, x.x, sum);
+    if (fabsf(x.y) < INFINITY) sum = fmaf(x.y, x.y, sum);
   }
-  return big;
+  return sum;
 }
 
-// fp16: a second half of the grid looks for the largest |v| (as a second loop of the same CTAs: 51 us for eight transcripts
-// up to 448, 20 heads; so 49, and 46 without |v|).
+// fp16: a second half of the grid looks for the largest ||v|| (as a second loop of the same CTAs: 51 us for eight transcripts
+// up to 448, 20 heads; so 49, and 46 without ||v||).
 template <typename T>
 __global__ void __launch_bounds__(256, 8) prompt_delta_kernel(GradArgs g) {
   __shared__ float s_max[8];
@@ -136,7 +138,10 @@ __global__ void __launch_bounds__(256, 8) prompt_delta_kernel(GradArgs g) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (row >= 0)
         v = reinterpret_cast<const uint4*>(static_cast<const T*>(g.v) + row * g.v_token + u % a.kv_heads * g.v_head)[lane & 7];
-      if (sequence_at(a, a.cu_k, row, &ordered, lane) >= 0) big = fmaxf(big, largest_finite<T>(v));
+      float sum = sequence_at(a, a.cu_k, row, &ordered, lane) >= 0 ? square<T>(v) : 0.f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      big = fmaxf(big, sum);
     }
   } else {
     const int64_t units = a.rows_q * a.heads;
@@ -145,7 +150,7 @@ __global__ void __launch_bounds__(256, 8) prompt_delta_kernel(GradArgs g) {
       const int64_t row = u < units ? u / a.heads : -1;
       const int head = static_cast<int>(u % a.heads);
       const int seq = sequence_at(a, a.cu_q, row, &ordered, lane);  // rows of no sequence may hold anything
-      float dot = 0.f, row_big = 0.f;
+      float dot = 0.f, sum = 0.f;
       if (seq >= 0) {
         const uint4 d =
             reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + row * g.d_token + head * g.d_head)[lane & 7];
@@ -156,20 +161,20 @@ __global__ void __launch_bounds__(256, 8) prompt_delta_kernel(GradArgs g) {
           const float2 x = Type16<T>::unpack(dw[i]), y = Type16<T>::unpack(ow[i]);
           dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
         }
-        if (!Type16<T>::kBf16) row_big = largest_finite<T>(d);
+        if (!Type16<T>::kBf16) sum = square<T>(d);
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) {
         dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        row_big = fmaxf(row_big, __shfl_xor_sync(0xffffffffu, row_big, o));
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-      big = fmaxf(big, row_big);
+      big = fmaxf(big, sum);
       if (seq >= 0 && (lane & 7) == 0) {
         const int64_t q0 = a.cu_q[seq], at = stat_start(q0, seq) + row - q0;
         float* st = stat_at(g, head, at);
         st[0] = kP - a.lse[head * a.rows_q + row] * kLog2;
         st[4] = -dot;
-        if (!Type16<T>::kBf16) g.norm[head * g.stat_rows + at] = normalizer(row_big);
+        if (!Type16<T>::kBf16) g.norm[head * g.stat_rows + at] = normalizer(sum);
       }
     }
   }
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       a_full[2], a_free[2], done, item_full[kRing], item_free[kRing];
   __shared__ uint32_t tmem_base_sh;
   __shared__ GradItem s_item[kRing];
-  __shared__ float s_norm, s_norm_v;  // powers of two for the call's largest |do| and |v|, the second for the latter alone
+  __shared__ float s_norm, s_norm_v;  // powers of two for the call's largest ||do|| and ||v||, the second for the latter alone
   const PromptArgs& a = g.p;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -601,13 +606,13 @@ __global__ void __launch_bounds__(kGradThreads, 1)
       gr.c = a.scale_log2;
       gr.off = gr.del = 0.f;
       gr.norm = 1.f;  // the factor of dS besides P's
-      if (!Type16<T>::kBf16 && keys) gr.norm = 0.25f * s_norm;
+      if (!Type16<T>::kBf16 && keys) gr.norm = 16.f * s_norm;
       if (!keys && live) {
         const int64_t at = stat_start(it.q0, it.seq) + token;
         const float* st = stat_at(g, head, at);
         gr.off = st[0];
         gr.del = st[4];
-        if (!Type16<T>::kBf16) gr.norm = 0.25f * s_norm_v * g.norm[head * g.stat_rows + at];
+        if (!Type16<T>::kBf16) gr.norm = 16.f * s_norm_v * g.norm[head * g.stat_rows + at];
       }
       gr.tx = tmem + lanes + 32 * grp;
       gr.ty = tmem + lanes + 256 + 32 * grp;

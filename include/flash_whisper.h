@@ -441,8 +441,8 @@ int fw_prompt_attention_workspace(int64_t rows_q, int64_t rows_k, int seqs, int 
  * they are and what they hold reaches no result (a NaN or infinity within a sequence reaches rows of its own that
  * share a tile, masked or not). Offsets as in the forward pass. Between the products, the probabilities and their
  * gradients are rounded to 16 bits (in fp16 scaled by powers of two, so that small gradients keep their bits and
- * none overflows: what lies below 2^-31 of the largest |v| of the call times the largest |do|, of its row for dq,
- * of the call for dk, may be lost); sums are fp32. */
+ * none overflows: what lies below 2^-37 of the largest norm of a row of v in the call times that of do, of its row
+ * for dq, the largest of the call for dk, may be lost); sums are fp32. */
 int fw_prompt_attention_grad(const fw_rows_t* q, const fw_rows_t* k, const fw_rows_t* v, const fw_rows_t* out,
                              const fw_rows_t* dout, const float* lse, const int64_t* cu_q, const int64_t* cu_k,
                              int seqs, int64_t rows_q, int64_t rows_k, int heads, int kv_heads, float scale, int causal,

@@ -4,6 +4,8 @@ values near the ends of fp16. Tolerances are those of test_gpu_prompt.py, test_g
 import pytest
 import torch
 
+from tests.test_gpu_loss import _check_grad as _check_loss_grad
+from tests.test_gpu_loss import _inputs
 from tests.test_gpu_prompt import _check, _cu, _make
 from tests.test_gpu_prompt_grad import _check_grad, _run, _within
 
@@ -247,3 +249,33 @@ def test_embedding_of_nearly_2_31_tokens(ext):
     assert ext.device_error() == 0
     assert out[-6:, 0].tolist() == [0, 4, 6, 8, 10, 12] and float(out[1 << 30]) == 2.0
     assert float(out.float().sum()) == 42.0
+
+
+@pytest.mark.parametrize('size', [100.0, 3000.0, 30000.0])
+def test_prompt_attention_grad_with_one_large_value(ext, size):
+    """fp16: one element of v far above the rest. The other sequence's ds is off by half a subnormal step more, 2^-37 ||do||
+    ||v||, below 2^-18 at 30000; the bound's p e_delta, with e_delta about 2^-6 here, covers that for p above 2^-12, and
+    scores of about +-1 over 90 keys leave hardly one below."""
+    lens = [90, 140]
+    q, k, v = _make(lens, lens, 4, 2, 'fp16', fused=False)
+    dout = torch.randn(q.shape, device='cuda').half()
+    v[200, 1, 7] = size
+    cu = _cu(lens)
+    grads = _run(ext, q, k, v, dout, cu, cu, 0.125, True)[2]
+    assert ext.device_error() == 0 and all(bool(x.isfinite().all()) for x in grads)
+    _check_grad(q, k, v, dout, grads, lens, lens, 0.125, True)
+    first = slice(0, 90)
+    _check_grad(q[first], k[first], v[first], dout[first], [x[first] for x in grads], lens[:1], lens[:1], 0.125, True)
+
+
+@pytest.mark.parametrize('n,vocab,hidden', [(300, 2000, 256), (70, 777, 72)])
+def test_loss_grad_accumulates_in_fp16(ext, n, vocab, hidden):
+    """dw added to what is there, by unequal weights whose copy of h is scaled."""
+    h, w, targets = _inputs(n, vocab, hidden, 'fp16')
+    loss, lse, g = torch.empty(n, device='cuda'), torch.empty(n, device='cuda'), torch.rand(n, device='cuda') * 3e-3
+    ext.lm_head_loss(h, w, targets, loss, lse)
+    base = torch.randn(vocab, hidden, device='cuda').half()
+    dw = base.clone()
+    ext.lm_head_loss_grad(h, w, targets, lse, g, None, dw, accumulate=True)
+    _check_loss_grad(h, w, targets, g, lse, None, dw, base=base)
+    assert ext.device_error() == 0
