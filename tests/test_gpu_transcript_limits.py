@@ -279,3 +279,28 @@ def test_loss_grad_accumulates_in_fp16(ext, n, vocab, hidden):
     ext.lm_head_loss_grad(h, w, targets, lse, g, None, dw, accumulate=True)
     _check_loss_grad(h, w, targets, g, lse, None, dw, base=base)
     assert ext.device_error() == 0
+
+
+@pytest.mark.parametrize('longer', [1, 50])
+def test_prompt_attention_many_tokens_with_bad_offsets_among_them(ext, longer):
+    """More sequences than the join looks at in one go, some of them prompts, with a bad one in the middle and rows of no
+    sequence in front and behind: keys are split, every good sequence is computed."""
+    lens = [1] * 200
+    lens[20] = lens[160] = longer
+    n, lk, bad = sum(lens), 300, 90
+    at_q, at_k = _cu(lens) + 7, torch.arange(201, device='cuda') * lk
+    q, k, v = _make([n + 30], [200 * lk], 2, 1, 'fp16', fused=False)
+    cu_q = at_q.clone()
+    cu_q[bad + 1] = 1 << 40  # its end and the next one's begin
+    assert ext.prompt_attention_workspace(n + 30, 200 * lk, 200, 2, 1) > 0
+    out, lse = torch.full_like(q, 3.0), torch.full((2, n + 30), 3.0, device='cuda')
+    ws = torch.full((ext.prompt_attention_workspace(n + 30, 200 * lk, 200, 2, 1),), 255, dtype=torch.uint8, device='cuda')
+    ext.device_error()
+    ext.prompt_attention(q, k, v, out, cu_q, at_k, 0.125, lse=lse, ws=ws)
+    assert ext.device_error() == 2
+    left = torch.ones(n + 30, dtype=torch.bool, device='cuda')
+    for first, end, size in ((0, bad, lens[:bad]), (bad + 2, 200, lens[bad + 2:])):
+        rq, rk = slice(int(at_q[first]), int(at_q[end])), slice(first * lk, end * lk)
+        _check(q[rq], k[rk], v[rk], out[rq], lse[:, rq], size, [lk] * len(size), 0.125, True)
+        left[rq] = False
+    assert bool((out[left] == 3).all()) and bool((lse[:, left] == 3).all())
