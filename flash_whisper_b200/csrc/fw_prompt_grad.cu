@@ -89,7 +89,8 @@ __device__ __forceinline__ int sequence_at(const PromptArgs& a, const int64_t* c
   if (__any_sync(0xffffffffu, lost)) {
     if (*ordered < 0) {
       bool back = false;
-      for (int b = lane; b < a.seqs; b += 32) back = back || cu[b] > cu[b + 1];
+#pragma unroll 8
+      for (int b = lane; b < a.seqs; b += 32) back |= cu[b] > cu[b + 1];
       *ordered = !__any_sync(0xffffffffu, back);
     }
     if (lost && !*ordered) {
