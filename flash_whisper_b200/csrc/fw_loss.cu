@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
         }
-        // dW added to what is there, 16 bytes a thread: 211 rows (fp16) 262 us against 125 that write, 8189 rows 2710 to 2750
-        // against 2620 to 2700.
+        // dW added to what is there, 16 bytes a thread: 211 rows (fp16) 262 us against 125 that write, 8189 rows 2710 to 2820
+        // against 2620 to 2760.
         if (direct) {
           if (row < a.width) {
             uint4* dst =
