@@ -18,6 +18,11 @@
 //   * gradient: the vocabulary is taken in pieces whose dz (16 bits) fits the scratch and mostly L2. Per piece one
 //     launch recomputes z and writes dz, a second one has both products of it: dh (contraction over the piece; fp32
 //     partial sums per k split, carried from piece to piece) and dW (contraction over the rows, final).
+// The target's logit is not taken from the tensor core, whose truncating sums are short by 1e-6 of it and more: where the target
+// has nearly all of the probability, that is more than the loss, and than exp(z - lse) - 1. It is a dot product of its own
+// (exact_logit), its column left out of the statistics: then the loss is log1p(others / target) and dz_t = expm1(z_t - lse), and
+// what the others' sums lack is a small part of either. (Five rows, vocabulary 226, hidden 1280, half of them sure: the gradient
+// was off by a tenth.) It costs no time: two warps beside the products in the forward pass, CTAs beside h's copy in the gradient.
 // 16-bit dz: exp(z - lse) - [v = t] lies in [-1, 1] whatever g is, so it is stored without g (times 2^12 in fp16,
 // which keeps probabilities down to 2^-36 above the smallest subnormal); g multiplies dh's rows in fp32 at the end, and
 // is folded into the 16-bit copy of h that dW's product reads, relative to the largest |g|, so that with equal
@@ -44,13 +49,14 @@ enum Kind { kStats, kDz, kGrads };  // what a launch computes
 constexpr int stages_of(int kind) { return kind == kGrads ? 5 : 6; }
 // Epilogue warps: twice as many where the products are short (dW of few rows) and the epilogue has little to compute.
 constexpr int epi_warps(int kind) { return kind == kGrads ? 16 : 8; }
-constexpr int threads_of(int kind) { return 32 * (2 + epi_warps(kind)); }
+constexpr int target_warps(int kind) { return kind == kStats ? 2 : 0; }
+constexpr int threads_of(int kind) { return 32 * (2 + epi_warps(kind) + target_warps(kind)); }
 constexpr int smem_of(int kind) {
   return stages_of(kind) * kStageBytes + (kind == kStats ? 0 : epi_warps(kind) * kOutBytes) + 1024;
 }
 // The tensor core's fp32 additions truncate: the 80 of a contraction of 1280 leave logits 1.3e-6 (bf16) or 2.4e-6 (fp16)
-// of their size short. The gradient, whose logits are rounded to 16 bits as probabilities next, leaves it at that. For the
-// loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
+// of their size short. The gradient, whose logits (but the targets') are rounded to 16 bits as probabilities next, leaves it at that. For
+// the loss, an fp32 result, it adds up at most 10 or 7 k blocks at a time, and the epilogue adds
 // those segments rounding to nearest: below 8e-7 for any contraction. The tensor core is at the next segment meanwhile;
 // shorter ones leave it idle during a tile's exponentials (16381 rows: none 1265 us, 10 1355, 7 1466, 4 1850).
 template <typename T>
@@ -68,7 +74,9 @@ struct LossArgs {
   const int64_t* targets;
   const float* lse;
   float2* stats;             // [2 * all n tiles][n]
-  float* target_logit;       // [n]
+  float *target_logit, *target_rest;  // [n], kStats
+  const void *h, *w;         // kStats
+  const float* target_dz;    // [n], kDz: what dz is at the target
   void* dz;                  // [n][ld_dz]
   int64_t ld_dz;
   float dz_scale;            // the factor stored with dz
@@ -78,6 +86,58 @@ struct LossArgs {
   int first_piece, accumulate;
   bool chunks;               // MN-major maps over [hidden / 64][rows][64]; hidden is a multiple of 64
 };
+
+// A row that counts: its target is a vocabulary row and not the one to be ignored.
+__device__ __forceinline__ bool counts(int64_t target, int64_t ignore, int vocab) {
+  return target >= 0 && target < vocab && target != ignore;
+}
+
+// x + y as a number and what its rounding lost (Knuth's two-sum), the latter added to what was lost before.
+__device__ __forceinline__ float2 add_exact(float2 x, float2 y) {
+  const float t = x.x + y.x, back = t - x.x;
+  return make_float2(t, ((x.x - (t - back)) + (y.x - back)) + (x.y + y.y));
+}
+
+// h . w by one warp, as a number and a rest: 256 sums of a few terms each in fp32, which round to nearest (1280 terms: five
+// each, off by 5 x 2^-24 of their size at most, and by a sixteenth of 2^-23 of the whole together as a rule), added up with
+// the rests. (With 64-bit sums beside the products: 1575 us for 16381 rows, 1590 if all sums are, in place of 1546.)
+template <typename T>
+__device__ __forceinline__ float2 exact_logit(const T* h, const T* w, int hidden, int lane) {
+  float acc[8] = {};
+#pragma unroll 4
+  for (int i = lane; i < hidden / 8; i += 32) {
+    const uint4 x = reinterpret_cast<const uint4*>(h)[i], y = reinterpret_cast<const uint4*>(w)[i];
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = Type16<T>::unpack(xw[j]), b = Type16<T>::unpack(yw[j]);
+      acc[2 * j] = fmaf(a.x, b.x, acc[2 * j]);
+      acc[2 * j + 1] = fmaf(a.y, b.y, acc[2 * j + 1]);
+    }
+  }
+  float2 sum = make_float2(acc[0], 0.f);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) sum = add_exact(sum, make_float2(acc[j], 0.f));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    sum = add_exact(sum, make_float2(__shfl_xor_sync(0xffffffffu, sum.x, o), __shfl_xor_sync(0xffffffffu, sum.y, o)));
+  if (!(fabsf(sum.x) < INFINITY)) sum.y = 0.f;  // infinities leave a NaN there
+  return sum;
+}
+// Rows first, first + step, ...: the logits of their targets.
+template <typename T>
+__device__ __forceinline__ void target_logits(const LossArgs& a, int first, int step, int lane) {
+  for (int row = first; row < a.n; row += step) {
+    const int64_t t = a.targets[row];
+    if (!counts(t, a.ignore, a.vocab)) continue;
+    const float2 z = exact_logit(static_cast<const T*>(a.h) + static_cast<int64_t>(row) * a.hidden,
+                                 static_cast<const T*>(a.w) + t * a.hidden, a.hidden, lane);
+    if (lane == 0) {
+      a.target_logit[row] = z.x;
+      a.target_rest[row] = z.y;
+    }
+  }
+}
 
 struct Tile {
   int m0, n0, kb0, kbs;
@@ -267,6 +327,8 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
       }
       if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
     }
+  } else if (warp >= 2 + epi_warps(kKind)) {  // kStats, beside the products
+    target_logits<T>(a, blockIdx.x * target_warps(kKind) + warp - 2 - epi_warps(kKind), gridDim.x * target_warps(kKind), lane);
   } else {
     // Warp w reads tensor-memory lanes 32 (w % 4) .. + 31 (one row of the tile per thread) and columns
     // kCols ((w - 2) / 4) .. + kCols - 1. dz, dW and dh's sums go through 4 KB of shared memory a warp (rows of 128
@@ -284,13 +346,14 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
       const int row = row0 + lane;
       const int c0 = x.n0 + kCols * part;
       int64_t target = -1;  // relative to this launch's vocabulary piece
-      float neg_lse = 0.f;
+      float neg_lse = 0.f, target_dz = 0.f;
       bool kept = false;
       if (kKind != kGrads && row < a.n) {
         const int64_t tg = a.targets[row];
-        kept = tg != a.ignore && tg >= 0 && tg < a.vocab;
-        target = tg - a.v0;
+        kept = counts(tg, a.ignore, a.vocab);
+        if (kept) target = tg - a.v0;
         if (kKind == kDz) neg_lse = -a.lse[row] * kLog2e;
+        if (kKind == kDz && kept) target_dz = a.target_dz[row];
       }
       if (kKind == kStats) {
         float z[128];
@@ -324,15 +387,15 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
           for (int j = 0; j < 128; ++j)
             if (c0 + j >= a.width) z[j] = -INFINITY;
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], z[j]), z[j + 1]);
-        if (target >= c0 && target < c0 + 128) {
+        if (target >= c0 && target < c0 + 128) {  // joined by loss_combine_kernel
           const int at = static_cast<int>(target) - c0;
 #pragma unroll
           for (int j = 0; j < 128; ++j)
-            if (j == at) a.target_logit[row] = z[j];
+            if (j == at) z[j] = -INFINITY;
         }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 128; j += 2) mx[(j >> 1) & 3] = fmaxf(fmaxf(mx[(j >> 1) & 3], z[j]), z[j + 1]);
         // the maximum in powers of two, rounded once: the sum is relative to exactly this number
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
         const float off = top == -INFINITY ? 0.f : -top;
@@ -370,7 +433,7 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
           const int at = target >= col && target < col + 32 ? static_cast<int>(target) - col : -1;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float p = ex2(fmaf(__uint_as_float(r[j]), kLog2e, neg_lse)) - (j == at ? 1.f : 0.f);
+            const float p = j == at ? target_dz : ex2(fmaf(__uint_as_float(r[j]), kLog2e, neg_lse));
             r[j] = __float_as_uint(kept ? p * a.dz_scale : 0.f);
           }
         } else if (!wide) {
@@ -461,7 +524,7 @@ __global__ void __launch_bounds__(threads_of(kKind), 1) __cluster_dims__(2, 1, 1
 // join, W at 4.9 TB/s (copies of 32 rows 37; in tiles of 256 rows 42; 64 rows 35, and 35 to 37 there). A thread owns a
 // vocabulary row of each tile: it keeps maximum and sum of every row of h over its tiles by itself, and the CTA joins its
 // 128 threads once, at the end.
-constexpr int kFewRows = 64, kFewStages = 6, kFewThreads = 32 * 6;
+constexpr int kFewRows = 64, kFewStages = 6, kFewThreads = 32 * 7;
 constexpr uint32_t few_stage(int rows) { return kHalfBytes + rows * 128; }
 constexpr int few_smem(int rows) { return kFewStages * few_stage(rows) + 1024; }
 
@@ -497,7 +560,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   }
   for (int i = threadIdx.x; i < kN; i += kFewThreads) {
     const int64_t t = i < a.n ? a.targets[i] : -1;
-    s_target[i] = t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
+    s_target[i] = counts(t, a.ignore, a.vocab) ? static_cast<int>(t) : -1;
   }
   tc_fence_before();
   __syncthreads();
@@ -554,6 +617,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       }
     }
     if (!ok && lane == 0) loss_flag(FW_DEVERR_TIMEOUT);
+  } else if (warp == 6) {
+    target_logits<T>(a, blockIdx.x, gridDim.x, lane);
   } else {
     const int q = warp & 3, mine = q * 32 + lane;  // this thread's vocabulary row of a tile
     float top[kN], sum[kN];
@@ -584,7 +649,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
       if (mine < box && v + mine < v1) {
 #pragma unroll
         for (int c = 0; c < kN; ++c) {
-          if (s_target[c] == v + mine) a.target_logit[c] = z[c];
+          if (s_target[c] == v + mine) z[c] = -INFINITY;  // joined by loss_combine_kernel
           // maxima in powers of two, rounded once: the sum is relative to exactly this number
           const float m = fmaxf(top[c], z[c] * kLog2e), off = m == -INFINITY ? 0.f : -m;
           sum[c] = sum[c] * ex2(top[c] + off) + ex2(fmaf(z[c], kLog2e, off));
@@ -631,8 +696,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 constexpr int kCombineThreads = 1024;
 __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const float2* __restrict__ stats, int halves,
                                                                        int n, const int64_t* __restrict__ targets,
-                                                                       int64_t ignore, int vocab, float* loss,
-                                                                       float* __restrict__ lse) {
+                                                                       int64_t ignore, int vocab, float* loss, float* lse) {
   constexpr int kWarps = kCombineThreads / 32;
   __shared__ float2 s_part[kWarps][32];
   pdl_wait();
@@ -658,12 +722,24 @@ __global__ void __launch_bounds__(kCombineThreads) loss_combine_kernel(const flo
   float s = 0.f;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) s += s_part[w][lane].y * ex2(s_part[w][lane].x + off);
-  const float l = m == -INFINITY ? logf(s) : fmaf(m, kLn2, logf(s));
   const int64_t t = targets[row];
-  const bool bad = t != ignore && (t < 0 || t >= vocab);
-  if (bad) loss_flag(FW_DEVERR_BAD_INDEX);
+  if (t != ignore && (t < 0 || t >= vocab)) loss_flag(FW_DEVERR_BAD_INDEX);
+  float l, nll = 0.f;
+  if (!counts(t, ignore, vocab)) {
+    l = m == -INFINITY ? logf(s) : fmaf(m, kLn2, logf(s));
+  } else {
+    const float z = loss[row], rest = lse[row];  // held the target's logit, which is not among the others
+    const float gap = fmaf(-rest, kLog2e, fmaf(-z, kLog2e, m));  // how far the others' maximum is above it, in powers of two
+    if (gap > 0.f) {
+      l = fmaf(m, kLn2, logf(s + ex2(-gap)));
+      nll = (l - z) - rest;
+    } else {
+      nll = log1pf(s * ex2(gap));
+      l = z + (rest + nll);
+    }
+  }
   lse[row] = l;
-  loss[row] = t == ignore || bad ? 0.f : l - loss[row];  // held the target's logit
+  loss[row] = nll;
 }
 
 constexpr int kScaleThreads = 256, kRangeBlocks = 592;
@@ -691,7 +767,7 @@ __global__ void __launch_bounds__(kScaleThreads) loss_range_kernel(const half* _
     const int64_t t = targets[row];
     const float w = fabsf(g[row]);
     const uint4 v = reinterpret_cast<const uint4*>(h)[i];
-    if (t < 0 || t >= vocab || t == ignore || !(w < INFINITY)) continue;
+    if (!counts(t, ignore, vocab) || !(w < INFINITY)) continue;
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
     big = fmaxf(big, w);
 #pragma unroll
@@ -707,16 +783,29 @@ __global__ void __launch_bounds__(kScaleThreads) loss_range_kernel(const half* _
 }
 
 // Gradient, before the products: h scaled by g relative to the largest finite |g| of the rows that count, zero in rows that
-// do not. bf16: each CTA finds that |g| by itself from L2. fp16: loss_range_kernel has, and the power of two that takes the
+// do not; further CTAs (from `blocks` on) have what dz is at the rows' targets. bf16: each CTA finds that |g| by itself from L2. fp16: loss_range_kernel has, and the power of two that takes the
 // largest |h g| to [2^14, 2^15) besides (1 at least, 2^24 at most). *unscale takes both back.
 template <typename T>
 __global__ void __launch_bounds__(kScaleThreads) loss_scale_kernel(const T* __restrict__ h, const float* __restrict__ g,
                                                          const int64_t* __restrict__ targets, int64_t ignore,
                                                          int vocab, int n, int hidden, T* __restrict__ scaled,
                                                          float* __restrict__ unscale, const float2* __restrict__ range,
-                                                         int ranges) {
+                                                         int ranges, int blocks, const T* __restrict__ w,
+                                                         const float* __restrict__ lse, float* __restrict__ target_dz) {
   __shared__ float s_max[2][kScaleThreads / 32];
   pdl_trigger();
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    const int lane = threadIdx.x & 31;
+    for (int row = (blockIdx.x - blocks) * (kScaleThreads / 32) + (threadIdx.x >> 5); row < n;
+         row += (gridDim.x - blocks) * (kScaleThreads / 32)) {
+      const int64_t t = targets[row];
+      if (!counts(t, ignore, vocab)) continue;
+      const float2 z = exact_logit(h + static_cast<int64_t>(row) * hidden, w + t * hidden, hidden, lane);
+      if (lane == 0) target_dz[row] = expm1f((z.x - lse[row]) + z.y);
+    }
+    if (!Type16<T>::kBf16) pdl_wait();
+    return;
+  }
   float m = 0.f, up = 1.f;
   if (Type16<T>::kBf16 || blockIdx.x == 0) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -748,13 +837,12 @@ __global__ void __launch_bounds__(kScaleThreads) loss_scale_kernel(const T* __re
   if (blockIdx.x == 0 && threadIdx.x == 0) *unscale = m / up;
   const int packs = hidden / 8;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < static_cast<int64_t>(n) * packs;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+       i += static_cast<int64_t>(blocks) * blockDim.x) {
     const int row = static_cast<int>(i / packs);
-    const int64_t t = targets[row];
-    const bool counts = t >= 0 && t < vocab && t != ignore;
-    const float f = counts ? g[row] / m * up : 0.f;
+    const bool kept = counts(targets[row], ignore, vocab);
+    const float f = kept ? g[row] / m * up : 0.f;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (counts) {
+    if (kept) {
       v = reinterpret_cast<const uint4*>(h)[i];
       uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
@@ -778,9 +866,8 @@ __global__ void __launch_bounds__(256) loss_dh_kernel(const float* __restrict__ 
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= static_cast<int64_t>(n) * packs) return;
   const int row = static_cast<int>(i / packs);
-  const int64_t t = targets[row];
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (t >= 0 && t < vocab && t != ignore) {
+  if (counts(targets[row], ignore, vocab)) {
     float acc[8] = {};
     const float4* src = reinterpret_cast<const float4*>(part) + 2 * i;
     const int64_t step = static_cast<int64_t>(n) * packs * 2;
@@ -824,7 +911,8 @@ static LossLayout loss_layout(int n, int vocab) {
 
 struct GradLayout {
   int pieces, width, splits;  // width: columns of a piece, a multiple of the tile
-  int64_t range, dz, part, total;  // offsets (range: loss_scale_kernel's factor, then loss_range_kernel's results); all bytes
+  // offsets (range: loss_scale_kernel's factor, then loss_range_kernel's results; target: dz at the targets); all bytes
+  int64_t range, target, dz, part, total;
 };
 
 // Time of a piece of `c` vocabulary tiles, in k blocks of the CTA pair that has the most to do (tiles are dealt out in turn,
@@ -871,7 +959,8 @@ static GradLayout grad_layout(int n, int vocab, int hidden) {
     }
   }
   l.range = up(static_cast<int64_t>(n) * hidden * 2, 256);
-  l.dz = l.range + up((1 + kRangeBlocks) * static_cast<int64_t>(sizeof(float2)), 256);
+  l.target = l.range + up((1 + kRangeBlocks) * static_cast<int64_t>(sizeof(float2)), 256);
+  l.dz = l.target + up(static_cast<int64_t>(n) * 4, 256);
   l.part = l.dz + up(static_cast<int64_t>(n) * l.width * 2, 256);
   l.total = l.part + static_cast<int64_t>(l.splits) * n * hidden * 4;
   return l;
@@ -964,7 +1053,10 @@ static int run_loss(const void* h, const void* w, const int64_t* targets, float*
   a.ignore = ignore;
   a.targets = targets;
   a.stats = static_cast<float2*>(ws);
-  a.target_logit = loss;  // replaced by the loss when the halves are joined
+  a.target_logit = loss;  // replaced by the results when the halves are joined
+  a.target_rest = lse;
+  a.h = h;
+  a.w = w;
   int rc = make_map(&tb, Type16<T>::kMap, w, hidden, vocab, hidden, l.share > 0 ? l.box : 128);
   if (rc) return rc;
   if (l.share > 0) {
@@ -988,6 +1080,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
   T* scaled = reinterpret_cast<T*>(b);
   float* unscale = reinterpret_cast<float*>(b + l.range);
   float2* range = reinterpret_cast<float2*>(b + l.range) + 1;
+  float* target_dz = reinterpret_cast<float*>(b + l.target);
   void* dz = b + l.dz;
   float* part = reinterpret_cast<float*>(b + l.part);
   const float dz_scale = Type16<T>::kBf16 ? 1.f : 4096.f;
@@ -1002,9 +1095,11 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     rc = launch_status(e, "lm_head_loss_grad range");
     if (rc) return rc;
   }
-  e = launch(loss_scale_kernel<T>, dim3(static_cast<unsigned>(blocks < 4 * num_sms() ? blocks : 4 * num_sms())),
-             dim3(kScaleThreads), 0, s, !Type16<T>::kBf16, static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden,
-             scaled, unscale, static_cast<const float2*>(range), ranges);
+  const int most = 4 * num_sms(), rows = (n + kScaleThreads / 32 - 1) / (kScaleThreads / 32);
+  const int scaling = static_cast<int>(blocks < most ? blocks : most);
+  e = launch(loss_scale_kernel<T>, dim3(scaling + (rows < most ? rows : most)), dim3(kScaleThreads), 0, s, !Type16<T>::kBf16,
+             static_cast<const T*>(h), g, targets, ignore, vocab, n, hidden, scaled, unscale,
+             static_cast<const float2*>(range), ranges, scaling, static_cast<const T*>(w), lse, target_dz);
   rc = launch_status(e, "lm_head_loss_grad scale");
   CUtensorMap ta, tb, ga, gb, ga2, gb2, tz, tw, tp;
   if (!rc) rc = make_map(&ta, Type16<T>::kMap, h, hidden, n, hidden, 128);
@@ -1042,6 +1137,7 @@ static int run_loss_grad(const void* h, const void* w, const int64_t* targets, c
     a.dz = dz;
     a.ld_dz = l.width;
     a.dz_scale = dz_scale;
+    a.target_dz = target_dz;
     rc = launch_gemm<kDz, T>(ta, tb, ta, tb, tz, tz, a, a.m_tiles * a.n_tiles, s, true);
     if (rc) return rc;
     a.m_tiles = dw != nullptr ? (width + kBM - 1) / kBM : 0;

@@ -454,7 +454,7 @@ int fw_prompt_attention_grad_workspace(int64_t rows_q, int64_t rows_k, int seqs,
 /* Softmax cross entropy of rows h [n, hidden] over the vocabulary matrix w [vocab, hidden] (the tied LM
  * head), in pieces of the vocabulary on tcgen05; the logits are never stored. With z = h . w^T (fp32):
  * lse[i] = log sum_v exp(z[i, v]), loss[i] = lse[i] - z[i, targets[i]] (minus the log probability of the
- * target). Rows whose target is ignore_index have loss 0 (lse is written); a target out of range counts
+ * target; computed as log1p of the others over the target, so that it keeps its bits where the target is sure). Rows whose target is ignore_index have loss 0 (lse is written); a target out of range counts
  * as ignored and sets FW_DEVERR_BAD_INDEX. h, w: FW_F16 or FW_BF16, row-major, 16-byte aligned; loss, lse
  * fp32 [n]; hidden a multiple of 8; n and vocab at most 4194304. */
 int fw_lm_head_loss(const void* h, const void* w, const int64_t* targets, float* loss, float* lse, int n, int vocab,
@@ -466,7 +466,7 @@ int fw_lm_head_loss_workspace(int n, int vocab, int64_t* bytes);
  * dh = dz . w and dw = [dw +] dz^T . h (accumulate 1 adds to dw, as the tied embedding's gradient needs).
  * lse is fw_lm_head_loss's for the same h and w, g fp32 [n] (1 / count for a mean). dh or dw may be NULL.
  * Ignored rows have dh = 0 and leave dw alone, whatever h and g hold there. The logits are recomputed in
- * pieces of the vocabulary, as plain fp32 tensor-core sums; exp(z - lse) - [..] is rounded to 16 bits between the products (scaled by 2^12
+ * pieces of the vocabulary, as plain fp32 tensor-core sums, the targets' apart and to the last bit; exp(z - lse) - [..] is rounded to 16 bits between the products (scaled by 2^12
  * in fp16), which run in fp32, and so is h times g over the largest |g| for dw (in fp16 taken up to 2^15 by a power
  * of two: what lies below 2^-39 of the largest |h g| is lost); dh and dw have the type of h and w. No atomics:
  * results do not vary from run to run. */

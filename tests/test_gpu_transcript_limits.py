@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.test_gpu_loss import _check_grad as _check_loss_grad
-from tests.test_gpu_loss import _inputs
+from tests.test_gpu_loss import _inputs, _logit_error
 from tests.test_gpu_prompt import _check, _cu, _make
 from tests.test_gpu_prompt_grad import _check_grad, _run, _within
 
@@ -304,3 +304,52 @@ def test_prompt_attention_many_tokens_with_bad_offsets_among_them(ext, longer):
         _check(q[rq], k[rk], v[rk], out[rq], lse[:, rq], size, [lk] * len(size), 0.125, True)
         left[rq] = False
     assert bool((out[left] == 3).all()) and bool((lse[:, left] == 3).all())
+
+
+@pytest.mark.parametrize('n,vocab,hidden', [(5, 226, 1280), (40, 3001, 1280), (100, 1000, 1280), (33, 700, 4096), (300, 900, 1288)])
+@pytest.mark.parametrize('dtype', ['fp16', 'bf16'])
+def test_loss_of_rows_that_are_sure_of_their_target(ext, n, vocab, hidden, dtype):
+    """Rows that leave from 1e-1 to 1e-8 to the other tokens: the loss and p - 1 are small differences of large numbers.
+
+    The target's logit is summed in 256 parts of hidden / 256 terms in fp32 and exactly from there, off by hidden / 256 x
+    2^-24 of sum |h w| at most, the others' are off by _logit_error. The loss is log1p of
+    others / target, so relative to itself it is off by that, and by 2^-18 for the exponentials; lse is rounded to fp32 (2^-24
+    of it, once more for the sum). dz at the target is expm1(z - lse), off by lse's rounding and the relative error of what
+    is left; with an lse from elsewhere, by z's error too. Then the 16-bit roundings (see test_gpu_loss.py)."""
+    gen = torch.Generator(device='cuda').manual_seed(n + hidden)
+    t, u = (torch.float16, 2.0 ** -11) if dtype == 'fp16' else (torch.bfloat16, 2.0 ** -8)
+    w = (torch.randn(vocab, hidden, device='cuda', generator=gen) * 1.43 / hidden ** 0.5).to(t)
+    targets = torch.randint(vocab, (n,), device='cuda', generator=gen)
+    size = torch.linspace(4.0, 12.0, n, device='cuda')[:, None]
+    h = (w[targets].float() * size).to(t)
+    g = torch.full((n,), 1.0 / n, device='cuda')
+    rows = torch.arange(n, device='cuda')
+    z = h.double() @ w.double().T
+    want_lse = torch.logsumexp(z, 1)
+    others = z.clone()
+    others[rows, targets] = -float('inf')
+    left = torch.exp(torch.logsumexp(others, 1) - want_lse)  # 1 - p without the cancellation
+    want_loss = -torch.log1p(-left)
+    z_err = (hidden / 256) * 2.0 ** -24 * (h.double().abs() * w[targets].double().abs()).sum(1)
+    rel = _logit_error(h, w) * 2 + 2.0 ** -18
+    loss, lse = torch.empty(n, device='cuda'), torch.empty(n, device='cuda')
+    ext.lm_head_loss(h, w, targets, loss, lse)
+    assert bool(((loss.double() - want_loss).abs() <= want_loss * rel).all())
+    assert bool(((lse.double() - want_lse).abs() <= z_err + 2.0 ** -23 * want_lse.abs() + left * rel).all())
+    dz = torch.exp(z - want_lse[:, None])
+    dz[rows, targets] = -left
+    want_h, want_w = (dz / n) @ w.double(), (dz / n).T @ h.double()
+    for given, off in ((lse, 0.0), (want_lse.float(), z_err)):
+        dh, dw = torch.empty_like(h), torch.empty_like(w)
+        ext.lm_head_loss_grad(h, w, targets, given, g, dh, dw)
+        e = dz.abs() * (u + 1.5 * rel[:, None]) + 2.0 ** -37
+        e += dz.abs() * (z_err + 2.0 ** -22 * want_lse.abs())[:, None]  # the others have lse's error
+        e[rows, targets] += 2.0 ** -23 * want_lse.abs() + off
+        k32 = 8 * 2.0 ** -23
+        bound = (e / n) @ w.double().abs() + (dz.abs() / n) @ w.double().abs() * k32 * vocab ** 0.5 + u * want_h.abs()
+        tiny = torch.finfo(t).smallest_normal * u
+        _within(dh, want_h, bound + tiny, 'dh')
+        copy = (dz.abs() / n).T @ h.double().abs() * u if dtype == 'bf16' else 0.0  # 1 / n is the same for all: exact
+        bound = (e / n).T @ h.double().abs() + copy + (dz.abs() / n).T @ h.double().abs() * k32 * n ** 0.5 + u * want_w.abs()
+        _within(dw, want_w, bound + tiny, 'dw')
+    assert ext.device_error() == 0
