@@ -353,3 +353,23 @@ def test_loss_of_rows_that_are_sure_of_their_target(ext, n, vocab, hidden, dtype
         bound = (e / n).T @ h.double().abs() + copy + (dz.abs() / n).T @ h.double().abs() * k32 * n ** 0.5 + u * want_w.abs()
         _within(dw, want_w, bound + tiny, 'dw')
     assert ext.device_error() == 0
+
+
+def test_loss_grad_of_rows_that_are_not_numbers(ext):
+    """NaN and infinities in rows that count stay visible; other rows' dh is as it was."""
+    for t in (torch.float16, torch.bfloat16):
+        h, w, targets = _inputs(90, 700, 128, 'fp16' if t == torch.float16 else 'bf16')
+        targets.clamp_(min=0)
+        loss, lse, g = torch.empty(90, device='cuda'), torch.empty(90, device='cuda'), torch.ones(90, device='cuda')
+        ext.lm_head_loss(h, w, targets, loss, lse)
+        want, dh, dw = torch.empty_like(h), torch.empty_like(h), torch.empty_like(w)
+        ext.lm_head_loss_grad(h, w, targets, lse, g, want, None)
+        h[7, 3], h[50, 9] = float('nan'), float('inf')
+        ext.lm_head_loss(h, w, targets, loss, lse)
+        assert not bool(loss[7].isfinite()) and not bool(loss[50].isfinite())
+        ext.lm_head_loss_grad(h, w, targets, lse, g, dh, dw)
+        assert bool(dh[7].isnan().all()) and not bool(dh[50].isfinite().all()) and not bool(dw.isfinite().any())
+        rest = torch.ones(90, dtype=torch.bool, device='cuda')
+        rest[7] = rest[50] = False
+        assert torch.equal(dh[rest], want[rest])
+    assert ext.device_error() == 0
