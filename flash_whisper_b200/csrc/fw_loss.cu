@@ -12,8 +12,8 @@
 // PFLOP/s, the tensor pipe 95% active; gradient of 8189 rows 2575 to 2740 us, 1.2 PFLOP/s by the formulas, which do not count
 // the logits that are formed again; of 211 rows (fp16) 125 to 139 us, of which dW's 133 MB of stores and dh's 133 MB of loads
 // take 40 at the memory's rate and overlap little.
-//   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row and picks the
-//     target's logit; loss_combine_kernel joins the halves of all vocabulary tiles. Reads h and W, writes 8 bytes per
+//   * forward: the epilogue reduces each 128-column half tile to (max, sum of exponentials) per row, the target
+//     left out; loss_combine_kernel joins the halves of all vocabulary tiles and the target's logit. Reads h and W, writes 8 bytes per
 //     row and half tile.
 //   * gradient: the vocabulary is taken in pieces whose dz (16 bits) fits the scratch and mostly L2. Per piece one
 //     launch recomputes z and writes dz, a second one has both products of it: dh (contraction over the piece; fp32
@@ -21,8 +21,7 @@
 // The target's logit is not taken from the tensor core, whose truncating sums are short by 1e-6 of it and more: where the target
 // has nearly all of the probability, that is more than the loss, and than exp(z - lse) - 1. It is a dot product of its own
 // (exact_logit), its column left out of the statistics: then the loss is log1p(others / target) and dz_t = expm1(z_t - lse), and
-// what the others' sums lack is a small part of either. (Five rows, vocabulary 226, hidden 1280, half of them sure: the gradient
-// was off by a tenth.) It costs no time: two warps beside the products in the forward pass, CTAs beside h's copy in the gradient.
+// what the others' sums lack is a small part of either. (Five rows over 226 tokens, all of them sure: the gradient was off by a tenth.) Two warps have it beside the products in the forward pass, CTAs beside h's copy in the gradient.
 // 16-bit dz: exp(z - lse) - [v = t] lies in [-1, 1] whatever g is, so it is stored without g (times 2^12 in fp16,
 // which keeps probabilities down to 2^-36 above the smallest subnormal); g multiplies dh's rows in fp32 at the end, and
 // is folded into the 16-bit copy of h that dW's product reads, relative to the largest |g|, so that with equal
@@ -100,7 +99,8 @@ __device__ __forceinline__ float2 add_exact(float2 x, float2 y) {
 
 // h . w by one warp, as a number and a rest: 256 sums of a few terms each in fp32, which round to nearest (1280 terms: five
 // each, off by 5 x 2^-24 of their size at most, and by a sixteenth of 2^-23 of the whole together as a rule), added up with
-// the rests. (With 64-bit sums beside the products: 1575 us for 16381 rows, 1590 if all sums are, in place of 1546.)
+// the rests. (Beside the products of 16381 rows: 1560 us, without it 1548; the 256 added up in 64 bits 1575, all sums in 64
+// bits 1590.)
 template <typename T>
 __device__ __forceinline__ float2 exact_logit(const T* h, const T* w, int hidden, int lane) {
   float acc[8] = {};
