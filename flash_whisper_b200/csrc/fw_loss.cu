@@ -8,7 +8,7 @@
 // (cta_group::2, 256 x 256 tiles: each CTA stages 128 rows of A and 128 rows of B per 64-deep k block, so a tile needs a
 // third less L2 traffic than two 128 x 256 tiles), fed by TMA through a ring of 5 or 6 stages, with the accumulators of
 // two tiles in tensor memory so that the epilogue of one runs under the MMAs of the next.
-// Measured (vocabulary 51866, hidden 1280, bf16), as the clocks allow: forward of 16381 rows 1340 to 1570 us, 1.4 to 1.6
+// Measured (vocabulary 51866, hidden 1280, bf16), as the clocks allow: forward of 16381 rows 1340 to 1625 us, 1.3 to 1.6
 // PFLOP/s, the tensor pipe 95% active; gradient of 8189 rows 2575 to 2740 us, 1.2 PFLOP/s by the formulas, which do not count
 // the logits that are formed again; of 211 rows (fp16) 125 to 139 us, of which dW's 133 MB of stores and dh's 133 MB of loads
 // take 40 at the memory's rate and overlap little.
